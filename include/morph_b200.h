@@ -230,8 +230,10 @@ MB_API int mb_adamw_step_noalloc(const mb_adamw_plan* plan, const mb_finalize_op
  * 2 s). The consumers' wait for that unit expires; the CTA stops, drains its own
  * copies in flight (bounded), frees what it holds and reports MB_ERR_TIMEOUT in
  * the step state (kernel 2: the step is refused, nothing changes) or raises the
- * GEMM's error flag. One arm is consumed by one launch; kernel 0 disarms all. */
-enum { MB_FAULT_APPLY = 1, MB_FAULT_STATS = 2, MB_FAULT_GEMM = 4 };
+ * GEMM's error flag (MB_FAULT_FFN: the same of a feed-forward block product's
+ * tile or CTA `unit`, reported by mb_ffn_status). One arm is consumed by one
+ * launch; kernel 0 disarms all. */
+enum { MB_FAULT_APPLY = 1, MB_FAULT_STATS = 2, MB_FAULT_GEMM = 4, MB_FAULT_FFN = 8 };
 MB_API int mb_debug_arm_fault(int32_t kernel, int64_t unit, int64_t wait_limit_ns);
 
 /* --------------------------------------- single tensor, host scalars -- */
@@ -397,6 +399,85 @@ MB_API int mb_export_f16(const float* src, int64_t n, void* dst, uint64_t* first
  * a nonfinite value or |x| > 65504 sets *err_flag to 1 (export.py:33). */
 MB_API int mb_cast_f32(const float* src, void* dst, int32_t dst_dtype, int64_t n, int32_t check,
                        int32_t* err_flag, mb_stream_t stream);
+
+/* Activation checkpoints in 8 bits: what a layer-replaying engine keeps of a
+ * stage's input (the forward boundaries of streamtrain/engine.py:165-211).
+ * x is [rows, d] of `dtype` (MB_F32, MB_F16, MB_BF16) with row pitch ld
+ * (elements); codes [rows, d] holds E4M3FN bytes and scales
+ * [rows, ceil(d / 128)] the biased exponents s + 127 of one power-of-two scale
+ * per 128 features: s is the smallest exponent (at least -127; 0 for a zero
+ * block) with max |finite x| 2^-s <= 448, code = e4m3fn(x 2^-s) rounded to
+ * nearest even, NaN for a nonfinite x. */
+MB_API int mb_act_pack(const void* x, int32_t dtype, int64_t rows, int64_t d, int64_t ld, uint8_t* codes,
+                       uint8_t* scales, mb_stream_t stream);
+
+/* Inverse of mb_act_pack: out[r][j] = code 2^s in out_dtype (row pitch ld), exact
+ * inside the type's range and its largest finite value beyond it. */
+MB_API int mb_act_unpack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t d, void* out,
+                         int32_t out_dtype, int64_t ld, mb_stream_t stream);
+
+/* Activations of the gated feed-forward block: g sigma(g), or GELU in its tanh form. */
+#define MB_ACT_SILU 0
+#define MB_ACT_GELU_TANH 1
+
+/* One gated feed-forward block (the SwiGLU of morph/model/morph_model.py:23-28):
+ * x [tokens, d], gate and up [f, d], down [d, f], all `dtype` (MB_BF16 or
+ * MB_F16), row-major with row pitches ld (elements, multiples of 8) and 16-byte
+ * aligned bases. Products accumulate in FP32; h, dh, dg and du are rounded to
+ * `dtype` once each, as the next product's operand. */
+typedef struct mb_ffn_args {
+  int32_t dtype;
+  int32_t activation; /* MB_ACT_* */
+  int64_t tokens, d, f;
+  const void* x;
+  int64_t ldx;
+  const void* gate;
+  int64_t ld_gate;
+  const void* up;
+  int64_t ld_up;
+  const void* down; /* unused by mb_gated_linear; NULL in the backward of it */
+  int64_t ld_down;
+} mb_ffn_args;
+
+/* h = act(x gate^T) * (x up^T), [tokens, f]: one launch. */
+MB_API int mb_gated_linear(const mb_ffn_args* args, void* h, int64_t ldh, mb_stream_t stream);
+
+/* y = h down^T, [tokens, d]. The workspace (device, 16-byte aligned) holds h for
+ * the call only. */
+MB_API size_t mb_feed_forward_workspace_bytes(int64_t tokens, int64_t f);
+MB_API int mb_feed_forward(const mb_ffn_args* args, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                           mb_stream_t stream);
+
+/* Gradients of the block, recomputing gate and up from args->x or, with codes and
+ * scales, from its 8-bit checkpoint (mb_act_pack; args->x is not read). dy is
+ * [tokens, d]; with args->down NULL the block is mb_gated_linear and dy is its
+ * output's gradient [tokens, f]. Each NULL gradient is left out; those given are
+ * overwritten (tokens == 0: weight gradients become zero). dx [tokens, d], dgate
+ * and dup [f, d], ddown [d, f]. */
+typedef struct mb_ffn_grads {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const void* dy;
+  int64_t lddy;
+  void* dx;
+  int64_t lddx;
+  void* dgate;
+  int64_t ld_dgate;
+  void* dup;
+  int64_t ld_dup;
+  void* ddown;
+  int64_t ld_ddown;
+} mb_ffn_grads;
+
+MB_API size_t mb_feed_forward_backward_workspace_bytes(int64_t tokens, int64_t d, int64_t f, int32_t from_codes,
+                                                       int32_t with_down);
+MB_API int mb_feed_forward_backward(const mb_ffn_args* args, const mb_ffn_grads* grads, void* workspace,
+                                    size_t workspace_bytes, mb_stream_t stream);
+
+/* Waits for the current device and reports whether a block kernel gave up one of
+ * its bounded waits since the last call: MB_ERR_TIMEOUT (its outputs are not
+ * valid) or MB_OK. Not for use during stream capture. */
+MB_API int mb_ffn_status(void);
 
 #ifdef __cplusplus
 }

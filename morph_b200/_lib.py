@@ -28,7 +28,8 @@ MB_ERR_TOO_LARGE = 9
 MB_F32, MB_F16, MB_BF16, MB_NONE = 0, 1, 2, 3
 MB_MUON_MAX_BATCH = 64
 
-MB_FAULT_APPLY, MB_FAULT_STATS, MB_FAULT_GEMM = 1, 2, 4
+MB_FAULT_APPLY, MB_FAULT_STATS, MB_FAULT_GEMM, MB_FAULT_FFN = 1, 2, 4, 8
+MB_ACT_SILU, MB_ACT_GELU_TANH = 0, 1
 
 MB_FIN_LOSS_SCALE = 1
 MB_FIN_GATE = 2
@@ -79,6 +80,17 @@ class HostScalars(ctypes.Structure):
     _fields_ = [(n, _f) for n in ("cwd", "omb1", "beta2", "omb2", "bc2s", "eps", "nss", "scale", "coef")]
 
 
+class FfnArgs(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("activation", _i32), ("tokens", _i64), ("d", _i64), ("f", _i64), ("x", _p),
+                ("ldx", _i64), ("gate", _p), ("ld_gate", _i64), ("up", _p), ("ld_up", _i64), ("down", _p),
+                ("ld_down", _i64)]
+
+
+class FfnGrads(ctypes.Structure):
+    _fields_ = [("codes", _p), ("scales", _p), ("dy", _p), ("lddy", _i64), ("dx", _p), ("lddx", _i64),
+                ("dgate", _p), ("ld_dgate", _i64), ("dup", _p), ("ld_dup", _i64), ("ddown", _p), ("ld_ddown", _i64)]
+
+
 assert ctypes.sizeof(Segment) == 64 and ctypes.sizeof(Group) == 32
 assert ctypes.sizeof(StepState) == 96 and ctypes.sizeof(FinalizeOpts) == 32
 
@@ -100,6 +112,14 @@ SIGNATURES = {
     "mb_cast_f32": (ctypes.c_int, [_p, _p, _i32, _i64, _i32, _p, _p]),
     "mb_fp8_pack": (ctypes.c_int, [_p, _i64, _p, _p, _p]),
     "mb_fp8_unpack": (ctypes.c_int, [_p, _p, _i64, _p, _i32, _p]),
+    "mb_act_pack": (ctypes.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _p]),
+    "mb_act_unpack": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _i32, _i64, _p]),
+    "mb_gated_linear": (ctypes.c_int, [_p, _p, _i64, _p]),
+    "mb_feed_forward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "mb_feed_forward": (ctypes.c_int, [_p, _p, _i64, _p, ctypes.c_size_t, _p]),
+    "mb_feed_forward_backward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i32, _i32]),
+    "mb_feed_forward_backward": (ctypes.c_int, [_p, _p, _p, ctypes.c_size_t, _p]),
+    "mb_ffn_status": (ctypes.c_int, []),
     "mb_offload_rows_step": (ctypes.c_int, [_p, _p, _p, _i64, _i64, _p, _i64, _p, _i32, _p, _p, _p, _i64, _p, _p,
                                             _p, _p]),
     "mb_stream_wait": (ctypes.c_int, [_p, _i64]),

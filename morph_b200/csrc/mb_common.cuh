@@ -245,7 +245,7 @@ int gemm16(const GemmCall& call, cudaStream_t stream);
 // Test-only fault injection (mb_debug_arm_fault): the next launch of the named
 // kernel in this process takes the armed plan; every other launch gets
 // {unit -1, the default wait bound}.
-enum { kFaultApply = 1, kFaultStats = 2, kFaultGemm = 4 };
+enum { kFaultApply = 1, kFaultStats = 2, kFaultGemm = 4, kFaultFfn = 8 };
 void take_fault(int kernel, int64_t* unit, uint64_t* limit_ns);
 
 // Host-side validation of a fused AdamW plan and of finalize options (MB_OK or

@@ -1,6 +1,7 @@
 // Test-only fault injection for the bounded device waits.
 //
-// Kernels 1 and 2 (bulk-staged forms) and the kernel-4 GEMM wait on mbarriers
+// Kernels 1 and 2 (bulk-staged forms), the kernel-4 GEMM and the feed-forward
+// block's kernels wait on mbarriers
 // for the copies their producer issues; every such wait gives up after a bound
 // (about 2 s by default), raises the CTA's abort flag, waits (bounded) for its
 // own copies in flight, frees what it holds and reports MB_ERR_TIMEOUT (or the
@@ -25,7 +26,7 @@ struct Armed {
 };
 
 std::mutex g_fault_mu;
-Armed g_armed[3];                   // kFaultApply, kFaultStats, kFaultGemm
+Armed g_armed[4];                   // kFaultApply, kFaultStats, kFaultGemm, kFaultFfn
 std::atomic<int> g_any_armed{0};
 
 int slot_of(int kernel) {
@@ -33,6 +34,7 @@ int slot_of(int kernel) {
     case kFaultApply: return 0;
     case kFaultStats: return 1;
     case kFaultGemm: return 2;
+    case kFaultFfn: return 3;
     default: return -1;
   }
 }

@@ -1,0 +1,1090 @@
+// Gated feed-forward block: forward and backward on the sm_100a tensor cores.
+//
+//   g = x Wg^T   u = x Wu^T   h = act(g) * u   y = h Wd^T
+//   x [T, d], Wg and Wu [f, d], Wd [d, f], 16-bit (BF16 or FP16), FP32 accumulation
+//   act(g) = g sigma(z): z = g (SiLU) or z = 2 sqrt(2/pi) (g + 0.044715 g^3) (GELU,
+//   tanh form: 0.5 (1 + tanh w) = sigma(2 w))
+// and, from x (or its 8-bit checkpoint, restored exactly into 16 bits first):
+//   dh = dy Wd          g, u recomputed, s = sigma(z)
+//   dg = dh u (s + g s (1 - s) z')      du = dh act(g)      h again for dWd
+//   dx = dg Wg + du Wu   dWg = dg^T x   dWu = du^T x   dWd = dy^T h
+// Everything between the products stays in FP32 registers; h, dh, dg and du are
+// rounded once to 16 bits because they are the next product's tensor-core operand.
+//
+// Two kernels do every product:
+//
+// k_ffn_pair (T > kSkinnyTokens, and all weight gradients): the CTA-pair tcgen05
+// form of mb_gemm.cu's header (256 x 256 output tile over two SMs, M = 256,
+// TMA-fed ring, two TMEM accumulators so that a tile's epilogue overlaps the next
+// tile's MMAs), with
+//   * operands read in the layout they have: K-major, or MN-major where the
+//     contraction runs over rows (dh, dx, dW), so that nothing is transposed;
+//   * gate and up as the two halves of one tile's B operand: the even CTA loads 128
+//     gate rows, the odd one the same 128 up rows, so a lane's TMEM row holds g in
+//     columns 0-127 and u of the same features in 128-255, and h (or dg, du, h from
+//     the dh tile, which TMA brings in meanwhile) is formed where they lie;
+//   * dx as one contraction over both (dg, Wg) and (du, Wu): one accumulator;
+//   * dWg and dWu as one launch;
+//   * stores through swizzled shared tiles and TMA, which clips ragged edges.
+// Tiles run in groups of kGroupM row tiles, so that what the ~74 pairs read at one
+// time (about 8 x 9 tiles' operands) stays in L2.
+//
+// k_ffn_skinny (T <= kSkinnyTokens): weights are the MMA's M side (128 rows per
+// CTA), tokens its N side (16 .. 256), so each weight is read once and the kernel is
+// a stream over them, bound by HBM up to ~150 tokens. Clusters of 1-8 CTAs split the
+// contraction; their FP32 partials are summed over distributed shared memory in
+// rank order (no atomics, no workspace, the same result every run).
+//
+// Waits are bounded as in mb_gemm.cu: on expiry a CTA raises the device's error word
+// (mb_ffn_status), waits (bounded) for its own copies, frees TMEM and returns.
+#include <atomic>
+#include <mutex>
+
+#include "mb_async.cuh"
+#include "mb_common.cuh"
+#include "mb_tc.cuh"
+
+namespace mb {
+
+int act_unpack(const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t d, void* out, int out_dtype,
+               int64_t ld, cudaStream_t st);
+
+namespace ffn {
+
+__device__ int32_t g_ffn_err;
+
+constexpr int BM = 128, BN = 256, BK = 64;
+constexpr int kFeat = BN / 2;  // features of a gated tile (gate | up halves)
+constexpr int kPairThreads = 192;
+constexpr int kTileA = BM * BK * 2;         // 16 KiB: this CTA's rows of A
+constexpr int kTileB = (BN / 2) * BK * 2;   // 16 KiB: this CTA's half of B
+constexpr int kBox = 64 * 64 * 2;           // 8 KiB: one 64 x 64 MN-major box
+constexpr int kStoreTile = 32 * 64 * 2;     // 4 KiB: a warp's 32 rows x 64 columns
+constexpr int kGroupM = 8;
+constexpr int kBarBytes = 512;
+constexpr uint32_t kTmemCols = 512;
+
+enum Epi { kPlain = 0, kGated = 1, kGatedBwd = 2 };
+
+// Ring stages and per-epilogue-warp store tiles. The backward epilogue holds the
+// two dh chunks of a tile (rewritten in place as h) beside dg and du.
+template <int kEpi> constexpr int stages() { return kEpi == kGatedBwd ? 5 : 6; }
+template <int kEpi> constexpr int store_tiles() { return kEpi == kGatedBwd ? 4 : 2; }
+template <int kEpi> constexpr int pair_smem() {
+  return 1024 + stages<kEpi>() * (kTileA + kTileB) + 4 * store_tiles<kEpi>() * kStoreTile + kBarBytes;
+}
+static_assert(pair_smem<kPlain>() <= 232448 && pair_smem<kGatedBwd>() <= 232448, "shared memory of one SM");
+
+struct Maps {
+  CUtensorMap a[2], b[2];  // K segments, problems, or (b) gate and up
+  CUtensorMap o[3];        // outputs (kGatedBwd: dg, du, h)
+  CUtensorMap dh;          // kGatedBwd input
+};
+
+struct PairArgs {
+  int M, N;       // output rows and columns (gated: features)
+  int kb;         // 64-deep blocks of one K segment
+  int nseg;       // K segments accumulated into one output (dx: 2)
+  int nprob;      // problems of one launch along M (weight gradients: up to 2)
+  int mt, nt;     // tiles of one problem
+  int act;
+  int want_h;     // kGatedBwd: store h
+  FaultPlan fault;  // test-only: a tile whose first k-block is withheld, and the launch's wait bound
+};
+
+// ------------------------------------------------------------- primitives --
+
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+      : "memory");
+}
+
+// Completes on the barrier at cluster address `bar` (the even CTA's); no multicast.
+__device__ __forceinline__ void load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
+
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int kLeft> __device__ __forceinline__ void store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Instruction descriptor (kind::f16): FP32 accumulator, A and B of one 16-bit type
+// (bits 7, 10: 1 = BF16), bits 15 / 16 set for an MN-major A / B, N >> 3, M >> 4.
+__device__ __forceinline__ uint32_t idesc(bool f16, bool a_mn, bool b_mn, int m, int n) {
+  const uint32_t t = f16 ? 0u : 1u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+// Shared-memory descriptors of 128-byte-swizzled tiles (layout type 2 at bits
+// 61-63, version 1 at bits 46-47), offsets in 16-byte units.
+// K-major: rows of 64 elements (128 B), 8-row groups 1024 B apart (SBO); a 16-deep
+// slice is 32 B further.
+// MN-major: boxes of 64 (MN) x 64 (K), one K index per 128-byte row: 8-K groups
+// 1024 B apart (SBO), the next 64 MN elements one box further (LBO); a 16-deep
+// slice is 16 rows = 2048 B further.
+template <bool kMn>
+__device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, int slice) {
+  const uint32_t a = saddr + (uint32_t)slice * (kMn ? 2048u : 32u);
+  const uint64_t lbo = kMn ? (uint64_t)(kBox >> 4) : 1u;
+  return (uint64_t)((a & 0x3FFFFu) >> 4) | (lbo << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// ------------------------------------------------------------- arithmetic --
+
+// sigma(z) in FP32; exp(-z) of a very negative z is infinite and sigma 0.
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+
+// Past |g| = 64 sigma(z) is 0 or 1 to the last bit of FP32; stopping there keeps g^3
+// finite, so that z' times a zero is not a NaN.
+__device__ __forceinline__ float gelu_arg(float g) { return fminf(fmaxf(g, -64.0f), 64.0f); }
+
+__device__ __forceinline__ float act_z(float g, int act) {
+  if (act == MB_ACT_SILU) return g;
+  const float c = gelu_arg(g);
+  return kGeluC * (c + kGeluA * c * c * c);
+}
+
+__device__ __forceinline__ float gated(float g, float u, int act) {
+  return g * sigmoid(act_z(g, act)) * u;
+}
+
+// dg, du and h at one element.
+__device__ __forceinline__ void gated_bwd(float g, float u, float dh, int act, float& dg, float& du, float& h) {
+  const float s = sigmoid(act_z(g, act));
+  const float c = gelu_arg(g);
+  const float zp = act == MB_ACT_SILU ? 1.0f : kGeluC * (1.0f + 3.0f * kGeluA * c * c);
+  const float a = g * s;
+  h = a * u;
+  du = dh * a;
+  dg = dh * u * (s + a * (1.0f - s) * zp);
+}
+
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (kF16) {
+    const __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  } else {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+}
+
+// 16-byte chunk `c` (0..7) of row `r` of a 128-byte-swizzled store tile.
+__device__ __forceinline__ uint4* tile_chunk(uint8_t* tile, int r, int c) {
+  return reinterpret_cast<uint4*>(tile + r * 128 + ((c ^ (r & 7)) << 4));
+}
+
+template <bool kF16>
+__device__ __forceinline__ void put_row(uint8_t* tile, int r, int c0, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *tile_chunk(tile, r, c0 + c) = make_uint4(pack2<kF16>(v[8 * c], v[8 * c + 1]), pack2<kF16>(v[8 * c + 2], v[8 * c + 3]),
+                                              pack2<kF16>(v[8 * c + 4], v[8 * c + 5]), pack2<kF16>(v[8 * c + 6], v[8 * c + 7]));
+}
+
+// ------------------------------------------------------------ pair kernel --
+
+// Tile t -> (problem, row tile, column tile): groups of kGroupM row tiles, row
+// tiles fastest inside a group.
+__device__ __forceinline__ void tile_of(const PairArgs& g, int t, int& prob, int& bm, int& bn) {
+  const int per = g.mt * g.nt;
+  prob = t / per;
+  t -= prob * per;
+  const int grp = t / (kGroupM * g.nt);
+  const int first = grp * kGroupM;
+  const int rows = g.mt - first < kGroupM ? g.mt - first : kGroupM;
+  const int in = t - first * g.nt;
+  bm = first + in % rows;
+  bn = in / rows;
+}
+
+template <int kEpi, bool kAMn, bool kBMn, bool kF16>
+__global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_constant__ Maps maps, const PairArgs g) {
+  constexpr int ST = stages<kEpi>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + ST * kTileA;
+  uint8_t* sOut = sB + ST * kTileB;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 4 * store_tiles<kEpi>() * kStoreTile);
+  uint64_t* empty = full + ST;
+  uint64_t* acc_full = empty + ST;      // [2]
+  uint64_t* acc_empty = acc_full + 2;   // [2]: one arrival per epilogue warp of both CTAs
+  uint64_t* drain = acc_empty + 2;
+  uint64_t* dh_full = drain + 1;        // [4]: one per epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dh_full + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int unit = (int)(blockIdx.x >> 1), n_units = (int)(gridDim.x >> 1);
+  const int total = g.nprob * g.mt * g.nt;
+  const int KB = g.kb * g.nseg;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 8);
+    }
+    mbar_init(drain, 1);
+    for (int w = 0; w < 4; ++w) mbar_init(&dh_full[w], 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int kit = 0;
+      for (int t = unit; t < total && !*abort_flag; t += n_units) {
+        int prob, bm, bn;
+        tile_of(g, t, prob, bm, bn);
+        const int arow = bm * 2 * BM + (int)rank * BM;
+        // gated tiles: 128 features from gate (even CTA) or up (odd CTA)
+        const int brow = kEpi == kPlain ? bn * BN + (int)rank * (BN / 2) : bn * kFeat;
+        for (int kb = 0; kb < KB; ++kb, ++kit) {
+          const int s = kit % ST;
+          if (!mbar_wait(&empty[s], ((kit / ST) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
+          if (t == g.fault.unit && kb == 0) continue;  // test-only: withhold; the MMA warp's wait expires
+          const int seg = kb >= g.kb ? 1 : 0;
+          const int k0 = (kb - seg * g.kb) * BK;
+          const CUtensorMap* ma = &maps.a[seg + prob];
+          const CUtensorMap* mb_ = &maps.b[kEpi == kPlain ? seg : (int)rank];
+          const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
+          if (leader) mbar_expect_tx(&full[s], 2 * (kTileA + kTileB));
+          uint8_t* a = sA + s * kTileA;
+          uint8_t* b = sB + s * kTileB;
+          if constexpr (kAMn) {
+            load_2d_pair(a, ma, bar, arow, k0);
+            load_2d_pair(a + kBox, ma, bar, arow + 64, k0);
+          } else {
+            load_2d_pair(a, ma, bar, k0, arow);
+          }
+          if constexpr (kBMn) {
+            load_2d_pair(b, mb_, bar, brow, k0);
+            load_2d_pair(b + kBox, mb_, bar, brow + 64, k0);
+          } else {
+            load_2d_pair(b, mb_, bar, k0, brow);
+          }
+        }
+      }
+      if (*abort_flag && leader) {
+        // bounded wait for both CTAs' loads still in flight (they land on the even CTA's barriers)
+        const uint64_t t0 = globaltimer();
+        for (int k = kit - ST > 0 ? kit - ST : 0; k < kit; ++k)
+          while (!mbar_try_wait(&full[k % ST], (k / ST) & 1) && globaltimer() - t0 < g.fault.limit_ns) {
+          }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      const uint32_t id = idesc(kF16, kAMn, kBMn, 2 * BM, BN);
+      int kit = 0, it = 0;
+      for (int t = unit; t < total && !*abort_flag; t += n_units, ++it) {
+        const int a = it & 1;
+        if (!mbar_wait_cluster(&acc_empty[a], ((it >> 1) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + (uint32_t)(a * BN);
+        for (int kb = 0; kb < KB; ++kb, ++kit) {
+          const int s = kit % ST;
+          if (!mbar_wait(&full[s], (kit / ST) & 1, abort_flag, g.fault.limit_ns)) break;
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + s * kTileA), b0 = smem_u32(sB + s * kTileB);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma_pair(acc, tile_desc<kAMn>(a0, k), tile_desc<kBMn>(b0, k), id, (kb | k) != 0 ? 1u : 0u);
+          umma_commit_both(&empty[s]);
+        }
+        // an aborted tile is not handed over: the odd CTA cannot see this CTA's abort flag
+        if (!*abort_flag) umma_commit_both(&acc_full[a]);
+      }
+      if (*abort_flag) {
+        umma_commit_pair(drain);
+        const uint64_t t0 = globaltimer();
+        while (!mbar_try_wait(drain, 0) && globaltimer() - t0 < g.fault.limit_ns) {
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3;  // TMEM lane quarter this warp may read
+    uint8_t* out = sOut + (warp - 2) * store_tiles<kEpi>() * kStoreTile;
+    uint64_t* dh_bar = &dh_full[warp - 2];
+    int it = 0, buf = 0;
+    uint32_t dh_round = 0;
+    for (int t = unit; t < total; t += n_units, ++it) {
+      const int a = it & 1;
+      int prob, bm, bn;
+      tile_of(g, t, prob, bm, bn);
+      const int row0 = bm * 2 * BM + (int)rank * BM + q * 32;
+      const int col0 = kEpi == kPlain ? bn * BN : bn * kFeat;
+      const bool rows_in = row0 < g.M;
+      bool dh_loaded = false;
+      if constexpr (kEpi == kGatedBwd) {
+        // this tile's dh: two 32 x 64 chunks, loaded while the MMAs run. The
+        // buffers' last h stores must have been read out first.
+        if (rows_in) {
+          dh_loaded = true;
+          if (lane == 0) {
+            store_wait_read<0>();
+            fence_async();
+            const bool two = col0 + 64 < g.N;
+            mbar_expect_tx(dh_bar, (two ? 2 : 1) * kStoreTile);
+            load_2d(out, &maps.dh, dh_bar, col0, row0);
+            if (two) load_2d(out + kStoreTile, &maps.dh, dh_bar, col0 + 64, row0);
+          }
+          __syncwarp();
+        }
+      }
+      int ok = 0;
+      if (lane == 0) ok = mbar_wait(&acc_full[a], (it >> 1) & 1, abort_flag, g.fault.limit_ns) && !*abort_flag;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if constexpr (kEpi == kGatedBwd) {
+        if (dh_loaded) {
+          // every lane waits: each then sees the loaded bytes. Bounded; also runs
+          // before an abort leaves, so that no copy outlives the CTA.
+          const uint64_t t0 = globaltimer();
+          bool here = false;
+          while (!(here = mbar_try_wait(dh_bar, dh_round & 1)) && globaltimer() - t0 < g.fault.limit_ns) {
+          }
+          ++dh_round;
+          if (!__all_sync(0xffffffffu, here)) {
+            *abort_flag = 1;
+            ok = 0;
+          }
+        }
+      }
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (uint32_t)(a * BN) + ((uint32_t)(q * 32) << 16);
+      if constexpr (kEpi == kPlain || kEpi == kGated) {
+        constexpr int kCols = kEpi == kPlain ? BN : kFeat;
+        for (int c = 0; c < kCols; c += 64) {
+          if (!rows_in || col0 + c >= g.N) break;  // warp-uniform
+          uint8_t* tile = out + buf * kStoreTile;
+          buf ^= 1;
+          if (lane == 0) store_wait_read<1>();  // the store before last has read this tile
+          __syncwarp();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float v[32];
+            if constexpr (kEpi == kPlain) {
+              uint32_t r[32];
+              tmem_ld32(acc + (uint32_t)(c + half * 32), r);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+            } else {
+              uint32_t rg[32], ru[32];
+              tmem_ld32_nowait(acc + (uint32_t)(c + half * 32), rg);
+              tmem_ld32(acc + (uint32_t)(kFeat + c + half * 32), ru);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = gated(__uint_as_float(rg[j]), __uint_as_float(ru[j]), g.act);
+            }
+            put_row<kF16>(tile, lane, half * 4, v);
+          }
+          fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            store_2d(&maps.o[prob], tile, col0 + c, row0);
+            store_commit();
+          }
+        }
+      } else {
+        uint8_t* tdg = out + 2 * kStoreTile;
+        uint8_t* tdu = out + 3 * kStoreTile;
+        for (int c = 0; c < kFeat; c += 64) {
+          if (!rows_in || col0 + c >= g.N) break;  // warp-uniform
+          uint8_t* tdh = out + (c >> 6) * kStoreTile;
+          if (lane == 0) store_wait_read<0>();  // dg and du of the chunk before have been read out
+          __syncwarp();
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            uint32_t rg[32], ru[32];
+            tmem_ld32_nowait(acc + (uint32_t)(c + half * 32), rg);
+            tmem_ld32(acc + (uint32_t)(kFeat + c + half * 32), ru);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4* cell = tile_chunk(tdh, lane, half * 4 + k);
+              const uint4 w = *cell;
+              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+              uint32_t og[4], ou[4], oh[4];
+#pragma unroll
+              for (int p = 0; p < 4; ++p) {
+                float dg[2], du[2], h[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float d = h2f<kF16>((uint16_t)(ww[p] >> (16 * e)));
+                  const int j = k * 8 + p * 2 + e;
+                  gated_bwd(__uint_as_float(rg[j]), __uint_as_float(ru[j]), d, g.act, dg[e], du[e], h[e]);
+                }
+                og[p] = pack2<kF16>(dg[0], dg[1]);
+                ou[p] = pack2<kF16>(du[0], du[1]);
+                oh[p] = pack2<kF16>(h[0], h[1]);
+              }
+              *tile_chunk(tdg, lane, half * 4 + k) = make_uint4(og[0], og[1], og[2], og[3]);
+              *tile_chunk(tdu, lane, half * 4 + k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+              *cell = make_uint4(oh[0], oh[1], oh[2], oh[3]);
+            }
+          }
+          fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            store_2d(&maps.o[0], tdg, col0 + c, row0);
+            store_2d(&maps.o[1], tdu, col0 + c, row0);
+            if (g.want_h) store_2d(&maps.o[2], tdh, col0 + c, row0);
+            store_commit();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[a]), 0));
+    }
+    if (lane == 0) store_wait_all();
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync();  // after every bounded wait of both CTAs
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ffn_err, 1);
+}
+
+// ---------------------------------------------------------- skinny kernel --
+
+constexpr int kSkinnyThreads = 128;
+
+struct SkinnyArgs {
+  int tokens;     // all tokens; blockIdx.y picks a tile of n
+  int n;          // tokens of a tile, padded to a multiple of 16 (MMA N)
+  int rows;       // output features
+  int kb, nseg;   // 64-deep blocks of one K segment; segments
+  int split;      // cluster CTAs sharing one tile's contraction
+  int st;         // ring stages
+  int act;
+  uint32_t tmem_cols;
+  void* o0;       // plain / gated output, or dg
+  void* o1;       // du
+  void* o2;       // h (or null)
+  const void* dh;
+  int64_t ldo, ldu, ldh, lddh;
+  FaultPlan fault;  // test-only: a CTA whose first k-block is withheld, and the launch's wait bound
+};
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int kEpi, bool kAMn, bool kF16>
+__global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_constant__ Maps maps, const SkinnyArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int tile_b = g.n * BK * 2;  // a multiple of 2048: every tile stays 1024-byte aligned
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + g.st * kTileA;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sB + g.st * tile_b);
+  uint64_t* empty = full + g.st;
+  uint64_t* acc_full = empty + g.st;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = g.split > 1 ? (int)cluster_rank() : 0;
+  const int tile = (int)blockIdx.x / g.split;
+  const int tok0 = (int)blockIdx.y * g.n;
+  const int KB = g.kb * g.nseg;
+  const int k_lo = (int)((int64_t)KB * rank / g.split), k_hi = (int)((int64_t)KB * (rank + 1) / g.split);
+  const int feat0 = tile * (kEpi == kPlain ? 128 : 64);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.st; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(g.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    int kit = 0;
+    for (int k = k_lo; k < k_hi; ++k, ++kit) {
+      const int s = kit % g.st;
+      if (!mbar_wait(&empty[s], ((kit / g.st) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
+      if ((int)blockIdx.x == g.fault.unit && kit == 0) continue;  // test-only, as in the pair kernel
+      const int seg = k >= g.kb ? 1 : 0;
+      const int k0 = (k - seg * g.kb) * BK;
+      mbar_expect_tx(&full[s], kTileA + tile_b);
+      uint8_t* a = sA + s * kTileA;
+      if constexpr (kAMn) {
+        load_2d(a, &maps.a[seg], &full[s], feat0, k0);
+        load_2d(a + kBox, &maps.a[seg], &full[s], feat0 + 64, k0);
+      } else if constexpr (kEpi == kPlain) {
+        load_2d(a, &maps.a[seg], &full[s], k0, feat0);
+        load_2d(a + kBox, &maps.a[seg], &full[s], k0, feat0 + 64);
+      } else {  // 64 gate rows, then the same 64 up rows
+        load_2d(a, &maps.a[0], &full[s], k0, feat0);
+        load_2d(a + kBox, &maps.a[1], &full[s], k0, feat0);
+      }
+      load_2d(sB + s * tile_b, &maps.b[seg], &full[s], k0, tok0);
+    }
+    if (*abort_flag) {  // bounded wait for this CTA's loads in flight
+      const uint64_t t0 = globaltimer();
+      for (int k = kit - g.st > 0 ? kit - g.st : 0; k < kit; ++k)
+        while (!mbar_try_wait(&full[k % g.st], (k / g.st) & 1) && globaltimer() - t0 < g.fault.limit_ns) {
+        }
+    }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t id = idesc(kF16, kAMn, false, 128, g.n);
+    int kit = 0;
+    for (int k = k_lo; k < k_hi; ++k, ++kit) {
+      const int s = kit % g.st;
+      if (!mbar_wait(&full[s], (kit / g.st) & 1, abort_flag, g.fault.limit_ns)) break;
+      tc_fence_after();
+      const uint32_t a0 = smem_u32(sA + s * kTileA), b0 = smem_u32(sB + s * tile_b);
+#pragma unroll
+      for (int i = 0; i < BK / 16; ++i)
+        umma_16(tmem, tile_desc<kAMn>(a0, i), tile_desc<false>(b0, i), id, (kit | i) != 0 ? 1u : 0u);
+      umma_commit(&empty[s]);
+    }
+    umma_commit(acc_full);  // also on abort: completion of every MMA issued
+  }
+  __syncwarp();
+  // Every thread waits for the last MMA: then the ring is idle and its memory holds
+  // the partials. An aborting CTA takes part in the cluster steps below and stores nothing.
+  mbar_wait(acc_full, 0, abort_flag, g.fault.limit_ns);
+  if (*abort_flag) {
+    const uint64_t t0 = globaltimer();
+    while (!mbar_try_wait(acc_full, 0) && globaltimer() - t0 < g.fault.limit_ns) {
+    }
+  }
+  __syncthreads();  // the producer's and the MMA thread's waits have ended too
+  tc_fence_after();
+  const int here = g.tokens - tok0 < g.n ? g.tokens - tok0 : g.n;
+  float* part = reinterpret_cast<float*>(smem);  // [token][128 features]
+  for (int c = 0; c < here; c += 16) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c + j < here) part[(c + j) * 128 + warp * 32 + lane] = k_hi > k_lo ? __uint_as_float(r[j]) : 0.0f;
+  }
+  tc_fence_before();
+  if (g.split > 1) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
+  }
+  if (!*abort_flag) {
+    // the tile's (token, feature) pairs, dealt to the cluster's threads; a pair's
+    // partials are added in rank order
+    constexpr int kPer = kEpi == kPlain ? 128 : 64;
+    const int items = here * kPer;
+    const uint32_t base = smem_u32(part);
+    for (int i = rank * kSkinnyThreads + (int)threadIdx.x; i < items; i += g.split * kSkinnyThreads) {
+      const int j = i / kPer, feat = i % kPer;
+      if (feat0 + feat >= g.rows) continue;
+      float v = 0.0f, w = 0.0f;
+      for (int r = 0; r < g.split; ++r) {
+        const uint32_t p = (g.split > 1 ? mapa_u32(base, (uint32_t)r) : base) + (uint32_t)(j * 128 + feat) * 4u;
+        v += ld_cluster_f32(p);
+        if constexpr (kEpi != kPlain) w += ld_cluster_f32(p + 64 * 4);
+      }
+      const int64_t tok = tok0 + j, col = feat0 + feat;
+      if constexpr (kEpi == kPlain) {
+        static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(v);
+      } else if constexpr (kEpi == kGated) {
+        static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(gated(v, w, g.act));
+      } else {
+        float dg, du, h;
+        gated_bwd(v, w, h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col]), g.act, dg, du, h);
+        static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(dg);
+        static_cast<uint16_t*>(g.o1)[tok * g.ldu + col] = f2h<kF16>(du);
+        if (g.o2 != nullptr) static_cast<uint16_t*>(g.o2)[tok * g.ldh + col] = f2h<kF16>(h);
+      }
+    }
+  }
+  if (g.split > 1) cluster_sync();  // no CTA leaves while a peer reads its partials
+  if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ffn_err, 1);
+}
+
+// ------------------------------------------------------------------ host --
+
+// 2-D 16-bit tensor [rows][cols], row pitch ld (elements); 128-byte swizzle.
+bool map_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows,
+            bool f16) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
+            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A 16-bit matrix in memory.
+struct Mat {
+  const void* p = nullptr;
+  int64_t rows = 0, cols = 0, ld = 0;
+};
+
+// One contraction: out = sum over segments of A B^T, or the gated forms of it.
+struct Product {
+  int epi = kPlain;
+  bool a_mn = false, b_mn = false;  // operand stored [K, M] / [K, N]
+  int nseg = 1, nprob = 1;
+  Mat a[2], b[2];    // gated: a[0] = x, b = gate, up
+  Mat o[3];          // outputs (kGatedBwd: dg, du, h or null)
+  Mat dh;
+  int64_t M = 0, N = 0, K = 0;  // N: features of a gated form
+  int act = 0;
+};
+
+constexpr int kMaxDevices = 64;
+
+struct KernelEntry {
+  std::once_flag once[kMaxDevices];
+  int rc[kMaxDevices];
+  int pairs[kMaxDevices];
+};
+
+int current_device(int* sms) {
+  static std::atomic<int> count[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -1;
+  int n = count[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return -1;
+    count[dev].store(n, std::memory_order_relaxed);
+  }
+  *sms = n;
+  return dev;
+}
+
+cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, dim3 grid, int threads, int smem, int cluster,
+                                  cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  if (cluster > 1) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  }
+  return cfg;
+}
+
+template <int kEpi, bool kAMn, bool kBMn, bool kF16>
+int launch_pair(const Product& q, cudaStream_t stream) {
+  auto kernel = &k_ffn_pair<kEpi, kAMn, kBMn, kF16>;
+  constexpr int smem = pair_smem<kEpi>();
+  static KernelEntry entry;  // of this instantiation
+  int sms = 0;
+  const int dev = current_device(&sms);
+  if (dev < 0) return MB_ERR_CUDA;
+  std::call_once(entry.once[dev], [&] {
+    entry.rc[dev] = MB_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return;
+    cudaLaunchAttribute at[1];
+    cudaLaunchConfig_t occ = cluster_config(at, dim3((unsigned)(2 * (sms / 2))), kPairThreads, smem, 2, nullptr);
+    int c = 0;
+    if (cudaOccupancyMaxActiveClusters(&c, kernel, &occ) != cudaSuccess || c <= 0) return;
+    entry.pairs[dev] = c;
+    entry.rc[dev] = MB_OK;
+  });
+  if (entry.rc[dev] != MB_OK) return entry.rc[dev];
+  Maps m;
+  bool ok = true;
+  const int na = kEpi == kPlain ? (q.nseg > q.nprob ? q.nseg : q.nprob) : 1;
+  const int nb = kEpi == kPlain ? q.nseg : 2;
+  for (int i = 0; i < na; ++i)
+    ok = ok && map_2d(&m.a[i], q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, kAMn ? 64 : BM, kF16);
+  for (int i = 0; i < nb; ++i)
+    ok = ok && map_2d(&m.b[i], q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, kBMn ? 64 : BN / 2, kF16);
+  for (int i = 0; i < 3; ++i)
+    if (q.o[i].p) ok = ok && map_2d(&m.o[i], q.o[i].p, q.o[i].rows, q.o[i].cols, q.o[i].ld, 64, 32, kF16);
+  if (kEpi == kGatedBwd) ok = ok && map_2d(&m.dh, q.dh.p, q.dh.rows, q.dh.cols, q.dh.ld, 64, 32, kF16);
+  if (!ok) return MB_ERR_CUDA;
+  const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), cols = kEpi == kPlain ? BN : kFeat;
+  const int64_t nt = (q.N + cols - 1) / cols;
+  const int64_t work = mt * nt * q.nprob;
+  const int64_t kb = (q.K + BK - 1) / BK;
+  if (work > ((int64_t)1 << 30) || kb * q.nseg > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+  PairArgs g{};
+  g.M = (int)q.M; g.N = (int)q.N;
+  g.kb = (int)kb; g.nseg = q.nseg; g.nprob = q.nprob;
+  g.mt = (int)mt; g.nt = (int)nt;
+  g.act = q.act; g.want_h = q.o[2].p != nullptr;
+  take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
+  const int units = (int)(work < entry.pairs[dev] ? work : entry.pairs[dev]);
+  cudaLaunchAttribute at[1];
+  cudaLaunchConfig_t cfg = cluster_config(at, dim3((unsigned)(2 * units)), kPairThreads, smem, 2, stream);
+  return cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
+}
+
+// Tokens up to which the weight-streaming kernel runs.
+constexpr int64_t kSkinnyTokens = 256;
+constexpr int kSkinnyRing = 200 * 1024;      // ring bytes of a CTA that has an SM to itself
+constexpr int kSkinnyRingHalf = 110 * 1024;  // ... of one that shares it
+constexpr int kSkinnyMaxSmem = kSkinnyRing + 1024 + kBarBytes;
+
+template <int kEpi, bool kAMn, bool kF16>
+int launch_skinny(const Product& q, cudaStream_t stream) {
+  // q is given as in the pair form (a: tokens, b: weights); the MMA swaps them
+  auto kernel = &k_ffn_skinny<kEpi, kAMn, kF16>;
+  static KernelEntry entry;
+  int sms = 0;
+  const int dev = current_device(&sms);
+  if (dev < 0) return MB_ERR_CUDA;
+  std::call_once(entry.once[dev], [&] {
+    entry.rc[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnyMaxSmem) ==
+                            cudaSuccess
+                        ? MB_OK
+                        : MB_ERR_CUDA;
+  });
+  if (entry.rc[dev] != MB_OK) return entry.rc[dev];
+  SkinnyArgs g{};
+  const int64_t T = q.M;
+  g.tokens = (int)T;
+  g.n = T >= 256 ? 256 : (int)((T + 15) / 16 * 16);
+  g.rows = (int)q.N;
+  const int64_t kb = (q.K + BK - 1) / BK;
+  if (kb * q.nseg > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+  g.kb = (int)kb; g.nseg = q.nseg;
+  const int64_t per = kEpi == kPlain ? 128 : 64;
+  const int64_t tiles = (q.N + per - 1) / per, ytiles = (T + g.n - 1) / g.n;
+  const int64_t KB = kb * q.nseg;
+  // Split the contraction until the launch has two CTAs for every SM, as long as
+  // a CTA keeps four k-blocks.
+  g.split = 1;
+  while (g.split < 8 && tiles * ytiles * g.split < 2 * sms && KB / (2 * g.split) >= 4) g.split *= 2;
+  // Two CTAs share an SM's memory while tokens are few; wide token tiles take it whole.
+  const int stage = kTileA + g.n * BK * 2;
+  const int64_t mine = (KB + g.split - 1) / g.split;
+  g.st = (g.n <= 64 ? kSkinnyRingHalf : kSkinnyRing) / stage;
+  if (g.st > mine) g.st = (int)mine;
+  const int need = g.n * 128 * 4;  // the partials reuse the ring
+  while (g.st * stage < need) ++g.st;
+  g.tmem_cols = 32;
+  while ((int)g.tmem_cols < g.n) g.tmem_cols *= 2;
+  g.act = q.act;
+  Maps m;
+  bool ok = true;
+  const int nw = kEpi == kPlain ? q.nseg : 2;
+  for (int i = 0; i < nw; ++i)
+    ok = ok && map_2d(&m.a[i], q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, 64, kF16);
+  for (int i = 0; i < q.nseg; ++i)
+    ok = ok && map_2d(&m.b[i], q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, g.n, kF16);
+  if (!ok) return MB_ERR_CUDA;
+  g.o0 = const_cast<void*>(q.o[0].p); g.ldo = q.o[0].ld;
+  g.o1 = const_cast<void*>(q.o[1].p); g.ldu = q.o[1].ld;
+  g.o2 = const_cast<void*>(q.o[2].p); g.ldh = q.o[2].ld;
+  g.dh = q.dh.p; g.lddh = q.dh.ld;
+  take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
+  if (tiles * g.split > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+  cudaLaunchAttribute at[1];
+  const int smem = g.st * stage + 1024 + kBarBytes;
+  cudaLaunchConfig_t cfg = cluster_config(at, dim3((unsigned)(tiles * g.split), (unsigned)ytiles), kSkinnyThreads, smem,
+                                          g.split, stream);
+  return cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
+}
+
+template <bool kF16>
+int run_product(const Product& q, cudaStream_t st) {
+  const bool skinny = !q.a_mn && q.M <= kSkinnyTokens;
+  if (q.epi == kGated) return skinny ? launch_skinny<kGated, false, kF16>(q, st) : launch_pair<kGated, false, false, kF16>(q, st);
+  if (q.epi == kGatedBwd)
+    return skinny ? launch_skinny<kGatedBwd, false, kF16>(q, st) : launch_pair<kGatedBwd, false, false, kF16>(q, st);
+  if (q.a_mn) return launch_pair<kPlain, true, true, kF16>(q, st);
+  if (q.b_mn) return skinny ? launch_skinny<kPlain, true, kF16>(q, st) : launch_pair<kPlain, false, true, kF16>(q, st);
+  return skinny ? launch_skinny<kPlain, false, kF16>(q, st) : launch_pair<kPlain, false, false, kF16>(q, st);
+}
+
+int product(int dtype, const Product& q, cudaStream_t st) {
+  return dtype == MB_F16 ? run_product<true>(q, st) : run_product<false>(q, st);
+}
+
+constexpr int64_t kMaxDim = (int64_t)1 << 30;
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+size_t area(int64_t rows, int64_t cols) { return ((size_t)rows * (size_t)pad8(cols) * 2 + 255) / 256 * 256; }
+
+// A caller's matrix: 16-byte aligned rows, as TMA needs them.
+int check_mat(const void* p, int64_t cols, int64_t ld) {
+  if (!p) return MB_ERR_ARG;
+  if (ld < cols) return MB_ERR_ARG;
+  if (ld % 8 || !aligned(p, 16) || ld >= ((int64_t)1 << 36)) return MB_ERR_ALIGN;
+  return MB_OK;
+}
+
+int check_args(const mb_ffn_args* a, bool need_x, bool need_down) {
+  if (!a) return MB_ERR_ARG;
+  if (a->dtype != MB_BF16 && a->dtype != MB_F16) return MB_ERR_ARG;
+  if (a->activation != MB_ACT_SILU && a->activation != MB_ACT_GELU_TANH) return MB_ERR_ARG;
+  if (a->tokens < 0 || a->d <= 0 || a->f <= 0) return MB_ERR_ARG;
+  if (a->tokens > kMaxDim || a->d > kMaxDim || a->f > kMaxDim) return MB_ERR_TOO_LARGE;
+  int rc = MB_OK;
+  if (need_x && a->tokens > 0) rc = check_mat(a->x, a->d, a->ldx);
+  if (rc == MB_OK) rc = check_mat(a->gate, a->d, a->ld_gate);
+  if (rc == MB_OK) rc = check_mat(a->up, a->d, a->ld_up);
+  if (rc == MB_OK && need_down) rc = check_mat(a->down, a->f, a->ld_down);
+  return rc;
+}
+
+Product gated_product(const mb_ffn_args* a, const Mat& x) {
+  Product q;
+  q.epi = kGated;
+  q.a[0] = x;
+  q.b[0] = {a->gate, a->f, a->d, a->ld_gate};
+  q.b[1] = {a->up, a->f, a->d, a->ld_up};
+  q.M = a->tokens; q.N = a->f; q.K = a->d;
+  q.act = a->activation;
+  return q;
+}
+
+int zero_rows(void* p, int64_t rows, int64_t cols, int64_t ld, cudaStream_t st) {
+  return cudaMemset2DAsync(p, (size_t)ld * 2, 0, (size_t)cols * 2, (size_t)rows, st) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
+}
+
+}  // namespace ffn
+}  // namespace mb
+
+using namespace mb;
+using namespace mb::ffn;
+
+extern "C" {
+
+MB_API int mb_gated_linear(const mb_ffn_args* a, void* h, int64_t ldh, mb_stream_t stream) {
+  int rc = check_args(a, true, false);
+  if (rc != MB_OK) return rc;
+  if (a->tokens == 0) return MB_OK;
+  rc = check_mat(h, a->f, ldh);
+  if (rc != MB_OK) return rc;
+  Product q = gated_product(a, {a->x, a->tokens, a->d, a->ldx});
+  q.o[0] = {h, a->tokens, a->f, ldh};
+  return product(a->dtype, q, (cudaStream_t)stream);
+}
+
+MB_API size_t mb_feed_forward_workspace_bytes(int64_t tokens, int64_t f) {
+  if (tokens <= 0 || f <= 0 || tokens > kMaxDim || f > kMaxDim) return 0;
+  return area(tokens, f);
+}
+
+MB_API int mb_feed_forward(const mb_ffn_args* a, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                           mb_stream_t stream) {
+  int rc = check_args(a, true, true);
+  if (rc != MB_OK) return rc;
+  if (a->tokens == 0) return MB_OK;
+  rc = check_mat(y, a->d, ldy);
+  if (rc != MB_OK) return rc;
+  if (!workspace || workspace_bytes < mb_feed_forward_workspace_bytes(a->tokens, a->f)) return MB_ERR_ARG;
+  if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
+  const Mat h{workspace, a->tokens, a->f, pad8(a->f)};
+  Product q = gated_product(a, {a->x, a->tokens, a->d, a->ldx});
+  q.o[0] = h;
+  rc = product(a->dtype, q, (cudaStream_t)stream);
+  if (rc != MB_OK) return rc;
+  Product p;
+  p.a[0] = h;
+  p.b[0] = {a->down, a->d, a->f, a->ld_down};
+  p.o[0] = {y, a->tokens, a->d, ldy};
+  p.M = a->tokens; p.N = a->d; p.K = a->f;
+  return product(a->dtype, p, (cudaStream_t)stream);
+}
+
+MB_API size_t mb_feed_forward_backward_workspace_bytes(int64_t tokens, int64_t d, int64_t f, int32_t from_codes,
+                                                       int32_t with_down) {
+  if (tokens <= 0 || d <= 0 || f <= 0 || tokens > kMaxDim || d > kMaxDim || f > kMaxDim) return 0;
+  return (with_down ? 3 : 2) * area(tokens, f) + (from_codes ? area(tokens, d) : 0);
+}
+
+MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r, void* workspace,
+                                    size_t workspace_bytes, mb_stream_t stream) {
+  if (!a || !r) return MB_ERR_ARG;
+  const bool from_codes = r->codes != nullptr, down = a->down != nullptr;
+  int rc = check_args(a, !from_codes, down);
+  if (rc != MB_OK) return rc;
+  const int64_t T = a->tokens, d = a->d, f = a->f;
+  if (r->dx && T > 0) rc = check_mat(r->dx, d, r->lddx);
+  if (rc == MB_OK && r->dgate) rc = check_mat(r->dgate, d, r->ld_dgate);
+  if (rc == MB_OK && r->dup) rc = check_mat(r->dup, d, r->ld_dup);
+  if (rc == MB_OK && r->ddown) rc = down ? check_mat(r->ddown, f, r->ld_ddown) : MB_ERR_ARG;
+  if (rc != MB_OK) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (T == 0) {  // sums over no tokens
+    if (r->dgate) rc = zero_rows(r->dgate, f, d, r->ld_dgate, st);
+    if (rc == MB_OK && r->dup) rc = zero_rows(r->dup, f, d, r->ld_dup, st);
+    if (rc == MB_OK && r->ddown) rc = zero_rows(r->ddown, d, f, r->ld_ddown, st);
+    return rc;
+  }
+  if (!r->dx && !r->dgate && !r->dup && !r->ddown) return MB_OK;
+  rc = check_mat(r->dy, down ? d : f, r->lddy);
+  if (rc != MB_OK) return rc;
+  if (from_codes && !r->scales) return MB_ERR_ARG;
+  if (!workspace ||
+      workspace_bytes < mb_feed_forward_backward_workspace_bytes(T, d, f, from_codes ? 1 : 0, down ? 1 : 0))
+    return MB_ERR_ARG;
+  if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t fp = pad8(f);
+  const Mat dg{ws, T, f, fp}, du{ws + area(T, f), T, f, fp};
+  Mat dh{r->dy, T, f, r->lddy}, h;
+  ws += 2 * area(T, f);
+  if (down) {
+    dh = {ws, T, f, fp};
+    h = dh;  // h takes dh's place, element by element
+    ws += area(T, f);
+  }
+  Mat x{a->x, T, d, a->ldx};
+  if (from_codes) {
+    x = {ws, T, d, pad8(d)};
+    rc = act_unpack(r->codes, r->scales, T, d, ws, a->dtype, pad8(d), st);
+    if (rc != MB_OK) return rc;
+  }
+  const Mat dy{r->dy, T, d, r->lddy};
+  if (down) {
+    Product q;
+    q.a[0] = dy;
+    q.b[0] = {a->down, d, f, a->ld_down};
+    q.b_mn = true;
+    q.o[0] = dh;
+    q.M = T; q.N = f; q.K = d;
+    rc = product(a->dtype, q, st);
+    if (rc != MB_OK) return rc;
+  }
+  {
+    Product q = gated_product(a, x);
+    q.epi = kGatedBwd;
+    q.dh = dh;
+    q.o[0] = dg; q.o[1] = du;
+    if (r->ddown) q.o[2] = h;
+    rc = product(a->dtype, q, st);
+    if (rc != MB_OK) return rc;
+  }
+  if (r->dx) {
+    Product q;
+    q.nseg = 2;
+    q.a[0] = dg; q.a[1] = du;
+    q.b[0] = {a->gate, f, d, a->ld_gate};
+    q.b[1] = {a->up, f, d, a->ld_up};
+    q.b_mn = true;
+    q.o[0] = {r->dx, T, d, r->lddx};
+    q.M = T; q.N = d; q.K = f;
+    rc = product(a->dtype, q, st);
+    if (rc != MB_OK) return rc;
+  }
+  if (r->dgate || r->dup) {
+    Product q;
+    q.a_mn = q.b_mn = true;
+    q.nprob = 0;
+    if (r->dgate) {
+      q.a[q.nprob] = dg;
+      q.o[q.nprob++] = {r->dgate, f, d, r->ld_dgate};
+    }
+    if (r->dup) {
+      q.a[q.nprob] = du;
+      q.o[q.nprob++] = {r->dup, f, d, r->ld_dup};
+    }
+    q.b[0] = x;
+    q.M = f; q.N = d; q.K = T;
+    rc = product(a->dtype, q, st);
+    if (rc != MB_OK) return rc;
+  }
+  if (r->ddown) {
+    Product q;
+    q.a_mn = q.b_mn = true;
+    q.a[0] = dy;
+    q.b[0] = h;
+    q.o[0] = {r->ddown, d, f, r->ld_ddown};
+    q.M = d; q.N = f; q.K = T;
+    rc = product(a->dtype, q, st);
+  }
+  return rc;
+}
+
+MB_API int mb_ffn_status(void) {
+  int32_t err = 0;
+  if (cudaMemcpyFromSymbol(&err, g_ffn_err, sizeof(err)) != cudaSuccess) return MB_ERR_CUDA;
+  if (err == 0) return MB_OK;
+  err = 0;
+  if (cudaMemcpyToSymbol(g_ffn_err, &err, sizeof(err)) != cudaSuccess) return MB_ERR_CUDA;
+  return MB_ERR_TIMEOUT;
+}
+
+}  // extern "C"

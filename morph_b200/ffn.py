@@ -1,0 +1,270 @@
+"""The gated feed-forward block (SwiGLU / GEGLU) on the sm_100a tensor cores,
+forward and backward, with 8-bit activation checkpoints.
+
+    h = act(x gate^T) * (x up^T)        gated_linear
+    y = h down^T                        feed_forward
+
+``x`` is [..., d]; ``gate`` and ``up`` are [f, d] and ``down`` [d, f], as
+``nn.Linear`` keeps the ``ffn.gate`` / ``ffn.up`` / ``ffn.down`` weights of
+morph/model/morph_model.py:23-28. Everything is bfloat16, or everything is
+float16; products accumulate in FP32, and h, dh and the gradients of the two
+projections' outputs are rounded to 16 bits once each.
+
+Both functions are differentiable. What they keep for the backward pass is the
+block's input only, as it is (``checkpoint="x"``) or in 8 bits
+(``checkpoint="fp8"``, ``precision.pack_activation``: 1 + 1/128 bytes per
+element); the projections are recomputed from it. The ``*_backward`` functions
+are the same backward pass for engines that replay stages themselves
+(streamtrain/engine.py:165-211): they take x or its ``(codes, scales)``.
+
+Calls run on the current stream of the tensors' device, allocate their outputs
+and workspace from torch's caching allocator and never synchronise, so they can
+be captured in a CUDA graph. Rows whose start is not 16-byte aligned (d or f not
+a multiple of 8, odd views) are copied to padded rows first.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .precision import check_activation, pack_activation
+
+ACTIVATIONS = {"silu": _lib.MB_ACT_SILU, "gelu_tanh": _lib.MB_ACT_GELU_TANH}
+CHECKPOINTS = ("x", "fp8")
+
+
+def _activation_code(activation) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
+    return ACTIVATIONS[activation]
+
+
+def _check(tensor, what, shape, like) -> None:
+    if not isinstance(tensor, torch.Tensor) or tuple(tensor.shape) != shape:
+        raise ValueError(f"{what} must be a tensor of shape {list(shape)}")
+    if tensor.dtype != like.dtype or tensor.device != like.device:
+        raise ValueError(f"{what} is {tensor.dtype} on {tensor.device}, expected {like.dtype} on {like.device}")
+
+
+def _check_weights(gate, up, down, d):
+    if not isinstance(gate, torch.Tensor) or gate.dim() != 2 or not gate.is_cuda:
+        raise ValueError("gate must be [f, d] on a CUDA device")
+    if gate.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"the block computes in bfloat16 or float16, not {gate.dtype}")
+    f = gate.shape[0]
+    if f == 0 or d == 0:
+        raise ValueError("d and f must be at least 1")
+    _check(gate, "gate", (f, d), gate)
+    _check(up, "up", (f, d), gate)
+    if down is not None:
+        _check(down, "down", (d, f), gate)
+    return f
+
+
+def _pad8(n: int) -> int:
+    return (n + 7) // 8 * 8
+
+
+def _rows(t):
+    """(tensor, pitch) of a 2-D tensor with 16-byte aligned rows: itself, or a padded copy."""
+    rows, cols = t.shape
+    ld = t.stride(0) if rows > 1 else _pad8(cols)
+    if (cols == 1 or t.stride(1) == 1) and ld >= cols and ld % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, ld
+    buf = torch.empty((rows, _pad8(cols)), dtype=t.dtype, device=t.device)
+    buf[:, :cols].copy_(t)
+    return buf, buf.shape[1]
+
+
+def _out(rows, cols, like):
+    """(buffer, pitch) for a [rows, cols] output with 16-byte aligned rows."""
+    return torch.empty((rows, _pad8(cols)), dtype=like.dtype, device=like.device), _pad8(cols)
+
+
+def _crop(buf, cols):
+    return buf if buf.shape[1] == cols else buf[:, :cols].contiguous()
+
+
+def _args(code, tokens, d, f, like, x, gate, up, down):
+    a = _lib.FfnArgs(_lib.dtype_code(like.dtype), code, tokens, d, f)
+    keep = []
+    for name, t in (("x", x), ("gate", gate), ("up", up), ("down", down)):
+        if t is not None:
+            buf, ld = _rows(t)
+            keep.append(buf)
+            setattr(a, name, buf.data_ptr())
+            setattr(a, "ldx" if name == "x" else "ld_" + name, ld)
+    return a, keep
+
+
+def _input(x, gate):
+    if not isinstance(x, torch.Tensor) or x.dim() == 0:
+        raise ValueError("x must be a tensor [..., d]")
+    if not isinstance(gate, torch.Tensor) or x.dtype != gate.dtype or x.device != gate.device:
+        raise ValueError("x and the weights must have one dtype and one device")
+    return x.shape[-1]
+
+
+def _forward(x, gate, up, down, activation):
+    code = _activation_code(activation)
+    d = _input(x, gate)
+    f = _check_weights(gate, up, down, d)
+    x2 = x.detach().reshape(-1, d)
+    tokens = x2.shape[0]
+    width = f if down is None else d
+    with torch.cuda.device(x.device):
+        a, keep = _args(code, tokens, d, f, x, x2, gate.detach(), up.detach(), None if down is None else down.detach())
+        out, ld = _out(tokens, width, x)
+        L = _lib.lib()
+        if down is None:
+            _lib.check(L.mb_gated_linear(ctypes.byref(a), out.data_ptr(), ld, _lib.stream_handle()), "gated_linear")
+        else:
+            nbytes = L.mb_feed_forward_workspace_bytes(tokens, f)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            _lib.check(L.mb_feed_forward(ctypes.byref(a), out.data_ptr(), ld, ws.data_ptr(), nbytes,
+                                         _lib.stream_handle()), "feed_forward")
+        del keep
+        return _crop(out, width).view(x.shape[:-1] + (width,))
+
+
+def _backward(grad, saved, gate, up, down, activation, needs):
+    code = _activation_code(activation)
+    if isinstance(saved, torch.Tensor):
+        d = _input(saved, gate)
+        shape, device = saved.shape, saved.device
+    else:
+        codes, scales = saved
+        check_activation(codes, scales)
+        shape, device, d = codes.shape, codes.device, codes.shape[-1]
+    f = _check_weights(gate, up, down, d)
+    if gate.device != device:
+        raise ValueError("the checkpoint and the weights are on different devices")
+    _check(grad, "the output's gradient", tuple(shape[:-1]) + (f if down is None else d,), gate)
+    if len(needs) != (3 if down is None else 4):
+        raise ValueError("needs names one truth value for x and each weight")
+    with torch.cuda.device(device):
+        g2 = grad.detach().reshape(-1, grad.shape[-1])
+        tokens = g2.shape[0]
+        x2 = saved.detach().reshape(-1, d) if isinstance(saved, torch.Tensor) else None
+        a, keep = _args(code, tokens, d, f, gate, x2, gate.detach(), up.detach(),
+                        None if down is None else down.detach())
+        g2, lddy = _rows(g2)
+        r = _lib.FfnGrads()
+        if x2 is None:
+            r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
+        r.dy, r.lddy = g2.data_ptr(), lddy
+        outs = []
+        for need, name, rows, cols in zip(needs, ("dx", "dgate", "dup", "ddown"), (tokens, f, f, d), (d, d, d, f)):
+            if not need:
+                outs.append(None)
+                continue
+            buf, ld = _out(rows, cols, gate)
+            setattr(r, name, buf.data_ptr())
+            setattr(r, "lddx" if name == "dx" else "ld_" + name, ld)
+            outs.append((buf, cols))
+        L = _lib.lib()
+        nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, x2 is None, down is not None)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _lib.check(L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), ws.data_ptr(), nbytes,
+                                              _lib.stream_handle()), "feed_forward_backward")
+        del keep
+        grads = [None if o is None else _crop(*o) for o in outs]
+        if grads[0] is not None:
+            grads[0] = grads[0].view(shape)
+        return tuple(grads)
+
+
+class _Block(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, activation, checkpoint):
+        ctx.activation, ctx.checkpoint = activation, checkpoint
+        kept = pack_activation(x) if checkpoint == "fp8" else (x,)
+        ctx.save_for_backward(gate, up, *(() if down is None else (down,)), *kept)
+        ctx.has_down = down is not None
+        return _forward(x, gate, up, down, activation)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        gate, up, *rest = ctx.saved_tensors
+        down = rest.pop(0) if ctx.has_down else None
+        saved = tuple(rest) if ctx.checkpoint == "fp8" else rest[0]
+        needs = ctx.needs_input_grad[:4 if ctx.has_down else 3]
+        grads = _backward(grad, saved, gate, up, down, ctx.activation, needs)
+        return (*grads, *([] if ctx.has_down else [None]), None, None)
+
+
+def _block(x, gate, up, down, activation, checkpoint):
+    if checkpoint not in CHECKPOINTS:
+        raise ValueError(f"checkpoint must be one of {list(CHECKPOINTS)}, not {checkpoint!r}")
+    leaves = (x, gate, up) if down is None else (x, gate, up, down)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in leaves):
+        _activation_code(activation)
+        _check_weights(gate, up, down, _input(x, gate))
+        return _Block.apply(x, gate, up, down, activation, checkpoint)
+    return _forward(x, gate, up, down, activation)
+
+
+def gated_linear(x, gate, up, activation="silu", checkpoint="x"):
+    """h = act(x gate^T) * (x up^T), [..., f], in one kernel. Differentiable;
+    ``checkpoint`` says what is kept of x for the backward pass."""
+    return _block(x, gate, up, None, activation, checkpoint)
+
+
+def gated_linear_backward(dh, x, gate, up, activation="silu", needs=(True, True, True)):
+    """(dx, dgate, dup) of ``gated_linear`` from its output's gradient ``dh``
+    [..., f]. ``x`` is the input, or the ``(codes, scales)`` of its 8-bit
+    checkpoint. An entry of ``needs`` that is false gives None."""
+    return _backward(dh, x, gate, up, None, activation, needs)
+
+
+def feed_forward(x, gate, up, down, activation="silu", checkpoint="x"):
+    """y = (act(x gate^T) * (x up^T)) down^T, [..., d]. Differentiable;
+    ``checkpoint`` says what is kept of x for the backward pass."""
+    if down is None:
+        raise ValueError("down must be a tensor")
+    return _block(x, gate, up, down, activation, checkpoint)
+
+
+def feed_forward_backward(dy, x, gate, up, down, activation="silu", needs=(True, True, True, True)):
+    """(dx, dgate, dup, ddown) of ``feed_forward`` from its output's gradient
+    ``dy`` [..., d]. ``x`` is the input, or the ``(codes, scales)`` of its 8-bit
+    checkpoint. An entry of ``needs`` that is false gives None."""
+    if down is None:
+        raise ValueError("down must be a tensor")
+    return _backward(dy, x, gate, up, down, activation, needs)
+
+
+def check(device=None) -> None:
+    """Wait for ``device`` (default: the current one) and raise TimeoutError if a
+    block kernel there gave up a bounded wait since the last check; what it wrote
+    is then not valid."""
+    with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+        torch.cuda.synchronize()
+        _lib.check(_lib.lib().mb_ffn_status(), "feed_forward")
+
+
+class GatedFeedForward(torch.nn.Module):
+    """The block as a module, with the reference's parameter names (``gate.weight``,
+    ``up.weight``, ``down.weight``: bias-free ``nn.Linear``, so ``muon.partition``
+    gives them to Muon and ``fp8_eligible`` admits them). It computes in ``dtype``;
+    FP32 masters are cast to it on the way, with gradients cast back."""
+
+    def __init__(self, d, f, activation="silu", checkpoint="x", dtype=torch.bfloat16, device=None,
+                 param_dtype=torch.float32):
+        super().__init__()
+        _activation_code(activation)
+        if checkpoint not in CHECKPOINTS:
+            raise ValueError(f"checkpoint must be one of {list(CHECKPOINTS)}, not {checkpoint!r}")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"the block computes in bfloat16 or float16, not {dtype}")
+        make = lambda i, o: torch.nn.Linear(i, o, bias=False, device=device, dtype=param_dtype)  # noqa: E731
+        self.gate, self.up, self.down = make(d, f), make(d, f), make(f, d)
+        self.activation, self.checkpoint, self.dtype = activation, checkpoint, dtype
+
+    def forward(self, x):
+        weights = (w.weight.to(self.dtype) for w in (self.gate, self.up, self.down))
+        return feed_forward(x.to(self.dtype), *weights, self.activation, self.checkpoint).to(x.dtype)

@@ -151,6 +151,72 @@ def unpack_fp8(encoded: torch.Tensor, scales: torch.Tensor, dtype=torch.float16,
     return out
 
 
+ACTIVATION_BLOCK = 128  # features per scale of an activation checkpoint
+
+
+def pack_activation(x: torch.Tensor):
+    """An activation checkpoint in 8 bits: what a layer-replaying engine keeps of
+    a stage's input between the forward pass and its replay
+    (streamtrain/engine.py:165-211).
+
+    ``x`` [..., d] is float32, float16 or bfloat16 on a CUDA device. Returns
+    ``(codes, scales)``, both uint8: E4M3FN codes of x's shape, and the biased
+    exponent (s + 127) of one power-of-two scale per 128 features of a row,
+    [..., ceil(d / 128)]. Nonfinite elements become NaN; their neighbours keep
+    their values. The relative error of a value within 2^-14 of its block's
+    largest is at most 2^-4; smaller ones round at a fixed step of their block."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("pack_activation expects a CUDA tensor")
+    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"unsupported dtype {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("pack_activation expects [..., d] with d >= 1")
+    d = x.shape[-1]
+    x = x.detach()
+    rows = x.numel() // d
+    flat = x.reshape(-1, d)
+    if rows and (flat.stride(1) != 1 and d > 1 or rows > 1 and flat.stride(0) < d):
+        flat = flat.contiguous()
+    ld = flat.stride(0) if rows > 1 else d
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(x.shape[:-1] + (-(-d // ACTIVATION_BLOCK),), dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().mb_act_pack(flat.data_ptr(), _lib.dtype_code(x.dtype), rows, d, ld, codes.data_ptr(),
+                                          scales.data_ptr(), _lib.stream_handle()), "pack_activation")
+    return codes, scales
+
+
+def check_activation(codes: torch.Tensor, scales: torch.Tensor):
+    """Raise ValueError unless (codes, scales) have the layout of ``pack_activation``."""
+    for t, what in ((codes, "codes"), (scales, "scales")):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous uint8 on a CUDA device")
+    if codes.dim() == 0 or codes.shape[-1] == 0:
+        raise ValueError("codes must be [..., d] with d >= 1")
+    if scales.device != codes.device:
+        raise ValueError("codes and scales are on different devices")
+    want = codes.shape[:-1] + (-(-codes.shape[-1] // ACTIVATION_BLOCK),)
+    if scales.shape != want:
+        raise ValueError(f"scales must be {tuple(want)}, one per {ACTIVATION_BLOCK} features of a row")
+
+
+def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:
+    """The values an activation checkpoint stands for, code * 2^s, in ``dtype``
+    (float32, float16 or bfloat16). Exact inside the type's range; a finite value
+    beyond it (float16, or next to the top of the others) restores as the largest
+    finite one."""
+    check_activation(codes, scales)
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"unsupported dtype {dtype}")
+    d = codes.shape[-1]
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    with torch.cuda.device(codes.device):
+        _lib.check(_lib.lib().mb_act_unpack(codes.data_ptr(), scales.data_ptr(), codes.numel() // d, d,
+                                            out.data_ptr(), _lib.dtype_code(dtype), d, _lib.stream_handle()),
+                   "unpack_activation")
+    return out
+
+
 def fp8_eligible(name: str) -> bool:
     """streamtrain/precision.py:20-21: the SwiGLU projections may travel as FP8."""
     return any(name.endswith(suffix) for suffix in ('ffn.gate.weight', 'ffn.up.weight', 'ffn.down.weight'))
