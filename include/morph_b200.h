@@ -423,8 +423,8 @@ MB_API int mb_act_unpack(const uint8_t* codes, const uint8_t* scales, int64_t ro
 /* One gated feed-forward block (the SwiGLU of morph/model/morph_model.py:23-28):
  * x [tokens, d], gate and up [f, d], down [d, f], all `dtype` (MB_BF16 or
  * MB_F16), row-major with row pitches ld (elements, multiples of 8) and 16-byte
- * aligned bases. Products accumulate in FP32; h, dh, dg and du are rounded to
- * `dtype` once each, as the next product's operand. */
+ * aligned bases. Products accumulate in FP32; h and the gradients of x gate^T and
+ * x up^T are rounded to `dtype` once each, as the next product's operand. */
 typedef struct mb_ffn_args {
   int32_t dtype;
   int32_t activation; /* MB_ACT_* */

@@ -8,8 +8,9 @@
 //   dh = dy Wd          g, u recomputed, s = sigma(z)
 //   dg = dh u (s + g s (1 - s) z')      du = dh act(g)      h again for dWd
 //   dx = dg Wg + du Wu   dWg = dg^T x   dWu = du^T x   dWd = dy^T h
-// Everything between the products stays in FP32 registers; h, dh, dg and du are
-// rounded once to 16 bits because they are the next product's tensor-core operand.
+// h, dg and du are rounded once to 16 bits because they are the next product's
+// tensor-core operand; dh is only read by the elementwise step, so it stays FP32
+// (rounding it too cost 0.0029 against 0.0023 relative error of the BF16 gradients).
 //
 // Two kernels do every product:
 //
@@ -64,21 +65,26 @@ constexpr int kGroupM = 8;
 constexpr int kBarBytes = 512;
 constexpr uint32_t kTmemCols = 512;
 
-enum Epi { kPlain = 0, kGated = 1, kGatedBwd = 2 };
+// What a product's epilogue does. kPlainF32: FP32 output (dh); kGatedBwd reads a
+// 16-bit dh (the caller's), kGatedBwdF32 an FP32 one.
+enum Epi { kPlain = 0, kGated = 1, kGatedBwd = 2, kPlainF32 = 3, kGatedBwdF32 = 4 };
+constexpr bool is_plain(int epi) { return epi == kPlain || epi == kPlainF32; }
+constexpr bool is_bwd(int epi) { return epi == kGatedBwd || epi == kGatedBwdF32; }
 
-// Ring stages and per-epilogue-warp store tiles. The backward epilogue holds the
-// two dh chunks of a tile (rewritten in place as h) beside dg and du.
-template <int kEpi> constexpr int stages() { return kEpi == kGatedBwd ? 5 : 6; }
-template <int kEpi> constexpr int store_tiles() { return kEpi == kGatedBwd ? 4 : 2; }
-template <int kEpi> constexpr int pair_smem() {
-  return 1024 + stages<kEpi>() * (kTileA + kTileB) + 4 * store_tiles<kEpi>() * kStoreTile + kBarBytes;
-}
-static_assert(pair_smem<kPlain>() <= 232448 && pair_smem<kGatedBwd>() <= 232448, "shared memory of one SM");
+// Ring stages and shared memory of an epilogue warp. The backward epilogue works
+// on 32 x 32 blocks: two dh blocks in flight and one block each of dg, du and h.
+constexpr int kDhBlock = 32 * 32 * 4;
+constexpr int kOutBlock = 32 * 32 * 2;
+constexpr int stages(int epi) { return is_bwd(epi) ? 5 : 6; }
+constexpr int warp_bytes(int epi) { return is_bwd(epi) ? 2 * kDhBlock + 3 * kOutBlock : 2 * kStoreTile; }
+constexpr int pair_smem(int epi) { return 1024 + stages(epi) * (kTileA + kTileB) + 4 * warp_bytes(epi) + kBarBytes; }
+static_assert(pair_smem(kPlain) <= 232448 && pair_smem(kGatedBwd) <= 232448, "shared memory of one SM");
+static_assert(warp_bytes(kGatedBwd) % 1024 % 512 == 0, "swizzled blocks stay aligned");
 
 struct Maps {
   CUtensorMap a[2], b[2];  // K segments, problems, or (b) gate and up
-  CUtensorMap o[3];        // outputs (kGatedBwd: dg, du, h)
-  CUtensorMap dh;          // kGatedBwd input
+  CUtensorMap o[3];        // outputs (backward: dg, du, h)
+  CUtensorMap dh;          // backward input
 };
 
 struct PairArgs {
@@ -88,7 +94,7 @@ struct PairArgs {
   int nprob;      // problems of one launch along M (weight gradients: up to 2)
   int mt, nt;     // tiles of one problem
   int act;
-  int want_h;     // kGatedBwd: store h
+  int want_h;     // backward: store h
   FaultPlan fault;  // test-only: a tile whose first k-block is withheld, and the launch's wait bound
 };
 
@@ -217,6 +223,11 @@ __device__ __forceinline__ void put_row(uint8_t* tile, int r, int c0, const floa
                                               pack2<kF16>(v[8 * c + 4], v[8 * c + 5]), pack2<kF16>(v[8 * c + 6], v[8 * c + 7]));
 }
 
+// The same of a 32 x 32 16-bit block (64-byte rows, 64-byte swizzle).
+__device__ __forceinline__ uint4* block_chunk(uint8_t* block, int r, int c) {
+  return reinterpret_cast<uint4*>(block + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+
 // ------------------------------------------------------------ pair kernel --
 
 // Tile t -> (problem, row tile, column tile): groups of kGroupM row tiles, row
@@ -235,19 +246,19 @@ __device__ __forceinline__ void tile_of(const PairArgs& g, int t, int& prob, int
 
 template <int kEpi, bool kAMn, bool kBMn, bool kF16>
 __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_constant__ Maps maps, const PairArgs g) {
-  constexpr int ST = stages<kEpi>();
+  constexpr int ST = stages(kEpi);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = sA + ST * kTileA;
   uint8_t* sOut = sB + ST * kTileB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 4 * store_tiles<kEpi>() * kStoreTile);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 4 * warp_bytes(kEpi));
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;      // [2]
   uint64_t* acc_empty = acc_full + 2;   // [2]: one arrival per epilogue warp of both CTAs
   uint64_t* drain = acc_empty + 2;
-  uint64_t* dh_full = drain + 1;        // [4]: one per epilogue warp
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dh_full + 4);
+  uint64_t* dh_full = drain + 1;        // [4][2]: each epilogue warp's dh blocks
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dh_full + 8);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
       mbar_init(&acc_empty[a], 8);
     }
     mbar_init(drain, 1);
-    for (int w = 0; w < 4; ++w) mbar_init(&dh_full[w], 1);
+    for (int w = 0; w < 8; ++w) mbar_init(&dh_full[w], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -290,7 +301,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
         tile_of(g, t, prob, bm, bn);
         const int arow = bm * 2 * BM + (int)rank * BM;
         // gated tiles: 128 features from gate (even CTA) or up (odd CTA)
-        const int brow = kEpi == kPlain ? bn * BN + (int)rank * (BN / 2) : bn * kFeat;
+        const int brow = is_plain(kEpi) ? bn * BN + (int)rank * (BN / 2) : bn * kFeat;
         for (int kb = 0; kb < KB; ++kb, ++kit) {
           const int s = kit % ST;
           if (!mbar_wait(&empty[s], ((kit / ST) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
@@ -298,7 +309,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
           const int seg = kb >= g.kb ? 1 : 0;
           const int k0 = (kb - seg * g.kb) * BK;
           const CUtensorMap* ma = &maps.a[seg + prob];
-          const CUtensorMap* mb_ = &maps.b[kEpi == kPlain ? seg : (int)rank];
+          const CUtensorMap* mb_ = &maps.b[is_plain(kEpi) ? seg : (int)rank];
           const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
           if (leader) mbar_expect_tx(&full[s], 2 * (kTileA + kTileB));
           uint8_t* a = sA + s * kTileA;
@@ -356,56 +367,58 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     }
   } else {
     const int q = warp & 3;  // TMEM lane quarter this warp may read
-    uint8_t* out = sOut + (warp - 2) * store_tiles<kEpi>() * kStoreTile;
-    uint64_t* dh_bar = &dh_full[warp - 2];
+    uint8_t* out = sOut + (warp - 2) * warp_bytes(kEpi);
+    uint64_t* dh_bar = &dh_full[2 * (warp - 2)];
     int it = 0, buf = 0;
-    uint32_t dh_round = 0;
+    uint32_t dh_asked = 0, dh_read = 0;  // dh blocks loaded / consumed so far
     for (int t = unit; t < total; t += n_units, ++it) {
       const int a = it & 1;
       int prob, bm, bn;
       tile_of(g, t, prob, bm, bn);
       const int row0 = bm * 2 * BM + (int)rank * BM + q * 32;
-      const int col0 = kEpi == kPlain ? bn * BN : bn * kFeat;
+      const int col0 = is_plain(kEpi) ? bn * BN : bn * kFeat;
       const bool rows_in = row0 < g.M;
-      bool dh_loaded = false;
-      if constexpr (kEpi == kGatedBwd) {
-        // this tile's dh: two 32 x 64 chunks, loaded while the MMAs run. The
-        // buffers' last h stores must have been read out first.
-        if (rows_in) {
-          dh_loaded = true;
-          if (lane == 0) {
-            store_wait_read<0>();
-            fence_async();
-            const bool two = col0 + 64 < g.N;
-            mbar_expect_tx(dh_bar, (two ? 2 : 1) * kStoreTile);
-            load_2d(out, &maps.dh, dh_bar, col0, row0);
-            if (two) load_2d(out + kStoreTile, &maps.dh, dh_bar, col0 + 64, row0);
-          }
-          __syncwarp();
+      // backward: 32-feature blocks of this warp's rows that exist
+      const int left = (g.N - col0 + 31) / 32;
+      const int blocks = is_bwd(kEpi) && rows_in ? (left < kFeat / 32 ? left : kFeat / 32) : 0;
+      auto ask_dh = [&](int j) {  // load dh block j of the tile; its buffer's readers are done
+        if (lane == 0) {
+          uint64_t* bar = &dh_bar[dh_asked & 1];
+          fence_async();
+          mbar_expect_tx(bar, kEpi == kGatedBwdF32 ? kDhBlock : kDhBlock / 2);
+          load_2d(out + (dh_asked & 1) * kDhBlock, &maps.dh, bar, col0 + 32 * j, row0);
         }
+        ++dh_asked;
+      };
+      if constexpr (is_bwd(kEpi)) {  // two blocks come in while the MMAs run
+        for (int j = 0; j < 2 && j < blocks; ++j) ask_dh(j);
       }
       int ok = 0;
       if (lane == 0) ok = mbar_wait(&acc_full[a], (it >> 1) & 1, abort_flag, g.fault.limit_ns) && !*abort_flag;
       ok = __shfl_sync(0xffffffffu, ok, 0);
-      if constexpr (kEpi == kGatedBwd) {
-        if (dh_loaded) {
-          // every lane waits: each then sees the loaded bytes. Bounded; also runs
-          // before an abort leaves, so that no copy outlives the CTA.
-          const uint64_t t0 = globaltimer();
-          bool here = false;
-          while (!(here = mbar_try_wait(dh_bar, dh_round & 1)) && globaltimer() - t0 < g.fault.limit_ns) {
-          }
-          ++dh_round;
-          if (!__all_sync(0xffffffffu, here)) {
-            *abort_flag = 1;
-            ok = 0;
-          }
-        }
-      }
       if (!ok) break;
       tc_fence_after();
       const uint32_t acc = tmem + (uint32_t)(a * BN) + ((uint32_t)(q * 32) << 16);
-      if constexpr (kEpi == kPlain || kEpi == kGated) {
+      if constexpr (kEpi == kPlainF32) {
+        for (int c = 0; c < BN; c += 32) {
+          if (!rows_in || col0 + c >= g.N) break;  // warp-uniform
+          uint8_t* tile = out + buf * kStoreTile;
+          buf ^= 1;
+          if (lane == 0) store_wait_read<1>();  // the store before last has read this tile
+          __syncwarp();
+          uint32_t r[32];
+          tmem_ld32(acc + (uint32_t)c, r);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            *tile_chunk(tile, lane, k) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+          fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            store_2d(&maps.o[prob], tile, col0 + c, row0);
+            store_commit();
+          }
+        }
+      } else if constexpr (kEpi == kPlain || kEpi == kGated) {
         constexpr int kCols = kEpi == kPlain ? BN : kFeat;
         for (int c = 0; c < kCols; c += 64) {
           if (!rows_in || col0 + c >= g.N) break;  // warp-uniform
@@ -438,57 +451,83 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
           }
         }
       } else {
-        uint8_t* tdg = out + 2 * kStoreTile;
-        uint8_t* tdu = out + 3 * kStoreTile;
-        for (int c = 0; c < kFeat; c += 64) {
-          if (!rows_in || col0 + c >= g.N) break;  // warp-uniform
-          uint8_t* tdh = out + (c >> 6) * kStoreTile;
-          if (lane == 0) store_wait_read<0>();  // dg and du of the chunk before have been read out
+        uint8_t* tdg = out + 2 * kDhBlock;
+        uint8_t* tdu = tdg + kOutBlock;
+        uint8_t* th = tdu + kOutBlock;
+        for (int j = 0; j < blocks; ++j) {
+          uint8_t* tdh = out + (dh_read & 1) * kDhBlock;
+          // every lane waits, so that each sees the loaded bytes (bounded)
+          if (!__all_sync(0xffffffffu, mbar_wait(&dh_bar[dh_read & 1], (dh_read >> 1) & 1, abort_flag,
+                                                 g.fault.limit_ns))) {
+            ok = 0;
+            break;
+          }
+          ++dh_read;
+          uint32_t rg[32], ru[32];
+          tmem_ld32_nowait(acc + (uint32_t)(32 * j), rg);
+          tmem_ld32(acc + (uint32_t)(kFeat + 32 * j), ru);
+          if (lane == 0) store_wait_read<0>();  // the block before has been read out
           __syncwarp();
-#pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            uint32_t rg[32], ru[32];
-            tmem_ld32_nowait(acc + (uint32_t)(c + half * 32), rg);
-            tmem_ld32(acc + (uint32_t)(kFeat + c + half * 32), ru);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint4* cell = tile_chunk(tdh, lane, half * 4 + k);
-              const uint4 w = *cell;
+          for (int k = 0; k < 4; ++k) {  // 8 features each
+            float dh[8];
+            if constexpr (kEpi == kGatedBwdF32) {
+#pragma unroll
+              for (int p = 0; p < 2; ++p) {
+                const uint4 w = *tile_chunk(tdh, lane, 2 * k + p);
+                dh[4 * p] = __uint_as_float(w.x); dh[4 * p + 1] = __uint_as_float(w.y);
+                dh[4 * p + 2] = __uint_as_float(w.z); dh[4 * p + 3] = __uint_as_float(w.w);
+              }
+            } else {
+              const uint4 w = *block_chunk(tdh, lane, k);
               const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-              uint32_t og[4], ou[4], oh[4];
 #pragma unroll
               for (int p = 0; p < 4; ++p) {
-                float dg[2], du[2], h[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float d = h2f<kF16>((uint16_t)(ww[p] >> (16 * e)));
-                  const int j = k * 8 + p * 2 + e;
-                  gated_bwd(__uint_as_float(rg[j]), __uint_as_float(ru[j]), d, g.act, dg[e], du[e], h[e]);
-                }
-                og[p] = pack2<kF16>(dg[0], dg[1]);
-                ou[p] = pack2<kF16>(du[0], du[1]);
-                oh[p] = pack2<kF16>(h[0], h[1]);
+                dh[2 * p] = h2f<kF16>((uint16_t)(ww[p] & 0xffffu));
+                dh[2 * p + 1] = h2f<kF16>((uint16_t)(ww[p] >> 16));
               }
-              *tile_chunk(tdg, lane, half * 4 + k) = make_uint4(og[0], og[1], og[2], og[3]);
-              *tile_chunk(tdu, lane, half * 4 + k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
-              *cell = make_uint4(oh[0], oh[1], oh[2], oh[3]);
             }
+            uint32_t og[4], ou[4], oh[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              float dg[2], du[2], h[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                gated_bwd(__uint_as_float(rg[k * 8 + p * 2 + e]), __uint_as_float(ru[k * 8 + p * 2 + e]),
+                          dh[2 * p + e], g.act, dg[e], du[e], h[e]);
+              og[p] = pack2<kF16>(dg[0], dg[1]);
+              ou[p] = pack2<kF16>(du[0], du[1]);
+              oh[p] = pack2<kF16>(h[0], h[1]);
+            }
+            *block_chunk(tdg, lane, k) = make_uint4(og[0], og[1], og[2], og[3]);
+            *block_chunk(tdu, lane, k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+            *block_chunk(th, lane, k) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
           }
           fence_async();
           __syncwarp();
           if (lane == 0) {
-            store_2d(&maps.o[0], tdg, col0 + c, row0);
-            store_2d(&maps.o[1], tdu, col0 + c, row0);
-            if (g.want_h) store_2d(&maps.o[2], tdh, col0 + c, row0);
+            const int col = col0 + 32 * j;
+            store_2d(&maps.o[0], tdg, col, row0);
+            store_2d(&maps.o[1], tdu, col, row0);
+            if (g.want_h) store_2d(&maps.o[2], th, col, row0);
             store_commit();
           }
+          if (j + 2 < blocks) ask_dh(j + 2);
         }
+        if (!ok) break;
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[a]), 0));
     }
-    if (lane == 0) store_wait_all();
+    if (lane == 0) {
+      store_wait_all();
+      // on abort: bounded wait for dh blocks still in flight
+      const uint64_t t0 = globaltimer();
+      for (; dh_read < dh_asked; ++dh_read)
+        while (!mbar_try_wait(&dh_bar[dh_read & 1], (dh_read >> 1) & 1) && globaltimer() - t0 < g.fault.limit_ns) {
+        }
+    }
     __syncwarp();
   }
   tc_fence_before();
@@ -516,7 +555,7 @@ struct SkinnyArgs {
   void* o0;       // plain / gated output, or dg
   void* o1;       // du
   void* o2;       // h (or null)
-  const void* dh;
+  const void* dh;  // FP32 (kGatedBwdF32) or 16-bit
   int64_t ldo, ldu, ldh, lddh;
   FaultPlan fault;  // test-only: a CTA whose first k-block is withheld, and the launch's wait bound
 };
@@ -546,7 +585,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   const int tok0 = (int)blockIdx.y * g.n;
   const int KB = g.kb * g.nseg;
   const int k_lo = (int)((int64_t)KB * rank / g.split), k_hi = (int)((int64_t)KB * (rank + 1) / g.split);
-  const int feat0 = tile * (kEpi == kPlain ? 128 : 64);
+  const int feat0 = tile * (is_plain(kEpi) ? 128 : 64);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.st; ++s) {
@@ -581,7 +620,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
       if constexpr (kAMn) {
         load_2d(a, &maps.a[seg], &full[s], feat0, k0);
         load_2d(a + kBox, &maps.a[seg], &full[s], feat0 + 64, k0);
-      } else if constexpr (kEpi == kPlain) {
+      } else if constexpr (is_plain(kEpi)) {
         load_2d(a, &maps.a[seg], &full[s], k0, feat0);
         load_2d(a + kBox, &maps.a[seg], &full[s], k0, feat0 + 64);
       } else {  // 64 gate rows, then the same 64 up rows
@@ -647,7 +686,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   if (!*abort_flag) {
     // the tile's (token, feature) pairs, dealt to the cluster's threads; a pair's
     // partials are added in rank order
-    constexpr int kPer = kEpi == kPlain ? 128 : 64;
+    constexpr int kPer = is_plain(kEpi) ? 128 : 64;
     const int items = here * kPer;
     const uint32_t base = smem_u32(part);
     for (int i = rank * kSkinnyThreads + (int)threadIdx.x; i < items; i += g.split * kSkinnyThreads) {
@@ -657,16 +696,21 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
       for (int r = 0; r < g.split; ++r) {
         const uint32_t p = (g.split > 1 ? mapa_u32(base, (uint32_t)r) : base) + (uint32_t)(j * 128 + feat) * 4u;
         v += ld_cluster_f32(p);
-        if constexpr (kEpi != kPlain) w += ld_cluster_f32(p + 64 * 4);
+        if constexpr (!is_plain(kEpi)) w += ld_cluster_f32(p + 64 * 4);
       }
       const int64_t tok = tok0 + j, col = feat0 + feat;
       if constexpr (kEpi == kPlain) {
         static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(v);
+      } else if constexpr (kEpi == kPlainF32) {
+        static_cast<float*>(g.o0)[tok * g.ldo + col] = v;
       } else if constexpr (kEpi == kGated) {
         static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(gated(v, w, g.act));
       } else {
         float dg, du, h;
-        gated_bwd(v, w, h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col]), g.act, dg, du, h);
+        float dh;
+        if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[tok * g.lddh + col];
+        else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col]);
+        gated_bwd(v, w, dh, g.act, dg, du, h);
         static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(dg);
         static_cast<uint16_t*>(g.o1)[tok * g.ldu + col] = f2h<kF16>(du);
         if (g.o2 != nullptr) static_cast<uint16_t*>(g.o2)[tok * g.ldh + col] = f2h<kF16>(h);
@@ -679,21 +723,23 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
 
 // ------------------------------------------------------------------ host --
 
-// 2-D 16-bit tensor [rows][cols], row pitch ld (elements); 128-byte swizzle.
-bool map_2d(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t ld, int box_cols, int box_rows,
-            bool f16) {
+// 2-D tensor [rows][cols] of `type`, row pitch ld (elements); boxes of 64 or 128
+// bytes a row, swizzled over that span.
+bool map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows, int64_t cols, int64_t ld,
+            int box_cols, int box_rows) {
   auto fn = encode_fn();
   if (!fn) return false;
+  const int elem = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * elem)};
   cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  return fn(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
-            dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            box_cols * elem == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A 16-bit matrix in memory.
+// A matrix in memory (16-bit; dh inside the backward pass: FP32).
 struct Mat {
   const void* p = nullptr;
   int64_t rows = 0, cols = 0, ld = 0;
@@ -705,7 +751,7 @@ struct Product {
   bool a_mn = false, b_mn = false;  // operand stored [K, M] / [K, N]
   int nseg = 1, nprob = 1;
   Mat a[2], b[2];    // gated: a[0] = x, b = gate, up
-  Mat o[3];          // outputs (kGatedBwd: dg, du, h or null)
+  Mat o[3];          // outputs (backward: dg, du, h or null)
   Mat dh;
   int64_t M = 0, N = 0, K = 0;  // N: features of a gated form
   int act = 0;
@@ -753,7 +799,9 @@ cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, dim3 grid, int thread
 template <int kEpi, bool kAMn, bool kBMn, bool kF16>
 int launch_pair(const Product& q, cudaStream_t stream) {
   auto kernel = &k_ffn_pair<kEpi, kAMn, kBMn, kF16>;
-  constexpr int smem = pair_smem<kEpi>();
+  constexpr int smem = pair_smem(kEpi);
+  constexpr CUtensorMapDataType t16 = kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  constexpr CUtensorMapDataType t32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   static KernelEntry entry;  // of this instantiation
   int sms = 0;
   const int dev = current_device(&sms);
@@ -771,17 +819,21 @@ int launch_pair(const Product& q, cudaStream_t stream) {
   if (entry.rc[dev] != MB_OK) return entry.rc[dev];
   Maps m;
   bool ok = true;
-  const int na = kEpi == kPlain ? (q.nseg > q.nprob ? q.nseg : q.nprob) : 1;
-  const int nb = kEpi == kPlain ? q.nseg : 2;
+  const int na = is_plain(kEpi) ? (q.nseg > q.nprob ? q.nseg : q.nprob) : 1;
+  const int nb = is_plain(kEpi) ? q.nseg : 2;
   for (int i = 0; i < na; ++i)
-    ok = ok && map_2d(&m.a[i], q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, kAMn ? 64 : BM, kF16);
+    ok = ok && map_2d(&m.a[i], t16, q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, kAMn ? 64 : BM);
   for (int i = 0; i < nb; ++i)
-    ok = ok && map_2d(&m.b[i], q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, kBMn ? 64 : BN / 2, kF16);
+    ok = ok && map_2d(&m.b[i], t16, q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, kBMn ? 64 : BN / 2);
+  constexpr bool f32_out = kEpi == kPlainF32;
   for (int i = 0; i < 3; ++i)
-    if (q.o[i].p) ok = ok && map_2d(&m.o[i], q.o[i].p, q.o[i].rows, q.o[i].cols, q.o[i].ld, 64, 32, kF16);
-  if (kEpi == kGatedBwd) ok = ok && map_2d(&m.dh, q.dh.p, q.dh.rows, q.dh.cols, q.dh.ld, 64, 32, kF16);
+    if (q.o[i].p)
+      ok = ok && map_2d(&m.o[i], f32_out ? t32 : t16, q.o[i].p, q.o[i].rows, q.o[i].cols, q.o[i].ld,
+                        f32_out || is_bwd(kEpi) ? 32 : 64, 32);
+  if (is_bwd(kEpi))
+    ok = ok && map_2d(&m.dh, kEpi == kGatedBwdF32 ? t32 : t16, q.dh.p, q.dh.rows, q.dh.cols, q.dh.ld, 32, 32);
   if (!ok) return MB_ERR_CUDA;
-  const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), cols = kEpi == kPlain ? BN : kFeat;
+  const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), cols = is_plain(kEpi) ? BN : kFeat;
   const int64_t nt = (q.N + cols - 1) / cols;
   const int64_t work = mt * nt * q.nprob;
   const int64_t kb = (q.K + BK - 1) / BK;
@@ -827,7 +879,7 @@ int launch_skinny(const Product& q, cudaStream_t stream) {
   const int64_t kb = (q.K + BK - 1) / BK;
   if (kb * q.nseg > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
   g.kb = (int)kb; g.nseg = q.nseg;
-  const int64_t per = kEpi == kPlain ? 128 : 64;
+  const int64_t per = is_plain(kEpi) ? 128 : 64;
   const int64_t tiles = (q.N + per - 1) / per, ytiles = (T + g.n - 1) / g.n;
   const int64_t KB = kb * q.nseg;
   // Split the contraction until the launch has two CTAs for every SM, as long as
@@ -846,11 +898,12 @@ int launch_skinny(const Product& q, cudaStream_t stream) {
   g.act = q.act;
   Maps m;
   bool ok = true;
-  const int nw = kEpi == kPlain ? q.nseg : 2;
+  const int nw = is_plain(kEpi) ? q.nseg : 2;
+  constexpr CUtensorMapDataType t16 = kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   for (int i = 0; i < nw; ++i)
-    ok = ok && map_2d(&m.a[i], q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, 64, kF16);
+    ok = ok && map_2d(&m.a[i], t16, q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, 64);
   for (int i = 0; i < q.nseg; ++i)
-    ok = ok && map_2d(&m.b[i], q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, g.n, kF16);
+    ok = ok && map_2d(&m.b[i], t16, q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, g.n);
   if (!ok) return MB_ERR_CUDA;
   g.o0 = const_cast<void*>(q.o[0].p); g.ldo = q.o[0].ld;
   g.o1 = const_cast<void*>(q.o[1].p); g.ldu = q.o[1].ld;
@@ -871,6 +924,11 @@ int run_product(const Product& q, cudaStream_t st) {
   if (q.epi == kGated) return skinny ? launch_skinny<kGated, false, kF16>(q, st) : launch_pair<kGated, false, false, kF16>(q, st);
   if (q.epi == kGatedBwd)
     return skinny ? launch_skinny<kGatedBwd, false, kF16>(q, st) : launch_pair<kGatedBwd, false, false, kF16>(q, st);
+  if (q.epi == kGatedBwdF32)
+    return skinny ? launch_skinny<kGatedBwdF32, false, kF16>(q, st)
+                  : launch_pair<kGatedBwdF32, false, false, kF16>(q, st);
+  if (q.epi == kPlainF32)
+    return skinny ? launch_skinny<kPlainF32, true, kF16>(q, st) : launch_pair<kPlainF32, false, true, kF16>(q, st);
   if (q.a_mn) return launch_pair<kPlain, true, true, kF16>(q, st);
   if (q.b_mn) return skinny ? launch_skinny<kPlain, true, kF16>(q, st) : launch_pair<kPlain, false, true, kF16>(q, st);
   return skinny ? launch_skinny<kPlain, false, kF16>(q, st) : launch_pair<kPlain, false, false, kF16>(q, st);
@@ -971,7 +1029,8 @@ MB_API int mb_feed_forward(const mb_ffn_args* a, void* y, int64_t ldy, void* wor
 MB_API size_t mb_feed_forward_backward_workspace_bytes(int64_t tokens, int64_t d, int64_t f, int32_t from_codes,
                                                        int32_t with_down) {
   if (tokens <= 0 || d <= 0 || f <= 0 || tokens > kMaxDim || d > kMaxDim || f > kMaxDim) return 0;
-  return (with_down ? 3 : 2) * area(tokens, f) + (from_codes ? area(tokens, d) : 0);
+  // dg, du; with down: h and an FP32 dh
+  return (with_down ? 5 : 2) * area(tokens, f) + (from_codes ? area(tokens, d) : 0);
 }
 
 MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r, void* workspace,
@@ -1007,9 +1066,9 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
   Mat dh{r->dy, T, f, r->lddy}, h;
   ws += 2 * area(T, f);
   if (down) {
-    dh = {ws, T, f, fp};
-    h = dh;  // h takes dh's place, element by element
-    ws += area(T, f);
+    h = {ws, T, f, fp};
+    dh = {ws + area(T, f), T, f, fp};
+    ws += 3 * area(T, f);
   }
   Mat x{a->x, T, d, a->ldx};
   if (from_codes) {
@@ -1020,6 +1079,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
   const Mat dy{r->dy, T, d, r->lddy};
   if (down) {
     Product q;
+    q.epi = kPlainF32;
     q.a[0] = dy;
     q.b[0] = {a->down, d, f, a->ld_down};
     q.b_mn = true;
@@ -1030,7 +1090,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
   }
   {
     Product q = gated_product(a, x);
-    q.epi = kGatedBwd;
+    q.epi = down ? kGatedBwdF32 : kGatedBwd;
     q.dh = dh;
     q.o[0] = dg; q.o[1] = du;
     if (r->ddown) q.o[2] = h;

@@ -7,8 +7,9 @@ forward and backward, with 8-bit activation checkpoints.
 ``x`` is [..., d]; ``gate`` and ``up`` are [f, d] and ``down`` [d, f], as
 ``nn.Linear`` keeps the ``ffn.gate`` / ``ffn.up`` / ``ffn.down`` weights of
 morph/model/morph_model.py:23-28. Everything is bfloat16, or everything is
-float16; products accumulate in FP32, and h, dh and the gradients of the two
-projections' outputs are rounded to 16 bits once each.
+float16; products accumulate in FP32, and h and the gradients of the two
+projections' outputs are rounded to 16 bits once each, as the next product's
+operand.
 
 Both functions are differentiable. What they keep for the backward pass is the
 block's input only, as it is (``checkpoint="x"``) or in 8 bits
@@ -34,6 +35,9 @@ from .precision import check_activation, pack_activation
 
 ACTIVATIONS = {"silu": _lib.MB_ACT_SILU, "gelu_tanh": _lib.MB_ACT_GELU_TANH}
 CHECKPOINTS = ("x", "fp8")
+DTYPES = {torch.bfloat16: _lib.MB_BF16, torch.float16: _lib.MB_F16}
+GRADS = ("dx", "dgate", "dup", "ddown")
+PITCHES = ("lddx", "ld_dgate", "ld_dup", "ld_ddown")
 
 
 def _activation_code(activation) -> int:
@@ -43,7 +47,7 @@ def _activation_code(activation) -> int:
 
 
 def _check(tensor, what, shape, like) -> None:
-    if not isinstance(tensor, torch.Tensor) or tuple(tensor.shape) != shape:
+    if not isinstance(tensor, torch.Tensor) or tensor.shape != shape:
         raise ValueError(f"{what} must be a tensor of shape {list(shape)}")
     if tensor.dtype != like.dtype or tensor.device != like.device:
         raise ValueError(f"{what} is {tensor.dtype} on {tensor.device}, expected {like.dtype} on {like.device}")
@@ -52,7 +56,7 @@ def _check(tensor, what, shape, like) -> None:
 def _check_weights(gate, up, down, d):
     if not isinstance(gate, torch.Tensor) or gate.dim() != 2 or not gate.is_cuda:
         raise ValueError("gate must be [f, d] on a CUDA device")
-    if gate.dtype not in (torch.bfloat16, torch.float16):
+    if gate.dtype not in DTYPES:
         raise ValueError(f"the block computes in bfloat16 or float16, not {gate.dtype}")
     f = gate.shape[0]
     if f == 0 or d == 0:
@@ -68,36 +72,43 @@ def _pad8(n: int) -> int:
     return (n + 7) // 8 * 8
 
 
-def _rows(t):
-    """(tensor, pitch) of a 2-D tensor with 16-byte aligned rows: itself, or a padded copy."""
-    rows, cols = t.shape
-    ld = t.stride(0) if rows > 1 else _pad8(cols)
-    if (cols == 1 or t.stride(1) == 1) and ld >= cols and ld % 8 == 0 and t.data_ptr() % 16 == 0:
+def _rows(t, rows, cols):
+    """(tensor, pitch) of a [rows, cols] tensor with 16-byte aligned rows: itself, or a padded copy."""
+    ld, inner = t.stride()
+    if rows <= 1:
+        ld = _pad8(cols)
+    if (inner == 1 or cols == 1) and ld % 8 == 0 and ld >= cols and t.data_ptr() % 16 == 0:
         return t, ld
     buf = torch.empty((rows, _pad8(cols)), dtype=t.dtype, device=t.device)
-    buf[:, :cols].copy_(t)
+    buf[:, :cols].copy_(t.detach())
     return buf, buf.shape[1]
 
 
 def _out(rows, cols, like):
-    """(buffer, pitch) for a [rows, cols] output with 16-byte aligned rows."""
-    return torch.empty((rows, _pad8(cols)), dtype=like.dtype, device=like.device), _pad8(cols)
+    """A buffer for a [rows, cols] output, its rows padded to 16 bytes."""
+    return torch.empty((rows, _pad8(cols)), dtype=like.dtype, device=like.device)
 
 
 def _crop(buf, cols):
     return buf if buf.shape[1] == cols else buf[:, :cols].contiguous()
 
 
-def _args(code, tokens, d, f, like, x, gate, up, down):
-    a = _lib.FfnArgs(_lib.dtype_code(like.dtype), code, tokens, d, f)
-    keep = []
-    for name, t in (("x", x), ("gate", gate), ("up", up), ("down", down)):
-        if t is not None:
-            buf, ld = _rows(t)
-            keep.append(buf)
-            setattr(a, name, buf.data_ptr())
-            setattr(a, "ldx" if name == "x" else "ld_" + name, ld)
-    return a, keep
+def _two_d(t):
+    return t if t.dim() == 2 else t.detach().reshape(-1, t.shape[-1])
+
+
+def _args(code, tokens, d, f, x, gate, up, down):
+    """The C arguments, and the tensors they point into."""
+    gate, ld_gate = _rows(gate, f, d)
+    up, ld_up = _rows(up, f, d)
+    a = _lib.FfnArgs(DTYPES[gate.dtype], code, tokens, d, f, None, 0, gate.data_ptr(), ld_gate, up.data_ptr(), ld_up)
+    if x is not None:
+        x, a.ldx = _rows(x, tokens, d)
+        a.x = x.data_ptr()
+    if down is not None:
+        down, a.ld_down = _rows(down, d, f)
+        a.down = down.data_ptr()
+    return a, (x, gate, up, down)
 
 
 def _input(x, gate):
@@ -108,83 +119,76 @@ def _input(x, gate):
     return x.shape[-1]
 
 
-def _forward(x, gate, up, down, activation):
-    code = _activation_code(activation)
+def _forward(x, gate, up, down, code):
     d = _input(x, gate)
     f = _check_weights(gate, up, down, d)
-    x2 = x.detach().reshape(-1, d)
-    tokens = x2.shape[0]
-    width = f if down is None else d
-    with torch.cuda.device(x.device):
-        a, keep = _args(code, tokens, d, f, x, x2, gate.detach(), up.detach(), None if down is None else down.detach())
-        out, ld = _out(tokens, width, x)
+    with _lib.on_device(x.device) as stream:
+        x2 = _two_d(x)
+        tokens = x2.shape[0]
+        width = f if down is None else d
+        a, keep = _args(code, tokens, d, f, x2, gate, up, down)
+        out = _out(tokens, width, x)
         L = _lib.lib()
         if down is None:
-            _lib.check(L.mb_gated_linear(ctypes.byref(a), out.data_ptr(), ld, _lib.stream_handle()), "gated_linear")
+            _lib.check(L.mb_gated_linear(ctypes.byref(a), out.data_ptr(), out.shape[1], stream), "gated_linear")
         else:
             nbytes = L.mb_feed_forward_workspace_bytes(tokens, f)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            _lib.check(L.mb_feed_forward(ctypes.byref(a), out.data_ptr(), ld, ws.data_ptr(), nbytes,
-                                         _lib.stream_handle()), "feed_forward")
+            _lib.check(L.mb_feed_forward(ctypes.byref(a), out.data_ptr(), out.shape[1], ws.data_ptr(), nbytes, stream),
+                       "feed_forward")
         del keep
-        return _crop(out, width).view(x.shape[:-1] + (width,))
+        out = _crop(out, width)
+        return out if x.dim() == 2 else out.view(x.shape[:-1] + (width,))
 
 
-def _backward(grad, saved, gate, up, down, activation, needs):
-    code = _activation_code(activation)
+def _backward(grad, saved, gate, up, down, code, needs):
     if isinstance(saved, torch.Tensor):
-        d = _input(saved, gate)
-        shape, device = saved.shape, saved.device
+        d, like, codes = _input(saved, gate), saved, None
     else:
         codes, scales = saved
         check_activation(codes, scales)
-        shape, device, d = codes.shape, codes.device, codes.shape[-1]
+        d, like = codes.shape[-1], codes
     f = _check_weights(gate, up, down, d)
-    if gate.device != device:
+    if gate.device != like.device:
         raise ValueError("the checkpoint and the weights are on different devices")
-    _check(grad, "the output's gradient", tuple(shape[:-1]) + (f if down is None else d,), gate)
+    _check(grad, "the output's gradient", like.shape[:-1] + (f if down is None else d,), gate)
     if len(needs) != (3 if down is None else 4):
         raise ValueError("needs names one truth value for x and each weight")
-    with torch.cuda.device(device):
-        g2 = grad.detach().reshape(-1, grad.shape[-1])
+    with _lib.on_device(gate.device) as stream:
+        g2 = _two_d(grad)
         tokens = g2.shape[0]
-        x2 = saved.detach().reshape(-1, d) if isinstance(saved, torch.Tensor) else None
-        a, keep = _args(code, tokens, d, f, gate, x2, gate.detach(), up.detach(),
-                        None if down is None else down.detach())
-        g2, lddy = _rows(g2)
+        a, keep = _args(code, tokens, d, f, None if codes is not None else _two_d(saved), gate, up, down)
         r = _lib.FfnGrads()
-        if x2 is None:
+        if codes is not None:
             r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
-        r.dy, r.lddy = g2.data_ptr(), lddy
-        outs = []
-        for need, name, rows, cols in zip(needs, ("dx", "dgate", "dup", "ddown"), (tokens, f, f, d), (d, d, d, f)):
-            if not need:
-                outs.append(None)
-                continue
-            buf, ld = _out(rows, cols, gate)
-            setattr(r, name, buf.data_ptr())
-            setattr(r, "lddx" if name == "dx" else "ld_" + name, ld)
-            outs.append((buf, cols))
+        g2, r.lddy = _rows(g2, tokens, f if down is None else d)
+        r.dy = g2.data_ptr()
+        grads = [None] * len(needs)
+        for i, (need, rows, cols) in enumerate(zip(needs, (tokens, f, f, d), (d, d, d, f))):
+            if need:
+                grads[i] = buf = _out(rows, cols, gate)
+                setattr(r, GRADS[i], buf.data_ptr())
+                setattr(r, PITCHES[i], buf.shape[1])
         L = _lib.lib()
-        nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, x2 is None, down is not None)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _lib.check(L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), ws.data_ptr(), nbytes,
-                                              _lib.stream_handle()), "feed_forward_backward")
+        nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, codes is not None, down is not None)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=gate.device)
+        _lib.check(L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), ws.data_ptr(), nbytes, stream),
+                   "feed_forward_backward")
         del keep
-        grads = [None if o is None else _crop(*o) for o in outs]
-        if grads[0] is not None:
-            grads[0] = grads[0].view(shape)
+        grads = [None if buf is None else _crop(buf, cols) for buf, cols in zip(grads, (d, d, d, f))]
+        if grads[0] is not None and like.dim() != 2:
+            grads[0] = grads[0].view(like.shape)
         return tuple(grads)
 
 
 class _Block(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate, up, down, activation, checkpoint):
-        ctx.activation, ctx.checkpoint = activation, checkpoint
+    def forward(ctx, x, gate, up, down, code, checkpoint):
+        ctx.code, ctx.checkpoint, ctx.has_down = code, checkpoint, down is not None
+        y = _forward(x, gate, up, down, code)
         kept = pack_activation(x) if checkpoint == "fp8" else (x,)
-        ctx.save_for_backward(gate, up, *(() if down is None else (down,)), *kept)
-        ctx.has_down = down is not None
-        return _forward(x, gate, up, down, activation)
+        ctx.save_for_backward(gate, up, *((down,) if ctx.has_down else ()), *kept)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -193,19 +197,17 @@ class _Block(torch.autograd.Function):
         down = rest.pop(0) if ctx.has_down else None
         saved = tuple(rest) if ctx.checkpoint == "fp8" else rest[0]
         needs = ctx.needs_input_grad[:4 if ctx.has_down else 3]
-        grads = _backward(grad, saved, gate, up, down, ctx.activation, needs)
-        return (*grads, *([] if ctx.has_down else [None]), None, None)
+        grads = _backward(grad, saved, gate, up, down, ctx.code, needs)
+        return (*grads, None, None) if ctx.has_down else (*grads, None, None, None)
 
 
 def _block(x, gate, up, down, activation, checkpoint):
+    code = _activation_code(activation)
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"checkpoint must be one of {list(CHECKPOINTS)}, not {checkpoint!r}")
-    leaves = (x, gate, up) if down is None else (x, gate, up, down)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in leaves):
-        _activation_code(activation)
-        _check_weights(gate, up, down, _input(x, gate))
-        return _Block.apply(x, gate, up, down, activation, checkpoint)
-    return _forward(x, gate, up, down, activation)
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, gate, up, down)):
+        return _Block.apply(x, gate, up, down, code, checkpoint)
+    return _forward(x, gate, up, down, code)
 
 
 def gated_linear(x, gate, up, activation="silu", checkpoint="x"):
@@ -218,7 +220,7 @@ def gated_linear_backward(dh, x, gate, up, activation="silu", needs=(True, True,
     """(dx, dgate, dup) of ``gated_linear`` from its output's gradient ``dh``
     [..., f]. ``x`` is the input, or the ``(codes, scales)`` of its 8-bit
     checkpoint. An entry of ``needs`` that is false gives None."""
-    return _backward(dh, x, gate, up, None, activation, needs)
+    return _backward(dh, x, gate, up, None, _activation_code(activation), needs)
 
 
 def feed_forward(x, gate, up, down, activation="silu", checkpoint="x"):
@@ -235,7 +237,7 @@ def feed_forward_backward(dy, x, gate, up, down, activation="silu", needs=(True,
     checkpoint. An entry of ``needs`` that is false gives None."""
     if down is None:
         raise ValueError("down must be a tensor")
-    return _backward(dy, x, gate, up, down, activation, needs)
+    return _backward(dy, x, gate, up, down, _activation_code(activation), needs)
 
 
 def check(device=None) -> None:
@@ -243,7 +245,7 @@ def check(device=None) -> None:
     block kernel there gave up a bounded wait since the last check; what it wrote
     is then not valid."""
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
-        torch.cuda.synchronize()
+        torch.cuda.synchronize()  # mb_ffn_status reads behind the default stream only
         _lib.check(_lib.lib().mb_ffn_status(), "feed_forward")
 
 

@@ -172,17 +172,18 @@ def pack_activation(x: torch.Tensor):
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("pack_activation expects [..., d] with d >= 1")
     d = x.shape[-1]
-    x = x.detach()
-    rows = x.numel() // d
-    flat = x.reshape(-1, d)
-    if rows and (flat.stride(1) != 1 and d > 1 or rows > 1 and flat.stride(0) < d):
-        flat = flat.contiguous()
-    ld = flat.stride(0) if rows > 1 else d
+    flat = x if x.dim() == 2 else x.detach().reshape(-1, d)
+    rows = flat.shape[0]
+    ld, inner = flat.stride()
+    if inner != 1 and d > 1 or rows > 1 and ld < d:
+        flat, ld = flat.detach().contiguous(), d
+    elif rows <= 1:
+        ld = d
     codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
     scales = torch.empty(x.shape[:-1] + (-(-d // ACTIVATION_BLOCK),), dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device) as stream:
         _lib.check(_lib.lib().mb_act_pack(flat.data_ptr(), _lib.dtype_code(x.dtype), rows, d, ld, codes.data_ptr(),
-                                          scales.data_ptr(), _lib.stream_handle()), "pack_activation")
+                                          scales.data_ptr(), stream), "pack_activation")
     return codes, scales
 
 
@@ -210,10 +211,9 @@ def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfl
         raise ValueError(f"unsupported dtype {dtype}")
     d = codes.shape[-1]
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
-    with torch.cuda.device(codes.device):
+    with _lib.on_device(codes.device) as stream:
         _lib.check(_lib.lib().mb_act_unpack(codes.data_ptr(), scales.data_ptr(), codes.numel() // d, d,
-                                            out.data_ptr(), _lib.dtype_code(dtype), d, _lib.stream_handle()),
-                   "unpack_activation")
+                                            out.data_ptr(), _lib.dtype_code(dtype), d, stream), "unpack_activation")
     return out
 
 

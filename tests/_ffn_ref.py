@@ -89,7 +89,7 @@ def forward_sigma(x, gate, up, down, kind, unit):
 
 def backward(dy, x, gate, up, down, kind):
     """Gradients, and one standard deviation of each one's error before its own
-    rounding (the roundings of dh, dg, du and h as independent errors of `unit`
+    rounding (the roundings of dg, du and h as independent errors of `unit`
     relative, passed on to first order)."""
     dy, x, gate, up = dy.double(), x.double(), gate.double(), up.double()
     g, u = x @ gate.T, x @ up.T
@@ -104,7 +104,7 @@ def backward(dy, x, gate, up, down, kind):
         f32 = lambda a, b: math.sqrt(a.shape[1]) * 2.0 ** -23 * _sq(a, b).sqrt()  # noqa: E731
         eg, eu = f32(x, gate.T), f32(x, up.T)
         # |act''| <= 1.2 for both activations (0.5 and 1.13 at 0)
-        edh = 0 if down is None else unit * dh.abs() + f32(dy, down.double())
+        edh = 0 if down is None else f32(dy, down.double())  # dh stays in FP32
         edg = unit * dg.abs() + (u * da * edh).abs() + (dh * da * eu).abs() + 1.2 * (dh * u * eg).abs() \
             + 2.0 ** -18 * (dh * u).abs()
         edu = unit * du.abs() + (a * edh).abs() + (dh * da * eg).abs() + 2.0 ** -20 * du.abs()
