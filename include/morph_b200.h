@@ -439,11 +439,14 @@ typedef struct mb_ffn_args {
   int64_t ld_down;
 } mb_ffn_args;
 
-/* h = act(x gate^T) * (x up^T), [tokens, f]: one launch. */
-MB_API int mb_gated_linear(const mb_ffn_args* args, void* h, int64_t ldh, mb_stream_t stream);
+/* h = act(x gate^T) * (x up^T), [tokens, f]. Workspaces (device, 256-byte aligned)
+ * need no preparation and hold nothing after the call; calls that may overlap need
+ * one each. */
+MB_API size_t mb_gated_linear_workspace_bytes(int64_t tokens);
+MB_API int mb_gated_linear(const mb_ffn_args* args, void* h, int64_t ldh, void* workspace, size_t workspace_bytes,
+                           mb_stream_t stream);
 
-/* y = h down^T, [tokens, d]. The workspace (device, 16-byte aligned) holds h for
- * the call only. */
+/* y = h down^T, [tokens, d]. */
 MB_API size_t mb_feed_forward_workspace_bytes(int64_t tokens, int64_t f);
 MB_API int mb_feed_forward(const mb_ffn_args* args, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
                            mb_stream_t stream);

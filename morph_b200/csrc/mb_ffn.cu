@@ -30,11 +30,22 @@
 // Tiles run in groups of kGroupM row tiles, so that what the ~74 pairs read at one
 // time (about 8 x 9 tiles' operands) stays in L2.
 //
-// k_ffn_skinny (T <= kSkinnyTokens): weights are the MMA's M side (128 rows per
-// CTA), tokens its N side (16 .. 256), so each weight is read once and the kernel is
-// a stream over them, bound by HBM up to ~150 tokens. Clusters of 1-8 CTAs split the
-// contraction; their FP32 partials are summed over distributed shared memory in
-// rank order (no atomics, no workspace, the same result every run).
+// Its grid is persistent: whole tiles in turn, and where the last round would leave
+// most pairs idle, that round's tiles are cut along the contraction into equal
+// pieces (Sched). Every piece writes its FP32 partial to the workspace and counts
+// itself in; the one that arrives last adds all of them in contraction order
+// (whichever it is, so the sum does not depend on timing) and runs the epilogue.
+// Nobody waits for another pair.
+//
+// k_ffn_skinny (T <= kSkinnyTokens): weights are the MMA's M side (128 rows per CTA:
+// 64 gate and 64 up rows in the gated forms), tokens its N side (16 ..), so each
+// weight is read once and the kernel is a stream over them, bound by HBM. Clusters of
+// 1-8 CTAs split the contraction; their FP32 partials are summed over distributed
+// shared memory in rank order (no atomics, no workspace).
+//
+// The kernels of one call follow each other with programmatic dependent launch: the
+// next one sets up (and the skinny one requests its first weights, which no kernel
+// of the call writes) while the previous one finishes.
 //
 // Waits are bounded as in mb_gemm.cu: on expiry a CTA raises the device's error word
 // (mb_ffn_status), waits (bounded) for its own copies, frees TMEM and returns.
@@ -56,7 +67,8 @@ __device__ int32_t g_ffn_err;
 
 constexpr int BM = 128, BN = 256, BK = 64;
 constexpr int kFeat = BN / 2;  // features of a gated tile (gate | up halves)
-constexpr int kPairThreads = 192;
+constexpr int kEpiWarps = 8;  // two per TMEM lane quarter, each with half of the tile's columns
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;
 constexpr int kTileA = BM * BK * 2;         // 16 KiB: this CTA's rows of A
 constexpr int kTileB = (BN / 2) * BK * 2;   // 16 KiB: this CTA's half of B
 constexpr int kBox = 64 * 64 * 2;           // 8 KiB: one 64 x 64 MN-major box
@@ -71,20 +83,31 @@ enum Epi { kPlain = 0, kGated = 1, kGatedBwd = 2, kPlainF32 = 3, kGatedBwdF32 = 
 constexpr bool is_plain(int epi) { return epi == kPlain || epi == kPlainF32; }
 constexpr bool is_bwd(int epi) { return epi == kGatedBwd || epi == kGatedBwdF32; }
 
-// Ring stages and shared memory of an epilogue warp. The backward epilogue works
-// on 32 x 32 blocks: two dh blocks in flight and one block each of dg, du and h.
-constexpr int kDhBlock = 32 * 32 * 4;
+// Ring stages and shared memory of an epilogue warp: one store tile, or in the
+// backward form a 32 x 32 block each of dg, du and h.
 constexpr int kOutBlock = 32 * 32 * 2;
 constexpr int stages(int epi) { return is_bwd(epi) ? 5 : 6; }
-constexpr int warp_bytes(int epi) { return is_bwd(epi) ? 2 * kDhBlock + 3 * kOutBlock : 2 * kStoreTile; }
-constexpr int pair_smem(int epi) { return 1024 + stages(epi) * (kTileA + kTileB) + 4 * warp_bytes(epi) + kBarBytes; }
+constexpr int warp_bytes(int epi) { return is_bwd(epi) ? 3 * kOutBlock : kStoreTile; }
+constexpr int pair_smem(int epi) {
+  return 1024 + stages(epi) * (kTileA + kTileB) + kEpiWarps * warp_bytes(epi) + kBarBytes;
+}
 static_assert(pair_smem(kPlain) <= 232448 && pair_smem(kGatedBwd) <= 232448, "shared memory of one SM");
-static_assert(warp_bytes(kGatedBwd) % 1024 % 512 == 0, "swizzled blocks stay aligned");
+static_assert(warp_bytes(kGatedBwd) % 512 == 0, "swizzled blocks stay aligned");
 
 struct Maps {
   CUtensorMap a[2], b[2];  // K segments, problems, or (b) gate and up
   CUtensorMap o[3];        // outputs (backward: dg, du, h)
-  CUtensorMap dh;          // backward input
+};
+
+// Work of one launch: `tiles` output tiles of `kb` k-blocks each over `units` CTA
+// pairs. Each of the first cut_tiles tiles is cut into `ways` pieces, one for each of
+// the first cut_tiles * ways units; the rest go whole, in turn.
+struct Sched {
+  int tiles, kb, units, cut_tiles, ways;
+};
+
+template <int N> struct Int {
+  static constexpr int value = N;
 };
 
 struct PairArgs {
@@ -93,8 +116,13 @@ struct PairArgs {
   int nseg;       // K segments accumulated into one output (dx: 2)
   int nprob;      // problems of one launch along M (weight gradients: up to 2)
   int mt, nt;     // tiles of one problem
+  Sched sched;
+  float* partials;    // workspace of tiles cut between units
+  int32_t* counters;
   int act;
-  int want_h;     // backward: store h
+  int want_h;       // backward: store h
+  const void* dh;   // backward input: FP32 (kGatedBwdF32) or 16-bit
+  int64_t lddh;
   FaultPlan fault;  // test-only: a tile whose first k-block is withheld, and the launch's wait bound
 };
 
@@ -154,16 +182,14 @@ __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, int slice) {
          ((uint64_t)2 << 61);
 }
 
-__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // ------------------------------------------------------------- arithmetic --
@@ -216,7 +242,7 @@ __device__ __forceinline__ uint4* tile_chunk(uint8_t* tile, int r, int c) {
 }
 
 template <bool kF16>
-__device__ __forceinline__ void put_row(uint8_t* tile, int r, int c0, const float (&v)[32]) {
+__device__ __forceinline__ void put_row(uint8_t* tile, int r, int c0, const float* v) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
     *tile_chunk(tile, r, c0 + c) = make_uint4(pack2<kF16>(v[8 * c], v[8 * c + 1]), pack2<kF16>(v[8 * c + 2], v[8 * c + 3]),
@@ -228,7 +254,68 @@ __device__ __forceinline__ uint4* block_chunk(uint8_t* block, int r, int c) {
   return reinterpret_cast<uint4*>(block + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
+// ------------------------------------------------------------- scheduling --
+
+// One piece of work: k-blocks [k0, k1) of a tile; `own` of the tile's `ways` pieces.
+struct Item {
+  int tile, k0, k1, ways, own;
+};
+
+struct Items {
+  int unit, next_tile;
+  bool cut;
+  __device__ __forceinline__ Items(const Sched& s, int u)
+      : unit(u), next_tile(s.cut_tiles + u), cut(u < s.cut_tiles * s.ways) {}
+  __device__ __forceinline__ bool next(const Sched& s, Item& it) {
+    if (cut) {
+      cut = false;
+      it.tile = unit / s.ways;
+      it.own = unit - it.tile * s.ways;
+      it.ways = s.ways;
+      it.k0 = (int)((int64_t)s.kb * it.own / s.ways);
+      it.k1 = (int)((int64_t)s.kb * (it.own + 1) / s.ways);
+      return true;
+    }
+    it.tile = next_tile;
+    it.k0 = 0;
+    it.k1 = s.kb;
+    it.ways = 1;
+    it.own = 0;
+    next_tile += s.units;
+    return it.tile < s.tiles;
+  }
+};
+
+// After a warp wrote its partial: true for the piece that arrives last, which then
+// sees all others' partials and leaves the counter at zero.
+__device__ __forceinline__ bool arrive_last(int32_t* counter, int ways, int lane) {
+  __threadfence();
+  __syncwarp();
+  int before = 0;
+  if (lane == 0) before = atomicAdd(counter, 1);
+  before = __shfl_sync(0xffffffffu, before, 0);
+  if (before != ways - 1) return false;
+  __threadfence();
+  if (lane == 0) *counter = 0;
+  return true;
+}
+
+// Programmatic dependent launch: let the next kernel of the call set up, and wait
+// for everything the previous ones wrote.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__global__ void k_zero(int32_t* p, int n) {
+  pdl_trigger();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0;
+}
+
 // ------------------------------------------------------------ pair kernel --
+
+// A warp's partial of a cut tile: its 32 rows x 128 accumulator columns (plain: half
+// the tile; gated: 64 features' g, then their u).
+constexpr int kWarpCols = BN / 2;
+constexpr int kWarpPartial = 32 * kWarpCols;  // floats
 
 // Tile t -> (problem, row tile, column tile): groups of kGroupM row tiles, row
 // tiles fastest inside a group.
@@ -244,6 +331,46 @@ __device__ __forceinline__ void tile_of(const PairArgs& g, int t, int& prob, int
   bn = in / rows;
 }
 
+// 32 dh values of one row from feature `col` on (zero past the last feature; rows
+// are 32-byte aligned in the FP32 form, 16-byte in the caller's 16-bit one).
+template <int kEpi, bool kF16>
+__device__ __forceinline__ void load_dh(const PairArgs& g, int64_t row, int col, float (&v)[32]) {
+  const bool in = row < g.M;
+  if constexpr (kEpi == kGatedBwdF32) {
+    const float* p = static_cast<const float*>(g.dh) + row * g.lddh + col;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (in && col + 8 * k < g.N) {  // the row's pitch covers the whole group of 8
+        asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[8 * k]), "=f"(v[8 * k + 1]), "=f"(v[8 * k + 2]), "=f"(v[8 * k + 3]), "=f"(v[8 * k + 4]),
+                       "=f"(v[8 * k + 5]), "=f"(v[8 * k + 6]), "=f"(v[8 * k + 7])
+                     : "l"(p + 8 * k)
+                     : "memory");
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * k + e] = 0.0f;
+      }
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(g.dh) + row * g.lddh + col;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (in && col + 8 * k + 8 <= g.N) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p + 8 * k);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[8 * k + 2 * e] = h2f<kF16>((uint16_t)(ww[e] & 0xffffu));
+          v[8 * k + 2 * e + 1] = h2f<kF16>((uint16_t)(ww[e] >> 16));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * k + e] = in && col + 8 * k + e < g.N ? h2f<kF16>(p[8 * k + e]) : 0.0f;
+      }
+    }
+  }
+}
+
 template <int kEpi, bool kAMn, bool kBMn, bool kF16>
 __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_constant__ Maps maps, const PairArgs g) {
   constexpr int ST = stages(kEpi);
@@ -252,21 +379,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
   uint8_t* sA = smem;
   uint8_t* sB = sA + ST * kTileA;
   uint8_t* sOut = sB + ST * kTileB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 4 * warp_bytes(kEpi));
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + kEpiWarps * warp_bytes(kEpi));
   uint64_t* empty = full + ST;
   uint64_t* acc_full = empty + ST;      // [2]
   uint64_t* acc_empty = acc_full + 2;   // [2]: one arrival per epilogue warp of both CTAs
   uint64_t* drain = acc_empty + 2;
-  uint64_t* dh_full = drain + 1;        // [4][2]: each epilogue warp's dh blocks
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dh_full + 8);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
-  const int unit = (int)(blockIdx.x >> 1), n_units = (int)(gridDim.x >> 1);
-  const int total = g.nprob * g.mt * g.nt;
-  const int KB = g.kb * g.nseg;
+  const int unit = (int)(blockIdx.x >> 1);
+  Item item;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -275,10 +400,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 8);
+      mbar_init(&acc_empty[a], 2 * kEpiWarps);
     }
     mbar_init(drain, 1);
-    for (int w = 0; w < 8; ++w) mbar_init(&dh_full[w], 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -292,20 +416,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
 
   if (warp == 0) {
     if (lane == 0) {
+      pdl_wait();
       int kit = 0;
-      for (int t = unit; t < total && !*abort_flag; t += n_units) {
+      for (Items work(g.sched, unit); !*abort_flag && work.next(g.sched, item);) {
         int prob, bm, bn;
-        tile_of(g, t, prob, bm, bn);
+        tile_of(g, item.tile, prob, bm, bn);
         const int arow = bm * 2 * BM + (int)rank * BM;
         // gated tiles: 128 features from gate (even CTA) or up (odd CTA)
         const int brow = is_plain(kEpi) ? bn * BN + (int)rank * (BN / 2) : bn * kFeat;
-        for (int kb = 0; kb < KB; ++kb, ++kit) {
+        for (int kb = item.k0; kb < item.k1; ++kb, ++kit) {
           const int s = kit % ST;
           if (!mbar_wait(&empty[s], ((kit / ST) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
-          if (t == g.fault.unit && kb == 0) continue;  // test-only: withhold; the MMA warp's wait expires
+          if (item.tile == g.fault.unit && kb == 0) continue;  // test-only: withhold; the MMA warp's wait expires
           const int seg = kb >= g.kb ? 1 : 0;
           const int k0 = (kb - seg * g.kb) * BK;
           const CUtensorMap* ma = &maps.a[seg + prob];
@@ -340,19 +466,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     if (lane == 0 && leader) {
       const uint32_t id = idesc(kF16, kAMn, kBMn, 2 * BM, BN);
       int kit = 0, it = 0;
-      for (int t = unit; t < total && !*abort_flag; t += n_units, ++it) {
+      for (Items work(g.sched, unit); !*abort_flag && work.next(g.sched, item); ++it) {
         const int a = it & 1;
         if (!mbar_wait_cluster(&acc_empty[a], ((it >> 1) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
         tc_fence_after();
         const uint32_t acc = tmem + (uint32_t)(a * BN);
-        for (int kb = 0; kb < KB; ++kb, ++kit) {
+        for (int kb = item.k0; kb < item.k1; ++kb, ++kit) {
           const int s = kit % ST;
           if (!mbar_wait(&full[s], (kit / ST) & 1, abort_flag, g.fault.limit_ns)) break;
           tc_fence_after();
           const uint32_t a0 = smem_u32(sA + s * kTileA), b0 = smem_u32(sB + s * kTileB);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            umma_pair(acc, tile_desc<kAMn>(a0, k), tile_desc<kBMn>(b0, k), id, (kb | k) != 0 ? 1u : 0u);
+            umma_pair(acc, tile_desc<kAMn>(a0, k), tile_desc<kBMn>(b0, k), id, kb != item.k0 || k != 0 ? 1u : 0u);
           umma_commit_both(&empty[s]);
         }
         // an aborted tile is not handed over: the odd CTA cannot see this CTA's abort flag
@@ -366,168 +492,193 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
       }
     }
   } else {
-    const int q = warp & 3;  // TMEM lane quarter this warp may read
+    const int q = warp & 3;              // TMEM lane quarter this warp may read
+    const int half = (warp - 2) >> 2;    // its half of the tile's columns (gated: features)
+    const int w16 = (int)rank * kEpiWarps + half * 4 + q;
     uint8_t* out = sOut + (warp - 2) * warp_bytes(kEpi);
-    uint64_t* dh_bar = &dh_full[2 * (warp - 2)];
-    int it = 0, buf = 0;
-    uint32_t dh_asked = 0, dh_read = 0;  // dh blocks loaded / consumed so far
-    for (int t = unit; t < total; t += n_units, ++it) {
+    int it = 0;
+    pdl_wait();
+    for (Items work(g.sched, unit); work.next(g.sched, item); ++it) {
       const int a = it & 1;
       int prob, bm, bn;
-      tile_of(g, t, prob, bm, bn);
+      tile_of(g, item.tile, prob, bm, bn);
       const int row0 = bm * 2 * BM + (int)rank * BM + q * 32;
-      const int col0 = is_plain(kEpi) ? bn * BN : bn * kFeat;
-      const bool rows_in = row0 < g.M;
-      // backward: 32-feature blocks of this warp's rows that exist
-      const int left = (g.N - col0 + 31) / 32;
-      const int blocks = is_bwd(kEpi) && rows_in ? (left < kFeat / 32 ? left : kFeat / 32) : 0;
-      auto ask_dh = [&](int j) {  // load dh block j of the tile; its buffer's readers are done
-        if (lane == 0) {
-          uint64_t* bar = &dh_bar[dh_asked & 1];
-          fence_async();
-          mbar_expect_tx(bar, kEpi == kGatedBwdF32 ? kDhBlock : kDhBlock / 2);
-          load_2d(out + (dh_asked & 1) * kDhBlock, &maps.dh, bar, col0 + 32 * j, row0);
-        }
-        ++dh_asked;
-      };
-      if constexpr (is_bwd(kEpi)) {  // two blocks come in while the MMAs run
-        for (int j = 0; j < 2 && j < blocks; ++j) ask_dh(j);
+      const int col0 = is_plain(kEpi) ? bn * BN + half * kWarpCols : bn * kFeat + half * (kFeat / 2);
+      const bool in = row0 < g.M && col0 < g.N;  // some of this warp's outputs exist
+      float dh[32];
+      if constexpr (is_bwd(kEpi)) {
+        if (in) load_dh<kEpi, kF16>(g, row0 + lane, col0, dh);  // arrives while the MMAs run
       }
       int ok = 0;
       if (lane == 0) ok = mbar_wait(&acc_full[a], (it >> 1) & 1, abort_flag, g.fault.limit_ns) && !*abort_flag;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t acc = tmem + (uint32_t)(a * BN) + ((uint32_t)(q * 32) << 16);
-      if constexpr (kEpi == kPlainF32) {
-        for (int c = 0; c < BN; c += 32) {
-          if (!rows_in || col0 + c >= g.N) break;  // warp-uniform
-          uint8_t* tile = out + buf * kStoreTile;
-          buf ^= 1;
-          if (lane == 0) store_wait_read<1>();  // the store before last has read this tile
-          __syncwarp();
+      // this warp's accumulator columns: plain 0..127 from here; gated g at 0..63, u at kFeat..
+      const uint32_t acc = tmem + (uint32_t)(a * BN) + ((uint32_t)(q * 32) << 16) +
+                           (uint32_t)(half * (is_plain(kEpi) ? kWarpCols : kFeat / 2));
+      // its partial of piece i: float4 j of lane l at j * 32 + l
+      auto partial = [&](int i) {
+        return reinterpret_cast<float4*>(g.partials) +
+               ((int64_t)(item.tile * item.ways + i) * 2 * kEpiWarps + w16) * (kWarpPartial / 4) + lane;
+      };
+      // 32 accumulator columns: block b (0..3) of this warp's 128, joined over the pieces
+      auto tmem_block = [&](int b) {
+        return acc + (uint32_t)(is_plain(kEpi) ? 32 * b : 32 * (b & 1) + kFeat * (b >> 1));
+      };
+      bool finish = in;
+      if (item.ways > 1 && in) {
+        float4* mine = partial(item.own);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
           uint32_t r[32];
-          tmem_ld32(acc + (uint32_t)c, r);
+          tmem_ld32(tmem_block(b), r);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            *tile_chunk(tile, lane, k) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
-          fence_async();
-          __syncwarp();
-          if (lane == 0) {
-            store_2d(&maps.o[prob], tile, col0 + c, row0);
-            store_commit();
-          }
+            mine[(b * 8 + k) * 32] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
+                                                 __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
         }
-      } else if constexpr (kEpi == kPlain || kEpi == kGated) {
-        constexpr int kCols = kEpi == kPlain ? BN : kFeat;
-        for (int c = 0; c < kCols; c += 64) {
-          if (!rows_in || col0 + c >= g.N) break;  // warp-uniform
-          uint8_t* tile = out + buf * kStoreTile;
-          buf ^= 1;
-          if (lane == 0) store_wait_read<1>();  // the store before last has read this tile
-          __syncwarp();
+        finish = arrive_last(g.counters + item.tile * 2 * kEpiWarps + w16, item.ways, lane);
+      }
+      // kNb blocks at once, so that as many partial loads are in flight
+      auto fetch = [&](auto nb, const int (&b)[decltype(nb)::value], float* v) {
+        constexpr int kNb = decltype(nb)::value;
+        uint32_t r[kNb][32];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            float v[32];
-            if constexpr (kEpi == kPlain) {
-              uint32_t r[32];
-              tmem_ld32(acc + (uint32_t)(c + half * 32), r);
+        for (int n = 0; n < kNb; ++n) tmem_ld32(tmem_block(b[n]), r[n]);
+        if (item.ways == 1) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-            } else {
-              uint32_t rg[32], ru[32];
-              tmem_ld32_nowait(acc + (uint32_t)(c + half * 32), rg);
-              tmem_ld32(acc + (uint32_t)(kFeat + c + half * 32), ru);
+          for (int n = 0; n < kNb; ++n)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = gated(__uint_as_float(rg[j]), __uint_as_float(ru[j]), g.act);
-            }
-            put_row<kF16>(tile, lane, half * 4, v);
-          }
-          fence_async();
-          __syncwarp();
-          if (lane == 0) {
-            store_2d(&maps.o[prob], tile, col0 + c, row0);
-            store_commit();
-          }
+            for (int j = 0; j < 32; ++j) v[n * 32 + j] = __uint_as_float(r[n][j]);
+          return;
         }
-      } else {
-        uint8_t* tdg = out + 2 * kDhBlock;
-        uint8_t* tdu = tdg + kOutBlock;
-        uint8_t* th = tdu + kOutBlock;
-        for (int j = 0; j < blocks; ++j) {
-          uint8_t* tdh = out + (dh_read & 1) * kDhBlock;
-          // every lane waits, so that each sees the loaded bytes (bounded)
-          if (!__all_sync(0xffffffffu, mbar_wait(&dh_bar[dh_read & 1], (dh_read >> 1) & 1, abort_flag,
-                                                 g.fault.limit_ns))) {
-            ok = 0;
-            break;
-          }
-          ++dh_read;
-          uint32_t rg[32], ru[32];
-          tmem_ld32_nowait(acc + (uint32_t)(32 * j), rg);
-          tmem_ld32(acc + (uint32_t)(kFeat + 32 * j), ru);
-          if (lane == 0) store_wait_read<0>();  // the block before has been read out
-          __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // 8 features each
-            float dh[8];
-            if constexpr (kEpi == kGatedBwdF32) {
+        for (int j = 0; j < kNb * 32; ++j) v[j] = 0.0f;
+        for (int i = 0; i < item.ways; ++i) {
+          if (i == item.own) {
 #pragma unroll
-              for (int p = 0; p < 2; ++p) {
-                const uint4 w = *tile_chunk(tdh, lane, 2 * k + p);
-                dh[4 * p] = __uint_as_float(w.x); dh[4 * p + 1] = __uint_as_float(w.y);
-                dh[4 * p + 2] = __uint_as_float(w.z); dh[4 * p + 3] = __uint_as_float(w.w);
+            for (int n = 0; n < kNb; ++n)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[n * 32 + j] += __uint_as_float(r[n][j]);
+          } else {
+            const float4* src = partial(i);
+            float4 x[kNb][8];
+#pragma unroll
+            for (int n = 0; n < kNb; ++n)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[n][k] = __ldcg(src + (b[n] * 8 + k) * 32);
+#pragma unroll
+            for (int n = 0; n < kNb; ++n)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                float* o = v + n * 32 + 4 * k;
+                o[0] += x[n][k].x; o[1] += x[n][k].y; o[2] += x[n][k].z; o[3] += x[n][k].w;
               }
-            } else {
-              const uint4 w = *block_chunk(tdh, lane, k);
-              const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          }
+        }
+      };
+      if (finish) {
+        if constexpr (kEpi == kPlainF32) {
+          for (int b = 0; b < 4; ++b) {
+            if (col0 + 32 * b >= g.N) break;  // warp-uniform
+            float v[32];
+            fetch(Int<1>{}, {b}, v);
+            if (lane == 0) store_wait_read<0>();  // the store before has read this tile
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              *tile_chunk(out, lane, k) = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
+                                                     __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3]));
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+              store_2d(&maps.o[prob], out, col0 + 32 * b, row0);
+              store_commit();
+            }
+          }
+        } else if constexpr (kEpi == kPlain) {
+          for (int b = 0; b < 4; b += 2) {
+            if (col0 + 32 * b >= g.N) break;  // warp-uniform
+            float v[64];
+            fetch(Int<2>{}, {b, b + 1}, v);
+            if (lane == 0) store_wait_read<0>();
+            __syncwarp();
+            put_row<kF16>(out, lane, 0, v);
+            put_row<kF16>(out, lane, 4, v + 32);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+              store_2d(&maps.o[prob], out, col0 + 32 * b, row0);
+              store_commit();
+            }
+          }
+        } else if constexpr (kEpi == kGated) {
+          if (lane == 0) store_wait_read<0>();  // the tile before has been read out
+          __syncwarp();
+#pragma unroll 1
+          for (int b = 0; b < 2; ++b) {
+            float v[64];
+            fetch(Int<2>{}, {b, b + 2}, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = gated(v[j], v[32 + j], g.act);
+            put_row<kF16>(out, lane, 4 * b, v);
+          }
+          fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            store_2d(&maps.o[0], out, col0, row0);
+            store_commit();
+          }
+        } else {
+          uint8_t* tdg = out;
+          uint8_t* tdu = tdg + kOutBlock;
+          uint8_t* th = tdu + kOutBlock;
+#pragma unroll 1
+          for (int b = 0; b < 2; ++b) {
+            if (col0 + 32 * b >= g.N) break;  // warp-uniform
+            float v[64];
+            fetch(Int<1>{}, {b}, v);  // one at a time: dh holds the registers of a second
+            fetch(Int<1>{}, {b + 2}, v + 32);
+            if (lane == 0) store_wait_read<0>();  // the block before has been read out
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // 8 features each
+              uint32_t og[4], ou[4], oh[4];
 #pragma unroll
               for (int p = 0; p < 4; ++p) {
-                dh[2 * p] = h2f<kF16>((uint16_t)(ww[p] & 0xffffu));
-                dh[2 * p + 1] = h2f<kF16>((uint16_t)(ww[p] >> 16));
+                float dg[2], du[2], h[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int j = k * 8 + p * 2 + e;
+                  gated_bwd(v[j], v[32 + j], dh[j], g.act, dg[e], du[e], h[e]);
+                }
+                og[p] = pack2<kF16>(dg[0], dg[1]);
+                ou[p] = pack2<kF16>(du[0], du[1]);
+                oh[p] = pack2<kF16>(h[0], h[1]);
               }
+              *block_chunk(tdg, lane, k) = make_uint4(og[0], og[1], og[2], og[3]);
+              *block_chunk(tdu, lane, k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+              *block_chunk(th, lane, k) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
             }
-            uint32_t og[4], ou[4], oh[4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              float dg[2], du[2], h[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                gated_bwd(__uint_as_float(rg[k * 8 + p * 2 + e]), __uint_as_float(ru[k * 8 + p * 2 + e]),
-                          dh[2 * p + e], g.act, dg[e], du[e], h[e]);
-              og[p] = pack2<kF16>(dg[0], dg[1]);
-              ou[p] = pack2<kF16>(du[0], du[1]);
-              oh[p] = pack2<kF16>(h[0], h[1]);
+            if (b == 0 && col0 + 32 < g.N) load_dh<kEpi, kF16>(g, row0 + lane, col0 + 32, dh);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+              const int col = col0 + 32 * b;
+              store_2d(&maps.o[0], tdg, col, row0);
+              store_2d(&maps.o[1], tdu, col, row0);
+              if (g.want_h) store_2d(&maps.o[2], th, col, row0);
+              store_commit();
             }
-            *block_chunk(tdg, lane, k) = make_uint4(og[0], og[1], og[2], og[3]);
-            *block_chunk(tdu, lane, k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
-            *block_chunk(th, lane, k) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
           }
-          fence_async();
-          __syncwarp();
-          if (lane == 0) {
-            const int col = col0 + 32 * j;
-            store_2d(&maps.o[0], tdg, col, row0);
-            store_2d(&maps.o[1], tdu, col, row0);
-            if (g.want_h) store_2d(&maps.o[2], th, col, row0);
-            store_commit();
-          }
-          if (j + 2 < blocks) ask_dh(j + 2);
         }
-        if (!ok) break;
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[a]), 0));
     }
-    if (lane == 0) {
-      store_wait_all();
-      // on abort: bounded wait for dh blocks still in flight
-      const uint64_t t0 = globaltimer();
-      for (; dh_read < dh_asked; ++dh_read)
-        while (!mbar_try_wait(&dh_bar[dh_read & 1], (dh_read >> 1) & 1) && globaltimer() - t0 < g.fault.limit_ns) {
-        }
-    }
+    if (lane == 0) store_wait_all();
     __syncwarp();
   }
   tc_fence_before();
@@ -544,8 +695,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
 constexpr int kSkinnyThreads = 128;
 
 struct SkinnyArgs {
-  int tokens;     // all tokens; blockIdx.y picks a tile of n
-  int n;          // tokens of a tile, padded to a multiple of 16 (MMA N)
+  int tokens;     // M of the product
+  int n;          // tokens padded to a multiple of 16 (MMA N)
   int rows;       // output features
   int kb, nseg;   // 64-deep blocks of one K segment; segments
   int split;      // cluster CTAs sharing one tile's contraction
@@ -560,10 +711,26 @@ struct SkinnyArgs {
   FaultPlan fault;  // test-only: a CTA whose first k-block is withheld, and the launch's wait bound
 };
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
+}
+
+// Four consecutive 16-bit values (8-byte aligned when all four exist).
+template <bool kF16>
+__device__ __forceinline__ void store_quad(void* p, int64_t e, int n, const float (&v)[4]) {
+  uint16_t* o = static_cast<uint16_t*>(p) + e;
+  if (n == 4) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<kF16>(v[0], v[1]), pack2<kF16>(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) o[j] = f2h<kF16>(v[j]);
+  }
 }
 
 template <int kEpi, bool kAMn, bool kF16>
@@ -582,7 +749,6 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = g.split > 1 ? (int)cluster_rank() : 0;
   const int tile = (int)blockIdx.x / g.split;
-  const int tok0 = (int)blockIdx.y * g.n;
   const int KB = g.kb * g.nseg;
   const int k_lo = (int)((int64_t)KB * rank / g.split), k_hi = (int)((int64_t)KB * (rank + 1) / g.split);
   const int feat0 = tile * (is_plain(kEpi) ? 128 : 64);
@@ -606,15 +772,12 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
 
   if (warp == 0 && lane == 0) {
-    int kit = 0;
-    for (int k = k_lo; k < k_hi; ++k, ++kit) {
-      const int s = kit % g.st;
-      if (!mbar_wait(&empty[s], ((kit / g.st) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
-      if ((int)blockIdx.x == g.fault.unit && kit == 0) continue;  // test-only, as in the pair kernel
-      const int seg = k >= g.kb ? 1 : 0;
-      const int k0 = (k - seg * g.kb) * BK;
+    const bool withhold = (int)blockIdx.x == g.fault.unit;  // test-only; the MMA thread's wait expires
+    auto load_weights = [&](int s, int k) {
+      const int seg = k >= g.kb ? 1 : 0, k0 = (k - seg * g.kb) * BK;
       mbar_expect_tx(&full[s], kTileA + tile_b);
       uint8_t* a = sA + s * kTileA;
       if constexpr (kAMn) {
@@ -622,12 +785,29 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
         load_2d(a + kBox, &maps.a[seg], &full[s], feat0 + 64, k0);
       } else if constexpr (is_plain(kEpi)) {
         load_2d(a, &maps.a[seg], &full[s], k0, feat0);
-        load_2d(a + kBox, &maps.a[seg], &full[s], k0, feat0 + 64);
       } else {  // 64 gate rows, then the same 64 up rows
         load_2d(a, &maps.a[0], &full[s], k0, feat0);
         load_2d(a + kBox, &maps.a[1], &full[s], k0, feat0);
       }
-      load_2d(sB + s * tile_b, &maps.b[seg], &full[s], k0, tok0);
+    };
+    auto load_tokens = [&](int s, int k) {
+      const int seg = k >= g.kb ? 1 : 0;
+      load_2d(sB + s * tile_b, &maps.b[seg], &full[s], (k - seg * g.kb) * BK, 0);
+    };
+    // the ring's first round: weights at once, tokens when the kernels before have written them
+    const int head = k_hi - k_lo < g.st ? k_hi - k_lo : g.st;
+    for (int i = withhold ? 1 : 0; i < head; ++i) load_weights(i, k_lo + i);
+    pdl_wait();
+    int kit = 0;
+    for (int k = k_lo; k < k_hi; ++k, ++kit) {
+      const int s = kit % g.st;
+      if (kit >= head) {
+        if (!mbar_wait(&empty[s], ((kit / g.st) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
+        load_weights(s, k);
+      } else if (withhold && kit == 0) {
+        continue;
+      }
+      load_tokens(s, k);
     }
     if (*abort_flag) {  // bounded wait for this CTA's loads in flight
       const uint64_t t0 = globaltimer();
@@ -661,20 +841,15 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   }
   __syncthreads();  // the producer's and the MMA thread's waits have ended too
   tc_fence_after();
-  const int here = g.tokens - tok0 < g.n ? g.tokens - tok0 : g.n;
-  float* part = reinterpret_cast<float*>(smem);  // [token][128 features]
-  for (int c = 0; c < here; c += 16) {
+  // [token][128 features], rows 16 bytes apart from a multiple of 128 B
+  constexpr int kPitch = 132;
+  float* part = reinterpret_cast<float*>(smem);
+  for (int c = 0; c < g.tokens; c += 16) {
     uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, r);
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (c + j < here) part[(c + j) * 128 + warp * 32 + lane] = k_hi > k_lo ? __uint_as_float(r[j]) : 0.0f;
+      if (c + j < g.tokens) part[(c + j) * kPitch + warp * 32 + lane] = __uint_as_float(r[j]);
   }
   tc_fence_before();
   if (g.split > 1) cluster_sync();
@@ -684,36 +859,54 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
   }
   if (!*abort_flag) {
-    // the tile's (token, feature) pairs, dealt to the cluster's threads; a pair's
+    pdl_wait();  // before the first access to what the kernels before may write or read
+    // the tile's (token, 4 features) groups, dealt to the cluster's threads; a group's
     // partials are added in rank order
-    constexpr int kPer = is_plain(kEpi) ? 128 : 64;
-    const int items = here * kPer;
+    constexpr int kPer = is_plain(kEpi) ? 32 : 16;
+    const int items = g.tokens * kPer;
     const uint32_t base = smem_u32(part);
     for (int i = rank * kSkinnyThreads + (int)threadIdx.x; i < items; i += g.split * kSkinnyThreads) {
-      const int j = i / kPer, feat = i % kPer;
-      if (feat0 + feat >= g.rows) continue;
-      float v = 0.0f, w = 0.0f;
+      const int j = i / kPer, f4 = (i % kPer) * 4;
+      const int64_t tok = j, col = feat0 + f4;
+      const int n = g.rows - (feat0 + f4) < 4 ? g.rows - (feat0 + f4) : 4;
+      if (n <= 0) continue;
+      float v[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t at = base + (uint32_t)(j * kPitch + f4) * 4u;
+#pragma unroll 4
       for (int r = 0; r < g.split; ++r) {
-        const uint32_t p = (g.split > 1 ? mapa_u32(base, (uint32_t)r) : base) + (uint32_t)(j * 128 + feat) * 4u;
-        v += ld_cluster_f32(p);
-        if constexpr (!is_plain(kEpi)) w += ld_cluster_f32(p + 64 * 4);
+        const uint32_t p = g.split > 1 ? mapa_u32(at, (uint32_t)r) : at;
+        const float4 x = ld_cluster_f32x4(p);
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+        if constexpr (!is_plain(kEpi)) {
+          const float4 y = ld_cluster_f32x4(p + 64 * 4);
+          w[0] += y.x; w[1] += y.y; w[2] += y.z; w[3] += y.w;
+        }
       }
-      const int64_t tok = tok0 + j, col = feat0 + feat;
       if constexpr (kEpi == kPlain) {
-        static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(v);
+        store_quad<kF16>(g.o0, tok * g.ldo + col, n, v);
       } else if constexpr (kEpi == kPlainF32) {
-        static_cast<float*>(g.o0)[tok * g.ldo + col] = v;
+        float* o = static_cast<float*>(g.o0) + tok * g.ldo + col;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < n) o[e] = v[e];
       } else if constexpr (kEpi == kGated) {
-        static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(gated(v, w, g.act));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = gated(v[e], w[e], g.act);
+        store_quad<kF16>(g.o0, tok * g.ldo + col, n, v);
       } else {
-        float dg, du, h;
-        float dh;
-        if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[tok * g.lddh + col];
-        else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col]);
-        gated_bwd(v, w, dh, g.act, dg, du, h);
-        static_cast<uint16_t*>(g.o0)[tok * g.ldo + col] = f2h<kF16>(dg);
-        static_cast<uint16_t*>(g.o1)[tok * g.ldu + col] = f2h<kF16>(du);
-        if (g.o2 != nullptr) static_cast<uint16_t*>(g.o2)[tok * g.ldh + col] = f2h<kF16>(h);
+        float dg[4], du[4], h[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float dh = 0.0f;
+          if (e < n) {
+            if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[tok * g.lddh + col + e];
+            else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col + e]);
+          }
+          gated_bwd(v[e], w[e], dh, g.act, dg[e], du[e], h[e]);
+        }
+        store_quad<kF16>(g.o0, tok * g.ldo + col, n, dg);
+        store_quad<kF16>(g.o1, tok * g.ldu + col, n, du);
+        if (g.o2 != nullptr) store_quad<kF16>(g.o2, tok * g.ldh + col, n, h);
       }
     }
   }
@@ -758,6 +951,10 @@ struct Product {
 };
 
 constexpr int kMaxDevices = 64;
+constexpr int kSkinnyWaves = 1;
+// When a pair launch cuts its last round: pieces of at least kMinPieceKb k-blocks, at
+// most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time.
+constexpr int kMinPieceKb = 4, kMaxWays = 8, kMinSavedKb = 16;
 
 struct KernelEntry {
   std::once_flag once[kMaxDevices];
@@ -778,26 +975,66 @@ int current_device(int* sms) {
   return dev;
 }
 
-cudaLaunchConfig_t cluster_config(cudaLaunchAttribute* at, dim3 grid, int threads, int smem, int cluster,
-                                  cudaStream_t stream) {
+// What the products of one call share.
+struct Ctx {
+  cudaStream_t stream;
+  float* partials;    // pair products: the pieces of cut tiles
+  int32_t* counters;  // ... and their counters
+  bool zeroed;        // the counters have been cleared
+  bool chained;       // the kernel before on the stream belongs to this call
+};
+
+cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int threads, int smem, int cluster,
+                                 const Ctx* ctx) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3((unsigned)grid, 1, 1);
   cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
+  cfg.stream = ctx ? ctx->stream : nullptr;
+  cfg.attrs = at;
   if (cluster > 1) {
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)cluster;
-    at[0].val.clusterDim.y = 1;
-    at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    at[cfg.numAttrs].val.clusterDim.y = 1;
+    at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (ctx && ctx->chained) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
   }
   return cfg;
 }
 
+constexpr int kMaxPairs = 96;  // pairs a launch may have, for the size of its workspace
+// Tokens up to which the weight-streaming kernel runs.
+constexpr int64_t kSkinnyTokens = 64;
+constexpr int kCounters = kMaxPairs * 2 * kEpiWarps;
+constexpr size_t kJoinBytes = kCounters * sizeof(int32_t) + (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial * 4;
+static_assert(kJoinBytes % 256 == 0, "what follows stays aligned");
+
+// The workspace's joining part; a call whose products are all skinny has none.
+size_t join_bytes(int64_t tokens) { return tokens <= kSkinnyTokens ? 0 : kJoinBytes; }
+
+// Deal `tiles` tiles of kb k-blocks over at most `most` pairs: full rounds of whole
+// tiles, and the last round's tiles cut when that saves enough.
+Sched make_sched(int tiles, int kb, int most) {
+  Sched s{tiles, kb, tiles < most ? tiles : most, 0, 1};
+  const int rest = tiles % most;
+  if (rest == 0) return s;
+  int ways = most / rest;
+  if (ways > kMaxWays) ways = kMaxWays;
+  if (ways > kb / kMinPieceKb) ways = kb / kMinPieceKb;
+  if (ways < 2 || kb - kb / ways < kMinSavedKb) return s;
+  s.cut_tiles = rest;
+  s.ways = ways;
+  s.units = tiles > most ? most : rest * ways;
+  return s;
+}
+
 template <int kEpi, bool kAMn, bool kBMn, bool kF16>
-int launch_pair(const Product& q, cudaStream_t stream) {
+int launch_pair(const Product& q, Ctx& ctx) {
   auto kernel = &k_ffn_pair<kEpi, kAMn, kBMn, kF16>;
   constexpr int smem = pair_smem(kEpi);
   constexpr CUtensorMapDataType t16 = kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -809,11 +1046,11 @@ int launch_pair(const Product& q, cudaStream_t stream) {
   std::call_once(entry.once[dev], [&] {
     entry.rc[dev] = MB_ERR_CUDA;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return;
-    cudaLaunchAttribute at[1];
-    cudaLaunchConfig_t occ = cluster_config(at, dim3((unsigned)(2 * (sms / 2))), kPairThreads, smem, 2, nullptr);
+    cudaLaunchAttribute at[2];
+    cudaLaunchConfig_t occ = launch_config(at, 2 * (sms / 2), kPairThreads, smem, 2, nullptr);
     int c = 0;
     if (cudaOccupancyMaxActiveClusters(&c, kernel, &occ) != cudaSuccess || c <= 0) return;
-    entry.pairs[dev] = c;
+    entry.pairs[dev] = c < kMaxPairs ? c : kMaxPairs;
     entry.rc[dev] = MB_OK;
   });
   if (entry.rc[dev] != MB_OK) return entry.rc[dev];
@@ -830,8 +1067,6 @@ int launch_pair(const Product& q, cudaStream_t stream) {
     if (q.o[i].p)
       ok = ok && map_2d(&m.o[i], f32_out ? t32 : t16, q.o[i].p, q.o[i].rows, q.o[i].cols, q.o[i].ld,
                         f32_out || is_bwd(kEpi) ? 32 : 64, 32);
-  if (is_bwd(kEpi))
-    ok = ok && map_2d(&m.dh, kEpi == kGatedBwdF32 ? t32 : t16, q.dh.p, q.dh.rows, q.dh.cols, q.dh.ld, 32, 32);
   if (!ok) return MB_ERR_CUDA;
   const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), cols = is_plain(kEpi) ? BN : kFeat;
   const int64_t nt = (q.N + cols - 1) / cols;
@@ -843,21 +1078,30 @@ int launch_pair(const Product& q, cudaStream_t stream) {
   g.kb = (int)kb; g.nseg = q.nseg; g.nprob = q.nprob;
   g.mt = (int)mt; g.nt = (int)nt;
   g.act = q.act; g.want_h = q.o[2].p != nullptr;
+  g.dh = q.dh.p; g.lddh = q.dh.ld;
   take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
-  const int units = (int)(work < entry.pairs[dev] ? work : entry.pairs[dev]);
-  cudaLaunchAttribute at[1];
-  cudaLaunchConfig_t cfg = cluster_config(at, dim3((unsigned)(2 * units)), kPairThreads, smem, 2, stream);
+  g.sched = make_sched((int)work, (int)(kb * q.nseg), entry.pairs[dev]);
+  if (g.sched.ways > 1) {
+    if (!ctx.zeroed) {  // once a call: the last piece of a tile leaves its counters at zero
+      cudaLaunchAttribute zat[2];
+      cudaLaunchConfig_t zero = launch_config(zat, 1, 512, 0, 1, &ctx);
+      if (cudaLaunchKernelEx(&zero, k_zero, ctx.counters, kCounters) != cudaSuccess) return MB_ERR_CUDA;
+      ctx.zeroed = ctx.chained = true;
+    }
+    g.partials = ctx.partials;
+    g.counters = ctx.counters;
+  }
+  cudaLaunchAttribute at[2];
+  cudaLaunchConfig_t cfg = launch_config(at, 2 * g.sched.units, kPairThreads, smem, 2, &ctx);
   return cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
 }
 
-// Tokens up to which the weight-streaming kernel runs.
-constexpr int64_t kSkinnyTokens = 256;
-constexpr int kSkinnyRing = 200 * 1024;      // ring bytes of a CTA that has an SM to itself
-constexpr int kSkinnyRingHalf = 110 * 1024;  // ... of one that shares it
-constexpr int kSkinnyMaxSmem = kSkinnyRing + 1024 + kBarBytes;
+// Shared memory of a skinny CTA: kSkinnyPerSm of them share an SM's 228 KB.
+constexpr int kSkinnyPerSm = 3;
+constexpr int kSkinnySmem = (228 / kSkinnyPerSm - 1) * 1024;
 
 template <int kEpi, bool kAMn, bool kF16>
-int launch_skinny(const Product& q, cudaStream_t stream) {
+int launch_skinny(const Product& q, const Ctx& ctx) {
   // q is given as in the pair form (a: tokens, b: weights); the MMA swaps them
   auto kernel = &k_ffn_skinny<kEpi, kAMn, kF16>;
   static KernelEntry entry;
@@ -865,34 +1109,27 @@ int launch_skinny(const Product& q, cudaStream_t stream) {
   const int dev = current_device(&sms);
   if (dev < 0) return MB_ERR_CUDA;
   std::call_once(entry.once[dev], [&] {
-    entry.rc[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnyMaxSmem) ==
+    entry.rc[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnySmem) ==
                             cudaSuccess
                         ? MB_OK
                         : MB_ERR_CUDA;
   });
   if (entry.rc[dev] != MB_OK) return entry.rc[dev];
   SkinnyArgs g{};
-  const int64_t T = q.M;
-  g.tokens = (int)T;
-  g.n = T >= 256 ? 256 : (int)((T + 15) / 16 * 16);
+  g.tokens = (int)q.M;
+  g.n = (int)((q.M + 15) / 16 * 16);
   g.rows = (int)q.N;
-  const int64_t kb = (q.K + BK - 1) / BK;
-  if (kb * q.nseg > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+  constexpr int kPer = is_plain(kEpi) ? 128 : 64;
+  const int64_t kb = (q.K + BK - 1) / BK, tiles = (q.N + kPer - 1) / kPer, KB = kb * q.nseg;
+  if (KB > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
   g.kb = (int)kb; g.nseg = q.nseg;
-  const int64_t per = is_plain(kEpi) ? 128 : 64;
-  const int64_t tiles = (q.N + per - 1) / per, ytiles = (T + g.n - 1) / g.n;
-  const int64_t KB = kb * q.nseg;
-  // Split the contraction until the launch has two CTAs for every SM, as long as
-  // a CTA keeps four k-blocks.
+  // Split the contraction until the launch has about kSkinnyWaves CTAs for every place
+  // on the GPU (enough that the last of them to start does not decide its time), as
+  // long as a CTA keeps four k-blocks.
   g.split = 1;
-  while (g.split < 8 && tiles * ytiles * g.split < 2 * sms && KB / (2 * g.split) >= 4) g.split *= 2;
-  // Two CTAs share an SM's memory while tokens are few; wide token tiles take it whole.
+  while (g.split < 8 && tiles * g.split < kSkinnyWaves * kSkinnyPerSm * sms && KB / (2 * g.split) >= 4) g.split *= 2;
   const int stage = kTileA + g.n * BK * 2;
-  const int64_t mine = (KB + g.split - 1) / g.split;
-  g.st = (g.n <= 64 ? kSkinnyRingHalf : kSkinnyRing) / stage;
-  if (g.st > mine) g.st = (int)mine;
-  const int need = g.n * 128 * 4;  // the partials reuse the ring
-  while (g.st * stage < need) ++g.st;
+  g.st = (kSkinnySmem - 1024 - kBarBytes) / stage;  // the partials fit the same ring
   g.tmem_cols = 32;
   while ((int)g.tmem_cols < g.n) g.tmem_cols *= 2;
   g.act = q.act;
@@ -901,7 +1138,8 @@ int launch_skinny(const Product& q, cudaStream_t stream) {
   const int nw = is_plain(kEpi) ? q.nseg : 2;
   constexpr CUtensorMapDataType t16 = kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   for (int i = 0; i < nw; ++i)
-    ok = ok && map_2d(&m.a[i], t16, q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, 64);
+    ok = ok && map_2d(&m.a[i], t16, q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64,
+                      is_plain(kEpi) && !kAMn ? 128 : 64);
   for (int i = 0; i < q.nseg; ++i)
     ok = ok && map_2d(&m.b[i], t16, q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, g.n);
   if (!ok) return MB_ERR_CUDA;
@@ -910,16 +1148,14 @@ int launch_skinny(const Product& q, cudaStream_t stream) {
   g.o2 = const_cast<void*>(q.o[2].p); g.ldh = q.o[2].ld;
   g.dh = q.dh.p; g.lddh = q.dh.ld;
   take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
-  if (tiles * g.split > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
-  cudaLaunchAttribute at[1];
-  const int smem = g.st * stage + 1024 + kBarBytes;
-  cudaLaunchConfig_t cfg = cluster_config(at, dim3((unsigned)(tiles * g.split), (unsigned)ytiles), kSkinnyThreads, smem,
-                                          g.split, stream);
+  cudaLaunchAttribute at[2];
+  cudaLaunchConfig_t cfg =
+      launch_config(at, (int)(tiles * g.split), kSkinnyThreads, kSkinnySmem, g.split, &ctx);
   return cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
 }
 
 template <bool kF16>
-int run_product(const Product& q, cudaStream_t st) {
+int run_product(const Product& q, Ctx& st) {
   const bool skinny = !q.a_mn && q.M <= kSkinnyTokens;
   if (q.epi == kGated) return skinny ? launch_skinny<kGated, false, kF16>(q, st) : launch_pair<kGated, false, false, kF16>(q, st);
   if (q.epi == kGatedBwd)
@@ -934,8 +1170,16 @@ int run_product(const Product& q, cudaStream_t st) {
   return skinny ? launch_skinny<kPlain, false, kF16>(q, st) : launch_pair<kPlain, false, false, kF16>(q, st);
 }
 
-int product(int dtype, const Product& q, cudaStream_t st) {
-  return dtype == MB_F16 ? run_product<true>(q, st) : run_product<false>(q, st);
+int product(int dtype, const Product& q, Ctx& ctx) {
+  const int rc = dtype == MB_F16 ? run_product<true>(q, ctx) : run_product<false>(q, ctx);
+  ctx.chained = true;
+  return rc;
+}
+
+// The call's context over the joining part of its workspace (its first kJoinBytes).
+Ctx make_ctx(void* workspace, cudaStream_t stream) {
+  int32_t* counters = static_cast<int32_t*>(workspace);
+  return {stream, reinterpret_cast<float*>(counters + kCounters), counters, false, false};
 }
 
 constexpr int64_t kMaxDim = (int64_t)1 << 30;
@@ -988,20 +1232,29 @@ using namespace mb::ffn;
 
 extern "C" {
 
-MB_API int mb_gated_linear(const mb_ffn_args* a, void* h, int64_t ldh, mb_stream_t stream) {
+MB_API size_t mb_gated_linear_workspace_bytes(int64_t tokens) {
+  return tokens <= 0 || tokens > kMaxDim ? 0 : join_bytes(tokens);
+}
+
+MB_API int mb_gated_linear(const mb_ffn_args* a, void* h, int64_t ldh, void* workspace, size_t workspace_bytes,
+                           mb_stream_t stream) {
   int rc = check_args(a, true, false);
   if (rc != MB_OK) return rc;
   if (a->tokens == 0) return MB_OK;
   rc = check_mat(h, a->f, ldh);
   if (rc != MB_OK) return rc;
+  const size_t need = mb_gated_linear_workspace_bytes(a->tokens);
+  if ((need > 0 && !workspace) || workspace_bytes < need) return MB_ERR_ARG;
+  if (!aligned(workspace, 256)) return MB_ERR_ALIGN;
+  Ctx ctx = make_ctx(workspace, (cudaStream_t)stream);
   Product q = gated_product(a, {a->x, a->tokens, a->d, a->ldx});
   q.o[0] = {h, a->tokens, a->f, ldh};
-  return product(a->dtype, q, (cudaStream_t)stream);
+  return product(a->dtype, q, ctx);
 }
 
 MB_API size_t mb_feed_forward_workspace_bytes(int64_t tokens, int64_t f) {
   if (tokens <= 0 || f <= 0 || tokens > kMaxDim || f > kMaxDim) return 0;
-  return area(tokens, f);
+  return join_bytes(tokens) + area(tokens, f);
 }
 
 MB_API int mb_feed_forward(const mb_ffn_args* a, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
@@ -1012,25 +1265,26 @@ MB_API int mb_feed_forward(const mb_ffn_args* a, void* y, int64_t ldy, void* wor
   rc = check_mat(y, a->d, ldy);
   if (rc != MB_OK) return rc;
   if (!workspace || workspace_bytes < mb_feed_forward_workspace_bytes(a->tokens, a->f)) return MB_ERR_ARG;
-  if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
-  const Mat h{workspace, a->tokens, a->f, pad8(a->f)};
+  if (!aligned(workspace, 256)) return MB_ERR_ALIGN;
+  Ctx ctx = make_ctx(workspace, (cudaStream_t)stream);
+  const Mat h{static_cast<uint8_t*>(workspace) + join_bytes(a->tokens), a->tokens, a->f, pad8(a->f)};
   Product q = gated_product(a, {a->x, a->tokens, a->d, a->ldx});
   q.o[0] = h;
-  rc = product(a->dtype, q, (cudaStream_t)stream);
+  rc = product(a->dtype, q, ctx);
   if (rc != MB_OK) return rc;
   Product p;
   p.a[0] = h;
   p.b[0] = {a->down, a->d, a->f, a->ld_down};
   p.o[0] = {y, a->tokens, a->d, ldy};
   p.M = a->tokens; p.N = a->d; p.K = a->f;
-  return product(a->dtype, p, (cudaStream_t)stream);
+  return product(a->dtype, p, ctx);
 }
 
 MB_API size_t mb_feed_forward_backward_workspace_bytes(int64_t tokens, int64_t d, int64_t f, int32_t from_codes,
                                                        int32_t with_down) {
   if (tokens <= 0 || d <= 0 || f <= 0 || tokens > kMaxDim || d > kMaxDim || f > kMaxDim) return 0;
-  // dg, du; with down: h and an FP32 dh
-  return (with_down ? 5 : 2) * area(tokens, f) + (from_codes ? area(tokens, d) : 0);
+  // the weight gradients always run on pairs; dg, du; with down: h and an FP32 dh
+  return kJoinBytes + (with_down ? 5 : 2) * area(tokens, f) + (from_codes ? area(tokens, d) : 0);
 }
 
 MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r, void* workspace,
@@ -1059,8 +1313,9 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
   if (!workspace ||
       workspace_bytes < mb_feed_forward_backward_workspace_bytes(T, d, f, from_codes ? 1 : 0, down ? 1 : 0))
     return MB_ERR_ARG;
-  if (!aligned(workspace, 16)) return MB_ERR_ALIGN;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (!aligned(workspace, 256)) return MB_ERR_ALIGN;
+  uint8_t* ws = static_cast<uint8_t*>(workspace) + kJoinBytes;
+  Ctx ctx = make_ctx(workspace, st);
   const int64_t fp = pad8(f);
   const Mat dg{ws, T, f, fp}, du{ws + area(T, f), T, f, fp};
   Mat dh{r->dy, T, f, r->lddy}, h;
@@ -1085,7 +1340,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     q.b_mn = true;
     q.o[0] = dh;
     q.M = T; q.N = f; q.K = d;
-    rc = product(a->dtype, q, st);
+    rc = product(a->dtype, q, ctx);
     if (rc != MB_OK) return rc;
   }
   {
@@ -1094,7 +1349,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     q.dh = dh;
     q.o[0] = dg; q.o[1] = du;
     if (r->ddown) q.o[2] = h;
-    rc = product(a->dtype, q, st);
+    rc = product(a->dtype, q, ctx);
     if (rc != MB_OK) return rc;
   }
   if (r->dx) {
@@ -1106,7 +1361,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     q.b_mn = true;
     q.o[0] = {r->dx, T, d, r->lddx};
     q.M = T; q.N = d; q.K = f;
-    rc = product(a->dtype, q, st);
+    rc = product(a->dtype, q, ctx);
     if (rc != MB_OK) return rc;
   }
   if (r->dgate || r->dup) {
@@ -1123,7 +1378,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     }
     q.b[0] = x;
     q.M = f; q.N = d; q.K = T;
-    rc = product(a->dtype, q, st);
+    rc = product(a->dtype, q, ctx);
     if (rc != MB_OK) return rc;
   }
   if (r->ddown) {
@@ -1133,7 +1388,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     q.b[0] = h;
     q.o[0] = {r->ddown, d, f, r->ld_ddown};
     q.M = d; q.N = f; q.K = T;
-    rc = product(a->dtype, q, st);
+    rc = product(a->dtype, q, ctx);
   }
   return rc;
 }

@@ -130,12 +130,11 @@ def _forward(x, gate, up, down, code):
         out = _out(tokens, width, x)
         L = _lib.lib()
         if down is None:
-            _lib.check(L.mb_gated_linear(ctypes.byref(a), out.data_ptr(), out.shape[1], stream), "gated_linear")
+            name, run, nbytes = "gated_linear", L.mb_gated_linear, L.mb_gated_linear_workspace_bytes(tokens)
         else:
-            nbytes = L.mb_feed_forward_workspace_bytes(tokens, f)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            _lib.check(L.mb_feed_forward(ctypes.byref(a), out.data_ptr(), out.shape[1], ws.data_ptr(), nbytes, stream),
-                       "feed_forward")
+            name, run, nbytes = "feed_forward", L.mb_feed_forward, L.mb_feed_forward_workspace_bytes(tokens, f)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.check(run(ctypes.byref(a), out.data_ptr(), out.shape[1], ws.data_ptr(), nbytes, stream), name)
         del keep
         out = _crop(out, width)
         return out if x.dim() == 2 else out.view(x.shape[:-1] + (width,))
