@@ -32,10 +32,11 @@
 //
 // Its grid is persistent: whole tiles in turn, and where the last round would leave
 // most pairs idle, that round's tiles are cut along the contraction into equal
-// pieces (Sched). Every piece writes its FP32 partial to the workspace and counts
-// itself in; the one that arrives last adds all of them in contraction order
-// (whichever it is, so the sum does not depend on timing) and runs the epilogue.
-// Nobody waits for another pair.
+// pieces (Sched). A piece writes its FP32 partial to the workspace, and k_ffn_join
+// adds a tile's pieces in contraction order and runs the epilogue. (Joining inside
+// the kernel, by the piece that arrives last, needs a fence that does not return
+// while the SM's TMA loads keep coming: 54.9 us against 49 for 256 tokens, d 4096,
+// f 11008.)
 //
 // k_ffn_skinny (T <= kSkinnyTokens): weights are the MMA's M side (128 rows per CTA:
 // 64 gate and 64 up rows in the gated forms), tokens its N side (16 ..), so each
@@ -106,10 +107,6 @@ struct Sched {
   int tiles, kb, units, cut_tiles, ways;
 };
 
-template <int N> struct Int {
-  static constexpr int value = N;
-};
-
 struct PairArgs {
   int M, N;       // output rows and columns (gated: features)
   int kb;         // 64-deep blocks of one K segment
@@ -117,8 +114,7 @@ struct PairArgs {
   int nprob;      // problems of one launch along M (weight gradients: up to 2)
   int mt, nt;     // tiles of one problem
   Sched sched;
-  float* partials;    // workspace of tiles cut between units
-  int32_t* counters;
+  float* partials;    // workspace of the pieces of cut tiles
   int act;
   int want_h;       // backward: store h
   const void* dh;   // backward input: FP32 (kGatedBwdF32) or 16-bit
@@ -143,6 +139,10 @@ __device__ __forceinline__ void load_2d_pair(void* dst, const CUtensorMap* map, 
       "[%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
       : "memory");
+}
+
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 __device__ __forceinline__ void store_2d(const CUtensorMap* map, const void* src, int x, int y) {
@@ -254,11 +254,24 @@ __device__ __forceinline__ uint4* block_chunk(uint8_t* block, int r, int c) {
   return reinterpret_cast<uint4*>(block + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
+// Four consecutive 16-bit values (8-byte aligned when all four exist).
+template <bool kF16>
+__device__ __forceinline__ void store_quad(void* p, int64_t e, int n, const float (&v)[4]) {
+  uint16_t* o = static_cast<uint16_t*>(p) + e;
+  if (n == 4) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<kF16>(v[0], v[1]), pack2<kF16>(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) o[j] = f2h<kF16>(v[j]);
+  }
+}
+
 // ------------------------------------------------------------- scheduling --
 
-// One piece of work: k-blocks [k0, k1) of a tile; `own` of the tile's `ways` pieces.
+// One piece of work: k-blocks [k0, k1) of a tile; `piece` of a cut tile, else -1.
 struct Item {
-  int tile, k0, k1, ways, own;
+  int tile, k0, k1, piece;
 };
 
 struct Items {
@@ -270,45 +283,24 @@ struct Items {
     if (cut) {
       cut = false;
       it.tile = unit / s.ways;
-      it.own = unit - it.tile * s.ways;
-      it.ways = s.ways;
-      it.k0 = (int)((int64_t)s.kb * it.own / s.ways);
-      it.k1 = (int)((int64_t)s.kb * (it.own + 1) / s.ways);
+      it.piece = unit - it.tile * s.ways;
+      it.k0 = (int)((int64_t)s.kb * it.piece / s.ways);
+      it.k1 = (int)((int64_t)s.kb * (it.piece + 1) / s.ways);
       return true;
     }
     it.tile = next_tile;
     it.k0 = 0;
     it.k1 = s.kb;
-    it.ways = 1;
-    it.own = 0;
+    it.piece = -1;
     next_tile += s.units;
     return it.tile < s.tiles;
   }
 };
 
-// After a warp wrote its partial: true for the piece that arrives last, which then
-// sees all others' partials and leaves the counter at zero.
-__device__ __forceinline__ bool arrive_last(int32_t* counter, int ways, int lane) {
-  __threadfence();
-  __syncwarp();
-  int before = 0;
-  if (lane == 0) before = atomicAdd(counter, 1);
-  before = __shfl_sync(0xffffffffu, before, 0);
-  if (before != ways - 1) return false;
-  __threadfence();
-  if (lane == 0) *counter = 0;
-  return true;
-}
-
 // Programmatic dependent launch: let the next kernel of the call set up, and wait
 // for everything the previous ones wrote.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-__global__ void k_zero(int32_t* p, int n) {
-  pdl_trigger();
-  for (int i = threadIdx.x; i < n; i += blockDim.x) p[i] = 0;
-}
 
 // ------------------------------------------------------------ pair kernel --
 
@@ -406,6 +398,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     *abort_flag = 0;
     mbar_fence_init();
   }
+  if (warp == 2 && lane < 7) prefetch_map(lane < 2 ? &maps.a[lane] : lane < 4 ? &maps.b[lane - 2] : &maps.o[lane - 4]);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kTmemCols)
@@ -517,73 +510,32 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
       // this warp's accumulator columns: plain 0..127 from here; gated g at 0..63, u at kFeat..
       const uint32_t acc = tmem + (uint32_t)(a * BN) + ((uint32_t)(q * 32) << 16) +
                            (uint32_t)(half * (is_plain(kEpi) ? kWarpCols : kFeat / 2));
-      // its partial of piece i: float4 j of lane l at j * 32 + l
-      auto partial = [&](int i) {
-        return reinterpret_cast<float4*>(g.partials) +
-               ((int64_t)(item.tile * item.ways + i) * 2 * kEpiWarps + w16) * (kWarpPartial / 4) + lane;
+      // 32 accumulator columns: block b (0..3) of this warp's 128
+      auto fetch = [&](int b, float* v) {
+        uint32_t r[32];
+        tmem_ld32(acc + (uint32_t)(is_plain(kEpi) ? 32 * b : 32 * (b & 1) + kFeat * (b >> 1)), r);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
       };
-      // 32 accumulator columns: block b (0..3) of this warp's 128, joined over the pieces
-      auto tmem_block = [&](int b) {
-        return acc + (uint32_t)(is_plain(kEpi) ? 32 * b : 32 * (b & 1) + kFeat * (b >> 1));
-      };
-      bool finish = in;
-      if (item.ways > 1 && in) {
-        float4* mine = partial(item.own);
+      if (in && item.piece >= 0) {
+        // the piece's partial: float4 j of lane l at j * 32 + l
+        float4* mine = reinterpret_cast<float4*>(g.partials) +
+                       ((int64_t)(item.tile * g.sched.ways + item.piece) * 2 * kEpiWarps + w16) * (kWarpPartial / 4) +
+                       lane;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          uint32_t r[32];
-          tmem_ld32(tmem_block(b), r);
+          float v[32];
+          fetch(b, v);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            mine[(b * 8 + k) * 32] = make_float4(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1]),
-                                                 __uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3]));
+            mine[(b * 8 + k) * 32] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
         }
-        finish = arrive_last(g.counters + item.tile * 2 * kEpiWarps + w16, item.ways, lane);
-      }
-      // kNb blocks at once, so that as many partial loads are in flight
-      auto fetch = [&](auto nb, const int (&b)[decltype(nb)::value], float* v) {
-        constexpr int kNb = decltype(nb)::value;
-        uint32_t r[kNb][32];
-#pragma unroll
-        for (int n = 0; n < kNb; ++n) tmem_ld32(tmem_block(b[n]), r[n]);
-        if (item.ways == 1) {
-#pragma unroll
-          for (int n = 0; n < kNb; ++n)
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[n * 32 + j] = __uint_as_float(r[n][j]);
-          return;
-        }
-#pragma unroll
-        for (int j = 0; j < kNb * 32; ++j) v[j] = 0.0f;
-        for (int i = 0; i < item.ways; ++i) {
-          if (i == item.own) {
-#pragma unroll
-            for (int n = 0; n < kNb; ++n)
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[n * 32 + j] += __uint_as_float(r[n][j]);
-          } else {
-            const float4* src = partial(i);
-            float4 x[kNb][8];
-#pragma unroll
-            for (int n = 0; n < kNb; ++n)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) x[n][k] = __ldcg(src + (b[n] * 8 + k) * 32);
-#pragma unroll
-            for (int n = 0; n < kNb; ++n)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                float* o = v + n * 32 + 4 * k;
-                o[0] += x[n][k].x; o[1] += x[n][k].y; o[2] += x[n][k].z; o[3] += x[n][k].w;
-              }
-          }
-        }
-      };
-      if (finish) {
+      } else if (in) {
         if constexpr (kEpi == kPlainF32) {
           for (int b = 0; b < 4; ++b) {
             if (col0 + 32 * b >= g.N) break;  // warp-uniform
             float v[32];
-            fetch(Int<1>{}, {b}, v);
+            fetch(b, v);
             if (lane == 0) store_wait_read<0>();  // the store before has read this tile
             __syncwarp();
 #pragma unroll
@@ -601,7 +553,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
           for (int b = 0; b < 4; b += 2) {
             if (col0 + 32 * b >= g.N) break;  // warp-uniform
             float v[64];
-            fetch(Int<2>{}, {b, b + 1}, v);
+            fetch(b, v);
+            fetch(b + 1, v + 32);
             if (lane == 0) store_wait_read<0>();
             __syncwarp();
             put_row<kF16>(out, lane, 0, v);
@@ -619,7 +572,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
 #pragma unroll 1
           for (int b = 0; b < 2; ++b) {
             float v[64];
-            fetch(Int<2>{}, {b, b + 2}, v);
+            fetch(b, v);
+            fetch(b + 2, v + 32);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = gated(v[j], v[32 + j], g.act);
             put_row<kF16>(out, lane, 4 * b, v);
@@ -638,8 +592,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
           for (int b = 0; b < 2; ++b) {
             if (col0 + 32 * b >= g.N) break;  // warp-uniform
             float v[64];
-            fetch(Int<1>{}, {b}, v);  // one at a time: dh holds the registers of a second
-            fetch(Int<1>{}, {b + 2}, v + 32);
+            fetch(b, v);
+            fetch(b + 2, v + 32);
             if (lane == 0) store_wait_read<0>();  // the block before has been read out
             __syncwarp();
 #pragma unroll
@@ -690,6 +644,76 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ffn_err, 1);
 }
 
+// Completes the cut tiles of a pair launch: adds each one's pieces in contraction
+// order and runs the product's epilogue. A warp takes 32 rows x 4 columns (features),
+// lane l row l as the pieces were written, so reads are whole 512-byte lines of L2.
+struct JoinArgs {
+  PairArgs p;
+  void* o[3];
+  int64_t ldo[3];
+};
+
+constexpr int kJoinThreads = 128;
+
+template <int kEpi, bool kF16>
+__global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const JoinArgs j) {
+  pdl_trigger();
+  const PairArgs& g = j.p;
+  constexpr int kQuads = is_plain(kEpi) ? 32 : 16;  // 4-column groups of a piece's warp
+  const int lane = threadIdx.x & 31;
+  const int item = (int)(blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5));
+  const int quad = item % kQuads, w16 = item / kQuads % (2 * kEpiWarps), tile = item / kQuads / (2 * kEpiWarps);
+  int prob, bm, bn;
+  tile_of(g, tile, prob, bm, bn);
+  const int half = (w16 & (kEpiWarps - 1)) >> 2;
+  const int64_t row = (int64_t)bm * 2 * BM + w16 / kEpiWarps * BM + (w16 & 3) * 32 + lane;
+  const int col = (is_plain(kEpi) ? bn * BN + half * kWarpCols : bn * kFeat + half * (kFeat / 2)) + 4 * quad;
+  if (row >= g.M || col >= g.N) return;
+  const int n = g.N - col < 4 ? g.N - col : 4;
+  pdl_wait();
+  const float4* src = reinterpret_cast<const float4*>(g.partials) +
+                      ((int64_t)tile * g.sched.ways * 2 * kEpiWarps + w16) * (kWarpPartial / 4) + quad * 32 + lane;
+  constexpr int64_t kPiece = (int64_t)2 * kEpiWarps * kWarpPartial / 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < g.sched.ways; ++i) {
+    const float4 x = __ldcg(src + i * kPiece);
+    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+    if constexpr (!is_plain(kEpi)) {
+      const float4 y = __ldcg(src + i * kPiece + kQuads * 32);
+      w[0] += y.x; w[1] += y.y; w[2] += y.z; w[3] += y.w;
+    }
+  }
+  if constexpr (kEpi == kPlain) {
+    store_quad<kF16>(j.o[prob], row * j.ldo[prob] + col, n, v);
+  } else if constexpr (kEpi == kPlainF32) {
+    float* o = static_cast<float*>(j.o[prob]) + row * j.ldo[prob] + col;
+    if (n == 4) {
+      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      for (int e = 0; e < n; ++e) o[e] = v[e];
+    }
+  } else if constexpr (kEpi == kGated) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = gated(v[e], w[e], g.act);
+    store_quad<kF16>(j.o[0], row * j.ldo[0] + col, n, v);
+  } else {
+    float dg[4], du[4], h[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float dh = 0.0f;
+      if (e < n) {
+        if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[row * g.lddh + col + e];
+        else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[row * g.lddh + col + e]);
+      }
+      gated_bwd(v[e], w[e], dh, g.act, dg[e], du[e], h[e]);
+    }
+    store_quad<kF16>(j.o[0], row * j.ldo[0] + col, n, dg);
+    store_quad<kF16>(j.o[1], row * j.ldo[1] + col, n, du);
+    if (g.want_h) store_quad<kF16>(j.o[2], row * j.ldo[2] + col, n, h);
+  }
+}
+
 // ---------------------------------------------------------- skinny kernel --
 
 constexpr int kSkinnyThreads = 128;
@@ -718,19 +742,6 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
                : "r"(addr)
                : "memory");
   return v;
-}
-
-// Four consecutive 16-bit values (8-byte aligned when all four exist).
-template <bool kF16>
-__device__ __forceinline__ void store_quad(void* p, int64_t e, int n, const float (&v)[4]) {
-  uint16_t* o = static_cast<uint16_t*>(p) + e;
-  if (n == 4) {
-    *reinterpret_cast<uint2*>(o) = make_uint2(pack2<kF16>(v[0], v[1]), pack2<kF16>(v[2], v[3]));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) o[j] = f2h<kF16>(v[j]);
-  }
 }
 
 template <int kEpi, bool kAMn, bool kF16>
@@ -762,6 +773,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     *abort_flag = 0;
     mbar_fence_init();
   }
+  if (warp == 2 && lane < 4) prefetch_map(lane < 2 ? &maps.a[lane] : &maps.b[lane - 2]);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(g.tmem_cols)
@@ -978,10 +990,8 @@ int current_device(int* sms) {
 // What the products of one call share.
 struct Ctx {
   cudaStream_t stream;
-  float* partials;    // pair products: the pieces of cut tiles
-  int32_t* counters;  // ... and their counters
-  bool zeroed;        // the counters have been cleared
-  bool chained;       // the kernel before on the stream belongs to this call
+  float* partials;  // pair products: the pieces of cut tiles
+  bool chained;     // the kernel before on the stream belongs to this call
 };
 
 cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int threads, int smem, int cluster,
@@ -1010,9 +1020,7 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
 constexpr int kMaxPairs = 96;  // pairs a launch may have, for the size of its workspace
 // Tokens up to which the weight-streaming kernel runs.
 constexpr int64_t kSkinnyTokens = 64;
-constexpr int kCounters = kMaxPairs * 2 * kEpiWarps;
-constexpr size_t kJoinBytes = kCounters * sizeof(int32_t) + (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial * 4;
-static_assert(kJoinBytes % 256 == 0, "what follows stays aligned");
+constexpr size_t kJoinBytes = (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial * 4;  // one piece a pair
 
 // The workspace's joining part; a call whose products are all skinny has none.
 size_t join_bytes(int64_t tokens) { return tokens <= kSkinnyTokens ? 0 : kJoinBytes; }
@@ -1068,6 +1076,10 @@ int launch_pair(const Product& q, Ctx& ctx) {
       ok = ok && map_2d(&m.o[i], f32_out ? t32 : t16, q.o[i].p, q.o[i].rows, q.o[i].cols, q.o[i].ld,
                         f32_out || is_bwd(kEpi) ? 32 : 64, 32);
   if (!ok) return MB_ERR_CUDA;
+  for (int i = na; i < 2; ++i) m.a[i] = m.a[0];  // every map the kernel prefetches is one
+  for (int i = nb; i < 2; ++i) m.b[i] = m.b[0];
+  for (int i = 0; i < 3; ++i)
+    if (!q.o[i].p) m.o[i] = m.o[0];
   const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), cols = is_plain(kEpi) ? BN : kFeat;
   const int64_t nt = (q.N + cols - 1) / cols;
   const int64_t work = mt * nt * q.nprob;
@@ -1081,19 +1093,21 @@ int launch_pair(const Product& q, Ctx& ctx) {
   g.dh = q.dh.p; g.lddh = q.dh.ld;
   take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
   g.sched = make_sched((int)work, (int)(kb * q.nseg), entry.pairs[dev]);
-  if (g.sched.ways > 1) {
-    if (!ctx.zeroed) {  // once a call: the last piece of a tile leaves its counters at zero
-      cudaLaunchAttribute zat[2];
-      cudaLaunchConfig_t zero = launch_config(zat, 1, 512, 0, 1, &ctx);
-      if (cudaLaunchKernelEx(&zero, k_zero, ctx.counters, kCounters) != cudaSuccess) return MB_ERR_CUDA;
-      ctx.zeroed = ctx.chained = true;
-    }
-    g.partials = ctx.partials;
-    g.counters = ctx.counters;
-  }
+  g.partials = ctx.partials;
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t cfg = launch_config(at, 2 * g.sched.units, kPairThreads, smem, 2, &ctx);
-  return cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, kernel, m, g) != cudaSuccess) return MB_ERR_CUDA;
+  ctx.chained = true;
+  if (g.sched.cut_tiles == 0) return MB_OK;
+  JoinArgs j{g, {}, {}};
+  for (int i = 0; i < 3; ++i) {
+    j.o[i] = const_cast<void*>(q.o[i].p);
+    j.ldo[i] = q.o[i].ld;
+  }
+  const int warps = g.sched.cut_tiles * 2 * kEpiWarps * (is_plain(kEpi) ? 32 : 16);
+  cudaLaunchAttribute jat[2];
+  cudaLaunchConfig_t join = launch_config(jat, warps / (kJoinThreads / 32), kJoinThreads, 0, 1, &ctx);
+  return cudaLaunchKernelEx(&join, k_ffn_join<kEpi, kF16>, j) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
 }
 
 // Shared memory of a skinny CTA: kSkinnyPerSm of them share an SM's 228 KB.
@@ -1101,7 +1115,7 @@ constexpr int kSkinnyPerSm = 3;
 constexpr int kSkinnySmem = (228 / kSkinnyPerSm - 1) * 1024;
 
 template <int kEpi, bool kAMn, bool kF16>
-int launch_skinny(const Product& q, const Ctx& ctx) {
+int launch_skinny(const Product& q, Ctx& ctx) {
   // q is given as in the pair form (a: tokens, b: weights); the MMA swaps them
   auto kernel = &k_ffn_skinny<kEpi, kAMn, kF16>;
   static KernelEntry entry;
@@ -1143,6 +1157,8 @@ int launch_skinny(const Product& q, const Ctx& ctx) {
   for (int i = 0; i < q.nseg; ++i)
     ok = ok && map_2d(&m.b[i], t16, q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, g.n);
   if (!ok) return MB_ERR_CUDA;
+  for (int i = nw; i < 2; ++i) m.a[i] = m.a[0];  // every map the kernel prefetches is one
+  for (int i = q.nseg; i < 2; ++i) m.b[i] = m.b[0];
   g.o0 = const_cast<void*>(q.o[0].p); g.ldo = q.o[0].ld;
   g.o1 = const_cast<void*>(q.o[1].p); g.ldu = q.o[1].ld;
   g.o2 = const_cast<void*>(q.o[2].p); g.ldh = q.o[2].ld;
@@ -1151,7 +1167,8 @@ int launch_skinny(const Product& q, const Ctx& ctx) {
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t cfg =
       launch_config(at, (int)(tiles * g.split), kSkinnyThreads, kSkinnySmem, g.split, &ctx);
-  return cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
+  ctx.chained = cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess;
+  return ctx.chained ? MB_OK : MB_ERR_CUDA;
 }
 
 template <bool kF16>
@@ -1171,16 +1188,11 @@ int run_product(const Product& q, Ctx& st) {
 }
 
 int product(int dtype, const Product& q, Ctx& ctx) {
-  const int rc = dtype == MB_F16 ? run_product<true>(q, ctx) : run_product<false>(q, ctx);
-  ctx.chained = true;
-  return rc;
+  return dtype == MB_F16 ? run_product<true>(q, ctx) : run_product<false>(q, ctx);
 }
 
 // The call's context over the joining part of its workspace (its first kJoinBytes).
-Ctx make_ctx(void* workspace, cudaStream_t stream) {
-  int32_t* counters = static_cast<int32_t*>(workspace);
-  return {stream, reinterpret_cast<float*>(counters + kCounters), counters, false, false};
-}
+Ctx make_ctx(void* workspace, cudaStream_t stream) { return {stream, static_cast<float*>(workspace), false}; }
 
 constexpr int64_t kMaxDim = (int64_t)1 << 30;
 
