@@ -269,6 +269,10 @@ __device__ __forceinline__ void store_quad(void* p, int64_t e, int n, const floa
 
 // ------------------------------------------------------------- scheduling --
 
+// When a pair launch cuts its last round: pieces of at least kMinPieceKb k-blocks, at
+// most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time.
+constexpr int kMinPieceKb = 4, kMaxWays = 4, kMinSavedKb = 16;
+
 // One piece of work: k-blocks [k0, k1) of a tile; `piece` of a cut tile, else -1.
 struct Item {
   int tile, k0, k1, piece;
@@ -645,8 +649,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
 }
 
 // Completes the cut tiles of a pair launch: adds each one's pieces in contraction
-// order and runs the product's epilogue. A warp takes 32 rows x 4 columns (features),
-// lane l row l as the pieces were written, so reads are whole 512-byte lines of L2.
+// order and runs the product's epilogue. A warp takes 32 rows x 16 columns (features),
+// lane l row l as the pieces were written: it reads whole 512-byte lines, all of a
+// thread's in flight at once, and writes whole sectors.
 struct JoinArgs {
   PairArgs p;
   void* o[3];
@@ -654,69 +659,103 @@ struct JoinArgs {
 };
 
 constexpr int kJoinThreads = 128;
+constexpr int kJoinCols = 16;
+
+// kJoinCols 16-bit values from element e on, the first n of them (rows are 16-byte
+// aligned and kJoinCols divides e's column).
+template <bool kF16>
+__device__ __forceinline__ void store_cols(void* p, int64_t e, int n, const float (&v)[kJoinCols]) {
+  uint16_t* o = static_cast<uint16_t*>(p) + e;
+  if (n == kJoinCols) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      reinterpret_cast<uint4*>(o)[h] =
+          make_uint4(pack2<kF16>(v[8 * h], v[8 * h + 1]), pack2<kF16>(v[8 * h + 2], v[8 * h + 3]),
+                     pack2<kF16>(v[8 * h + 4], v[8 * h + 5]), pack2<kF16>(v[8 * h + 6], v[8 * h + 7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kJoinCols; ++j)
+      if (j < n) o[j] = f2h<kF16>(v[j]);
+  }
+}
 
 template <int kEpi, bool kF16>
 __global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const JoinArgs j) {
   pdl_trigger();
   const PairArgs& g = j.p;
-  constexpr int kQuads = is_plain(kEpi) ? 32 : 16;  // 4-column groups of a piece's warp
+  constexpr int kGroups = (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;  // of a piece's warp
+  constexpr int kParts = is_plain(kEpi) ? 1 : 2;                                 // value, or g and u
   const int lane = threadIdx.x & 31;
   const int item = (int)(blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5));
-  const int quad = item % kQuads, w16 = item / kQuads % (2 * kEpiWarps), tile = item / kQuads / (2 * kEpiWarps);
+  const int group = item % kGroups, w16 = item / kGroups % (2 * kEpiWarps), tile = item / kGroups / (2 * kEpiWarps);
   int prob, bm, bn;
   tile_of(g, tile, prob, bm, bn);
   const int half = (w16 & (kEpiWarps - 1)) >> 2;
   const int64_t row = (int64_t)bm * 2 * BM + w16 / kEpiWarps * BM + (w16 & 3) * 32 + lane;
-  const int col = (is_plain(kEpi) ? bn * BN + half * kWarpCols : bn * kFeat + half * (kFeat / 2)) + 4 * quad;
+  const int col =
+      (is_plain(kEpi) ? bn * BN + half * kWarpCols : bn * kFeat + half * (kFeat / 2)) + kJoinCols * group;
   if (row >= g.M || col >= g.N) return;
-  const int n = g.N - col < 4 ? g.N - col : 4;
+  const int n = g.N - col < kJoinCols ? g.N - col : kJoinCols;
   pdl_wait();
   const float4* src = reinterpret_cast<const float4*>(g.partials) +
-                      ((int64_t)tile * g.sched.ways * 2 * kEpiWarps + w16) * (kWarpPartial / 4) + quad * 32 + lane;
+                      ((int64_t)tile * g.sched.ways * 2 * kEpiWarps + w16) * (kWarpPartial / 4) +
+                      group * (kJoinCols / 4) * 32 + lane;
   constexpr int64_t kPiece = (int64_t)2 * kEpiWarps * kWarpPartial / 4;
-  float v[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = 0; i < g.sched.ways; ++i) {
-    const float4 x = __ldcg(src + i * kPiece);
-    v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-    if constexpr (!is_plain(kEpi)) {
-      const float4 y = __ldcg(src + i * kPiece + kQuads * 32);
-      w[0] += y.x; w[1] += y.y; w[2] += y.z; w[3] += y.w;
-    }
+  float v[kParts][kJoinCols];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p)
+#pragma unroll
+    for (int c = 0; c < kJoinCols; ++c) v[p][c] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMaxWays; ++i) {
+    if (i >= g.sched.ways) break;
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+      for (int c = 0; c < kJoinCols / 4; ++c) {
+        const float4 x = __ldcg(src + i * kPiece + (p * (kFeat / 2) / 4 + c) * 32);
+        v[p][4 * c] += x.x; v[p][4 * c + 1] += x.y; v[p][4 * c + 2] += x.z; v[p][4 * c + 3] += x.w;
+      }
   }
   if constexpr (kEpi == kPlain) {
-    store_quad<kF16>(j.o[prob], row * j.ldo[prob] + col, n, v);
+    store_cols<kF16>(j.o[prob], row * j.ldo[prob] + col, n, v[0]);
   } else if constexpr (kEpi == kPlainF32) {
     float* o = static_cast<float*>(j.o[prob]) + row * j.ldo[prob] + col;
-    if (n == 4) {
-      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      for (int e = 0; e < n; ++e) o[e] = v[e];
+#pragma unroll
+    for (int c = 0; c < kJoinCols; c += 4) {
+      if (c + 4 <= n) {
+        *reinterpret_cast<float4*>(o + c) = make_float4(v[0][c], v[0][c + 1], v[0][c + 2], v[0][c + 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < n) o[c + e] = v[0][c + e];
+      }
     }
   } else if constexpr (kEpi == kGated) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = gated(v[e], w[e], g.act);
-    store_quad<kF16>(j.o[0], row * j.ldo[0] + col, n, v);
+    for (int c = 0; c < kJoinCols; ++c) v[0][c] = gated(v[0][c], v[1][c], g.act);
+    store_cols<kF16>(j.o[0], row * j.ldo[0] + col, n, v[0]);
   } else {
-    float dg[4], du[4], h[4];
+    float dg[kJoinCols], du[kJoinCols], h[kJoinCols];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int c = 0; c < kJoinCols; ++c) {
       float dh = 0.0f;
-      if (e < n) {
-        if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[row * g.lddh + col + e];
-        else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[row * g.lddh + col + e]);
+      if (c < n) {
+        if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[row * g.lddh + col + c];
+        else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[row * g.lddh + col + c]);
       }
-      gated_bwd(v[e], w[e], dh, g.act, dg[e], du[e], h[e]);
+      gated_bwd(v[0][c], v[1][c], dh, g.act, dg[c], du[c], h[c]);
     }
-    store_quad<kF16>(j.o[0], row * j.ldo[0] + col, n, dg);
-    store_quad<kF16>(j.o[1], row * j.ldo[1] + col, n, du);
-    if (g.want_h) store_quad<kF16>(j.o[2], row * j.ldo[2] + col, n, h);
+    store_cols<kF16>(j.o[0], row * j.ldo[0] + col, n, dg);
+    store_cols<kF16>(j.o[1], row * j.ldo[1] + col, n, du);
+    if (g.want_h) store_cols<kF16>(j.o[2], row * j.ldo[2] + col, n, h);
   }
 }
 
 // ---------------------------------------------------------- skinny kernel --
 
 constexpr int kSkinnyThreads = 128;
+constexpr int kSkinnyPitch = 132;  // floats between tokens' 128 partials in shared memory
 
 struct SkinnyArgs {
   int tokens;     // M of the product
@@ -853,15 +892,13 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   }
   __syncthreads();  // the producer's and the MMA thread's waits have ended too
   tc_fence_after();
-  // [token][128 features], rows 16 bytes apart from a multiple of 128 B
-  constexpr int kPitch = 132;
   float* part = reinterpret_cast<float*>(smem);
   for (int c = 0; c < g.tokens; c += 16) {
     uint32_t r[16];
     tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, r);
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (c + j < g.tokens) part[(c + j) * kPitch + warp * 32 + lane] = __uint_as_float(r[j]);
+      if (c + j < g.tokens) part[(c + j) * kSkinnyPitch + warp * 32 + lane] = __uint_as_float(r[j]);
   }
   tc_fence_before();
   if (g.split > 1) cluster_sync();
@@ -883,7 +920,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
       const int n = g.rows - (feat0 + f4) < 4 ? g.rows - (feat0 + f4) : 4;
       if (n <= 0) continue;
       float v[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
-      const uint32_t at = base + (uint32_t)(j * kPitch + f4) * 4u;
+      const uint32_t at = base + (uint32_t)(j * kSkinnyPitch + f4) * 4u;
 #pragma unroll 4
       for (int r = 0; r < g.split; ++r) {
         const uint32_t p = g.split > 1 ? mapa_u32(at, (uint32_t)r) : at;
@@ -963,10 +1000,6 @@ struct Product {
 };
 
 constexpr int kMaxDevices = 64;
-constexpr int kSkinnyWaves = 1;
-// When a pair launch cuts its last round: pieces of at least kMinPieceKb k-blocks, at
-// most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time.
-constexpr int kMinPieceKb = 4, kMaxWays = 8, kMinSavedKb = 16;
 
 struct KernelEntry {
   std::once_flag once[kMaxDevices];
@@ -1019,7 +1052,7 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
 
 constexpr int kMaxPairs = 96;  // pairs a launch may have, for the size of its workspace
 // Tokens up to which the weight-streaming kernel runs.
-constexpr int64_t kSkinnyTokens = 64;
+constexpr int64_t kSkinnyTokens = 128;
 constexpr size_t kJoinBytes = (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial * 4;  // one piece a pair
 
 // The workspace's joining part; a call whose products are all skinny has none.
@@ -1104,15 +1137,14 @@ int launch_pair(const Product& q, Ctx& ctx) {
     j.o[i] = const_cast<void*>(q.o[i].p);
     j.ldo[i] = q.o[i].ld;
   }
-  const int warps = g.sched.cut_tiles * 2 * kEpiWarps * (is_plain(kEpi) ? 32 : 16);
+  const int warps = g.sched.cut_tiles * 2 * kEpiWarps * (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;
   cudaLaunchAttribute jat[2];
   cudaLaunchConfig_t join = launch_config(jat, warps / (kJoinThreads / 32), kJoinThreads, 0, 1, &ctx);
   return cudaLaunchKernelEx(&join, k_ffn_join<kEpi, kF16>, j) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
 }
 
-// Shared memory of a skinny CTA: kSkinnyPerSm of them share an SM's 228 KB.
-constexpr int kSkinnyPerSm = 3;
-constexpr int kSkinnySmem = (228 / kSkinnyPerSm - 1) * 1024;
+constexpr int kSkinnyPerSm = 3, kSkinnyStages = 3;
+constexpr int kSkinnyMaxSmem = 227 * 1024;
 
 template <int kEpi, bool kAMn, bool kF16>
 int launch_skinny(const Product& q, Ctx& ctx) {
@@ -1123,7 +1155,7 @@ int launch_skinny(const Product& q, Ctx& ctx) {
   const int dev = current_device(&sms);
   if (dev < 0) return MB_ERR_CUDA;
   std::call_once(entry.once[dev], [&] {
-    entry.rc[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnySmem) ==
+    entry.rc[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSkinnyMaxSmem) ==
                             cudaSuccess
                         ? MB_OK
                         : MB_ERR_CUDA;
@@ -1137,15 +1169,23 @@ int launch_skinny(const Product& q, Ctx& ctx) {
   const int64_t kb = (q.K + BK - 1) / BK, tiles = (q.N + kPer - 1) / kPer, KB = kb * q.nseg;
   if (KB > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
   g.kb = (int)kb; g.nseg = q.nseg;
-  // Split the contraction until the launch has about kSkinnyWaves CTAs for every place
-  // on the GPU (enough that the last of them to start does not decide its time), as
-  // long as a CTA keeps four k-blocks.
-  g.split = 1;
-  while (g.split < 8 && tiles * g.split < kSkinnyWaves * kSkinnyPerSm * sms && KB / (2 * g.split) >= 4) g.split *= 2;
-  const int stage = kTileA + g.n * BK * 2;
-  g.st = (kSkinnySmem - 1024 - kBarBytes) / stage;  // the partials fit the same ring
+  const int stage = kTileA + g.n * BK * 2, partials = (int)q.M * kSkinnyPitch * 4;  // the ring's memory holds both
   g.tmem_cols = 32;
   while ((int)g.tmem_cols < g.n) g.tmem_cols *= 2;
+  // As many CTAs on an SM as leave each kSkinnyStages stages. All that the memory lets
+  // in must find TMEM columns too: CTAs of two clusters that waited for each other's
+  // columns would never end.
+  int per_sm = kSkinnyPerSm + 1, smem;
+  do {
+    --per_sm;
+    smem = (228 / per_sm - 1) * 1024;
+    g.st = (smem - 1024 - kBarBytes) / stage;
+  } while (per_sm > 1 && (g.st < kSkinnyStages || g.st * stage < partials || per_sm * g.tmem_cols > 512));
+  if (g.st < 1 || g.st * stage < partials || smem > kSkinnyMaxSmem) return MB_ERR_TOO_LARGE;
+  // Split the contraction as far as all CTAs find room at once and keep four k-blocks
+  // each.
+  g.split = 1;
+  while (g.split < 8 && tiles * 2 * g.split <= (int64_t)per_sm * sms && KB / (2 * g.split) >= 4) g.split *= 2;
   g.act = q.act;
   Maps m;
   bool ok = true;
@@ -1166,7 +1206,7 @@ int launch_skinny(const Product& q, Ctx& ctx) {
   take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t cfg =
-      launch_config(at, (int)(tiles * g.split), kSkinnyThreads, kSkinnySmem, g.split, &ctx);
+      launch_config(at, (int)(tiles * g.split), kSkinnyThreads, smem, g.split, &ctx);
   ctx.chained = cudaLaunchKernelEx(&cfg, kernel, m, g) == cudaSuccess;
   return ctx.chained ? MB_OK : MB_ERR_CUDA;
 }
