@@ -209,16 +209,16 @@ class on_device:
         self.index = device.index
 
     def __enter__(self):
-        import torch
-        self.before = torch._C._cuda_getDevice()
+        from torch import _C
+        self.before = _C._cuda_getDevice()
         if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
+            _C._cuda_setDevice(self.index)
+        return _C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
-        import torch
         if self.before != self.index:
-            torch.cuda.set_device(self.before)
+            from torch import _C
+            _C._cuda_setDevice(self.before)
         return False
 
 

@@ -58,11 +58,12 @@ def _check_weights(gate, up, down, d):
         raise ValueError("gate must be [f, d] on a CUDA device")
     if gate.dtype not in DTYPES:
         raise ValueError(f"the block computes in bfloat16 or float16, not {gate.dtype}")
-    f = gate.shape[0]
+    f, width = gate.shape
     if f == 0 or d == 0:
         raise ValueError("d and f must be at least 1")
-    _check(gate, "gate", (f, d), gate)
-    _check(up, "up", (f, d), gate)
+    if width != d:
+        raise ValueError(f"gate must be a tensor of shape {[f, d]}")
+    _check(up, "up", gate.shape, gate)
     if down is not None:
         _check(down, "down", (d, f), gate)
     return f
@@ -86,7 +87,16 @@ def _rows(t, rows, cols):
 
 def _out(rows, cols, like):
     """A buffer for a [rows, cols] output, its rows padded to 16 bytes."""
-    return torch.empty((rows, _pad8(cols)), dtype=like.dtype, device=like.device)
+    return like.new_empty((rows, _pad8(cols)))
+
+
+def _workspace(nbytes, like):
+    """(tensor, address): a buffer from the caching allocator, which a captured
+    graph keeps for itself; none for an empty one."""
+    if nbytes == 0:
+        return None, None
+    ws = like.new_empty(nbytes, dtype=torch.uint8)
+    return ws, ws.data_ptr()
 
 
 def _crop(buf, cols):
@@ -133,9 +143,9 @@ def _forward(x, gate, up, down, code):
             name, run, nbytes = "gated_linear", L.mb_gated_linear, L.mb_gated_linear_workspace_bytes(tokens)
         else:
             name, run, nbytes = "feed_forward", L.mb_feed_forward, L.mb_feed_forward_workspace_bytes(tokens, f)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        _lib.check(run(ctypes.byref(a), out.data_ptr(), out.shape[1], ws.data_ptr(), nbytes, stream), name)
-        del keep
+        ws, address = _workspace(nbytes, x)
+        _lib.check(run(ctypes.byref(a), out.data_ptr(), _pad8(width), address, nbytes, stream), name)
+        del keep, ws
         out = _crop(out, width)
         return out if x.dim() == 2 else out.view(x.shape[:-1] + (width,))
 
@@ -167,13 +177,13 @@ def _backward(grad, saved, gate, up, down, code, needs):
             if need:
                 grads[i] = buf = _out(rows, cols, gate)
                 setattr(r, GRADS[i], buf.data_ptr())
-                setattr(r, PITCHES[i], buf.shape[1])
+                setattr(r, PITCHES[i], _pad8(cols))
         L = _lib.lib()
         nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, codes is not None, down is not None)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=gate.device)
-        _lib.check(L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), ws.data_ptr(), nbytes, stream),
+        ws, address = _workspace(nbytes, gate)
+        _lib.check(L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), address, nbytes, stream),
                    "feed_forward_backward")
-        del keep
+        del keep, ws
         grads = [None if buf is None else _crop(buf, cols) for buf, cols in zip(grads, (d, d, d, f))]
         if grads[0] is not None and like.dim() != 2:
             grads[0] = grads[0].view(like.shape)
@@ -204,7 +214,10 @@ def _block(x, gate, up, down, activation, checkpoint):
     code = _activation_code(activation)
     if checkpoint not in CHECKPOINTS:
         raise ValueError(f"checkpoint must be one of {list(CHECKPOINTS)}, not {checkpoint!r}")
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, gate, up, down)):
+    leaves = (x, gate, up) if down is None else (x, gate, up, down)
+    if not all([isinstance(t, torch.Tensor) for t in leaves]):
+        raise ValueError("x and the weights must be tensors")
+    if torch.is_grad_enabled() and any([t.requires_grad for t in leaves]):
         return _Block.apply(x, gate, up, down, code, checkpoint)
     return _forward(x, gate, up, down, code)
 

@@ -152,6 +152,7 @@ def unpack_fp8(encoded: torch.Tensor, scales: torch.Tensor, dtype=torch.float16,
 
 
 ACTIVATION_BLOCK = 128  # features per scale of an activation checkpoint
+_DTYPE_CODES = {torch.float32: _lib.MB_F32, torch.float16: _lib.MB_F16, torch.bfloat16: _lib.MB_BF16}
 
 
 def pack_activation(x: torch.Tensor):
@@ -167,23 +168,25 @@ def pack_activation(x: torch.Tensor):
     largest is at most 2^-4; smaller ones round at a fixed step of their block."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("pack_activation expects a CUDA tensor")
-    if x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    code = _DTYPE_CODES.get(x.dtype)
+    if code is None:
         raise ValueError(f"unsupported dtype {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
         raise ValueError("pack_activation expects [..., d] with d >= 1")
-    d = x.shape[-1]
-    flat = x if x.dim() == 2 else x.detach().reshape(-1, d)
+    d = shape[-1]
+    flat = x if len(shape) == 2 else x.detach().reshape(-1, d)
     rows = flat.shape[0]
     ld, inner = flat.stride()
     if inner != 1 and d > 1 or rows > 1 and ld < d:
         flat, ld = flat.detach().contiguous(), d
     elif rows <= 1:
         ld = d
-    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(x.shape[:-1] + (-(-d // ACTIVATION_BLOCK),), dtype=torch.uint8, device=x.device)
+    codes = x.new_empty(shape, dtype=torch.uint8)
+    scales = x.new_empty(shape[:-1] + (-(-d // ACTIVATION_BLOCK),), dtype=torch.uint8)
     with _lib.on_device(x.device) as stream:
-        _lib.check(_lib.lib().mb_act_pack(flat.data_ptr(), _lib.dtype_code(x.dtype), rows, d, ld, codes.data_ptr(),
-                                          scales.data_ptr(), stream), "pack_activation")
+        _lib.check(_lib.lib().mb_act_pack(flat.data_ptr(), code, rows, d, ld, codes.data_ptr(), scales.data_ptr(),
+                                          stream), "pack_activation")
     return codes, scales
 
 
@@ -207,13 +210,14 @@ def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfl
     beyond it (float16, or next to the top of the others) restores as the largest
     finite one."""
     check_activation(codes, scales)
-    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+    code = _DTYPE_CODES.get(dtype)
+    if code is None:
         raise ValueError(f"unsupported dtype {dtype}")
     d = codes.shape[-1]
-    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    out = codes.new_empty(codes.shape, dtype=dtype)
     with _lib.on_device(codes.device) as stream:
         _lib.check(_lib.lib().mb_act_unpack(codes.data_ptr(), scales.data_ptr(), codes.numel() // d, d,
-                                            out.data_ptr(), _lib.dtype_code(dtype), d, stream), "unpack_activation")
+                                            out.data_ptr(), code, d, stream), "unpack_activation")
     return out
 
 
