@@ -156,7 +156,6 @@ __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.com
 template <int kLeft> __device__ __forceinline__ void store_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
 }
-__device__ __forceinline__ void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Instruction descriptor (kind::f16): FP32 accumulator, A and B of one 16-bit type
@@ -636,7 +635,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[a]), 0));
     }
-    if (lane == 0) store_wait_all();
+    if (lane == 0) store_wait_read<0>();  // the stores have read their tiles; the kernel's end completes them
     __syncwarp();
   }
   tc_fence_before();

@@ -58,12 +58,13 @@ def _check_weights(gate, up, down, d):
         raise ValueError("gate must be [f, d] on a CUDA device")
     if gate.dtype not in DTYPES:
         raise ValueError(f"the block computes in bfloat16 or float16, not {gate.dtype}")
-    f, width = gate.shape
+    shape = gate.shape
+    f, width = shape
     if f == 0 or d == 0:
         raise ValueError("d and f must be at least 1")
     if width != d:
         raise ValueError(f"gate must be a tensor of shape {[f, d]}")
-    _check(up, "up", gate.shape, gate)
+    _check(up, "up", shape, gate)
     if down is not None:
         _check(down, "down", (d, f), gate)
     return f
@@ -74,15 +75,22 @@ def _pad8(n: int) -> int:
 
 
 def _rows(t, rows, cols):
-    """(tensor, pitch) of a [rows, cols] tensor with 16-byte aligned rows: itself, or a padded copy."""
-    ld, inner = t.stride()
-    if rows <= 1:
-        ld = _pad8(cols)
-    if (inner == 1 or cols == 1) and ld % 8 == 0 and ld >= cols and t.data_ptr() % 16 == 0:
-        return t, ld
-    buf = torch.empty((rows, _pad8(cols)), dtype=t.dtype, device=t.device)
+    """(tensor, address, pitch) of a [rows, cols] tensor with 16-byte aligned rows:
+    itself, or a padded copy."""
+    address = t.data_ptr()
+    if address % 16 == 0:
+        if t.is_contiguous():
+            if cols % 8 == 0:
+                return t, address, cols
+            if rows <= 1:
+                return t, address, _pad8(cols)
+        else:
+            ld, inner = t.stride()
+            if (inner == 1 or cols == 1) and ld % 8 == 0 and ld >= cols:
+                return t, address, ld
+    buf = t.new_empty((rows, _pad8(cols)))
     buf[:, :cols].copy_(t.detach())
-    return buf, buf.shape[1]
+    return buf, buf.data_ptr(), buf.shape[1]
 
 
 def _out(rows, cols, like):
@@ -100,7 +108,7 @@ def _workspace(nbytes, like):
 
 
 def _crop(buf, cols):
-    return buf if buf.shape[1] == cols else buf[:, :cols].contiguous()
+    return buf if cols % 8 == 0 else buf[:, :cols].contiguous()
 
 
 def _two_d(t):
@@ -109,16 +117,16 @@ def _two_d(t):
 
 def _args(code, tokens, d, f, x, gate, up, down):
     """The C arguments, and the tensors they point into."""
-    gate, ld_gate = _rows(gate, f, d)
-    up, ld_up = _rows(up, f, d)
-    a = _lib.FfnArgs(DTYPES[gate.dtype], code, tokens, d, f, None, 0, gate.data_ptr(), ld_gate, up.data_ptr(), ld_up)
+    dtype = DTYPES[gate.dtype]
+    gate, at_gate, ld_gate = _rows(gate, f, d)
+    up, at_up, ld_up = _rows(up, f, d)
+    at_x, ldx, at_down, ld_down = None, 0, None, 0
     if x is not None:
-        x, a.ldx = _rows(x, tokens, d)
-        a.x = x.data_ptr()
+        x, at_x, ldx = _rows(x, tokens, d)
     if down is not None:
-        down, a.ld_down = _rows(down, d, f)
-        a.down = down.data_ptr()
-    return a, (x, gate, up, down)
+        down, at_down, ld_down = _rows(down, d, f)
+    return (_lib.FfnArgs(dtype, code, tokens, d, f, at_x, ldx, at_gate, ld_gate, at_up, ld_up, at_down, ld_down),
+            (x, gate, up, down))
 
 
 def _input(x, gate):
@@ -144,7 +152,9 @@ def _forward(x, gate, up, down, code):
         else:
             name, run, nbytes = "feed_forward", L.mb_feed_forward, L.mb_feed_forward_workspace_bytes(tokens, f)
         ws, address = _workspace(nbytes, x)
-        _lib.check(run(ctypes.byref(a), out.data_ptr(), _pad8(width), address, nbytes, stream), name)
+        rc = run(ctypes.byref(a), out.data_ptr(), _pad8(width), address, nbytes, stream)
+        if rc:
+            _lib.check(rc, name)
         del keep, ws
         out = _crop(out, width)
         return out if x.dim() == 2 else out.view(x.shape[:-1] + (width,))
@@ -170,8 +180,7 @@ def _backward(grad, saved, gate, up, down, code, needs):
         r = _lib.FfnGrads()
         if codes is not None:
             r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
-        g2, r.lddy = _rows(g2, tokens, f if down is None else d)
-        r.dy = g2.data_ptr()
+        g2, r.dy, r.lddy = _rows(g2, tokens, f if down is None else d)
         grads = [None] * len(needs)
         for i, (need, rows, cols) in enumerate(zip(needs, (tokens, f, f, d), (d, d, d, f))):
             if need:
@@ -181,8 +190,9 @@ def _backward(grad, saved, gate, up, down, code, needs):
         L = _lib.lib()
         nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, codes is not None, down is not None)
         ws, address = _workspace(nbytes, gate)
-        _lib.check(L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), address, nbytes, stream),
-                   "feed_forward_backward")
+        rc = L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), address, nbytes, stream)
+        if rc:
+            _lib.check(rc, "feed_forward_backward")
         del keep, ws
         grads = [None if buf is None else _crop(buf, cols) for buf, cols in zip(grads, (d, d, d, f))]
         if grads[0] is not None and like.dim() != 2:
