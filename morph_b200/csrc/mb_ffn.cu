@@ -95,24 +95,34 @@ constexpr int pair_smem(int epi) {
 static_assert(pair_smem(kPlain) <= 232448 && pair_smem(kGatedBwd) <= 232448, "shared memory of one SM");
 static_assert(warp_bytes(kGatedBwd) % 512 == 0, "swizzled blocks stay aligned");
 
-struct Maps {
-  CUtensorMap a[2], b[2];  // K segments, problems, or (b) gate and up
-  CUtensorMap o[3];        // outputs (backward: dg, du, h)
+// One problem of a pair launch: an output [M, N] (gated: N features) and up to two K
+// segments accumulated into it. Operands and output name the launch's maps.
+struct Problem {
+  int M, N;
+  int kb, nseg;      // 64-deep blocks of one segment; segments
+  int a_mn;          // A is stored [K, M] (the form that takes either)
+  int a[2], b[2];    // by segment; gated: b by CTA of the pair (gate, up)
+  int o;             // backward: dg, du, h at o, o + 1, o + 2
+  int mt, nt, tile0; // row and column tiles; its first tile's number
 };
 
-// Work of one launch: `tiles` output tiles of `kb` k-blocks each over `units` CTA
-// pairs. Each of the first cut_tiles tiles is cut into `ways` pieces, one for each of
-// the first cut_tiles * ways units; the rest go whole, in turn.
+constexpr int kMaxProblems = 4, kMaxMaps = 11;
+
+struct PairMaps {
+  CUtensorMap m[kMaxMaps];
+};
+
+// How a launch's tiles are dealt to its units (CTA pairs). The first long_tiles tiles
+// (all of problem 0) go first, whole (ways 1) or each cut into `ways` pieces: n_long
+// items in turn. Of the n_rest tiles after them, the first `early` go to the units from
+// `late_units` on, which had one long item less, and the others to all in turn.
 struct Sched {
-  int tiles, kb, units, cut_tiles, ways;
+  int units, long_tiles, ways, n_long, n_rest, early, late_units;
 };
 
 struct PairArgs {
-  int M, N;       // output rows and columns (gated: features)
-  int kb;         // 64-deep blocks of one K segment
-  int nseg;       // K segments accumulated into one output (dx: 2)
-  int nprob;      // problems of one launch along M (weight gradients: up to 2)
-  int mt, nt;     // tiles of one problem
+  Problem p[kMaxProblems];
+  int nprob, nmaps;
   Sched sched;
   float* partials;    // workspace of the pieces of cut tiles
   int act;
@@ -270,33 +280,61 @@ __device__ __forceinline__ void store_quad(void* p, int64_t e, int n, const floa
 
 // When a pair launch cuts its last round: pieces of at least kMinPieceKb k-blocks, at
 // most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time.
-constexpr int kMinPieceKb = 4, kMaxWays = 4, kMinSavedKb = 16;
+constexpr int kMinPieceKb = 4, kMaxWays = 4, kMinSavedKb = 24;
 
-// One piece of work: k-blocks [k0, k1) of a tile; `piece` of a cut tile, else -1.
+// One piece of work: k-blocks [k0, k1) of row tile bm, column tile bn of a problem;
+// `piece` of a cut tile, else -1.
 struct Item {
-  int tile, k0, k1, piece;
+  int tile, prob, bm, bn, k0, k1, piece;
 };
 
+// Tile -> problem and place: groups of kGroupM row tiles, row tiles fastest inside a group.
+__device__ __forceinline__ void place_tile(const PairArgs& g, Item& it) {
+  it.prob = 0;
+  for (int i = 1; i < kMaxProblems; ++i)
+    if (i < g.nprob && it.tile >= g.p[i].tile0) it.prob = i;
+  const Problem& p = g.p[it.prob];
+  const int t = it.tile - p.tile0;
+  const int first = t / (kGroupM * p.nt) * kGroupM;
+  const int rows = p.mt - first < kGroupM ? p.mt - first : kGroupM;
+  const int in = t - first * p.nt;
+  it.bm = first + in % rows;
+  it.bn = in / rows;
+  it.k0 = 0;
+  it.k1 = p.kb * p.nseg;
+  it.piece = -1;
+}
+
 struct Items {
-  int unit, next_tile;
-  bool cut;
+  int unit, next_long, next_early, next_rest;
   __device__ __forceinline__ Items(const Sched& s, int u)
-      : unit(u), next_tile(s.cut_tiles + u), cut(u < s.cut_tiles * s.ways) {}
-  __device__ __forceinline__ bool next(const Sched& s, Item& it) {
-    if (cut) {
-      cut = false;
-      it.tile = unit / s.ways;
-      it.piece = unit - it.tile * s.ways;
-      it.k0 = (int)((int64_t)s.kb * it.piece / s.ways);
-      it.k1 = (int)((int64_t)s.kb * (it.piece + 1) / s.ways);
+      : unit(u), next_long(u), next_early(u >= s.late_units ? u - s.late_units : s.early), next_rest(s.early + u) {}
+  __device__ __forceinline__ bool next(const PairArgs& g, Item& it) {
+    const Sched& s = g.sched;
+    if (next_long < s.n_long) {
+      it.tile = next_long / s.ways;
+      place_tile(g, it);
+      if (s.ways > 1) {
+        const int kb = it.k1;
+        it.piece = next_long - it.tile * s.ways;
+        it.k0 = (int)((int64_t)kb * it.piece / s.ways);
+        it.k1 = (int)((int64_t)kb * (it.piece + 1) / s.ways);
+      }
+      next_long += s.units;
       return true;
     }
-    it.tile = next_tile;
-    it.k0 = 0;
-    it.k1 = s.kb;
-    it.piece = -1;
-    next_tile += s.units;
-    return it.tile < s.tiles;
+    int j;
+    if (next_early < s.early) {
+      j = next_early;
+      next_early += s.units - s.late_units;
+    } else {
+      j = next_rest;
+      if (j >= s.n_rest) return false;
+      next_rest += s.units;
+    }
+    it.tile = s.long_tiles + j;
+    place_tile(g, it);
+    return true;
   }
 };
 
@@ -312,30 +350,17 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 constexpr int kWarpCols = BN / 2;
 constexpr int kWarpPartial = 32 * kWarpCols;  // floats
 
-// Tile t -> (problem, row tile, column tile): groups of kGroupM row tiles, row
-// tiles fastest inside a group.
-__device__ __forceinline__ void tile_of(const PairArgs& g, int t, int& prob, int& bm, int& bn) {
-  const int per = g.mt * g.nt;
-  prob = t / per;
-  t -= prob * per;
-  const int grp = t / (kGroupM * g.nt);
-  const int first = grp * kGroupM;
-  const int rows = g.mt - first < kGroupM ? g.mt - first : kGroupM;
-  const int in = t - first * g.nt;
-  bm = first + in % rows;
-  bn = in / rows;
-}
-
 // 32 dh values of one row from feature `col` on (zero past the last feature; rows
 // are 32-byte aligned in the FP32 form, 16-byte in the caller's 16-bit one).
 template <int kEpi, bool kF16>
 __device__ __forceinline__ void load_dh(const PairArgs& g, int64_t row, int col, float (&v)[32]) {
-  const bool in = row < g.M;
+  const int M = g.p[0].M, N = g.p[0].N;
+  const bool in = row < M;
   if constexpr (kEpi == kGatedBwdF32) {
     const float* p = static_cast<const float*>(g.dh) + row * g.lddh + col;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (in && col + 8 * k < g.N) {  // the row's pitch covers the whole group of 8
+      if (in && col + 8 * k < N) {  // the row's pitch covers the whole group of 8
         asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=f"(v[8 * k]), "=f"(v[8 * k + 1]), "=f"(v[8 * k + 2]), "=f"(v[8 * k + 3]), "=f"(v[8 * k + 4]),
                        "=f"(v[8 * k + 5]), "=f"(v[8 * k + 6]), "=f"(v[8 * k + 7])
@@ -350,7 +375,7 @@ __device__ __forceinline__ void load_dh(const PairArgs& g, int64_t row, int col,
     const uint16_t* p = static_cast<const uint16_t*>(g.dh) + row * g.lddh + col;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (in && col + 8 * k + 8 <= g.N) {
+      if (in && col + 8 * k + 8 <= N) {
         const uint4 w = *reinterpret_cast<const uint4*>(p + 8 * k);
         const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -360,14 +385,16 @@ __device__ __forceinline__ void load_dh(const PairArgs& g, int64_t row, int col,
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[8 * k + e] = in && col + 8 * k + e < g.N ? h2f<kF16>(p[8 * k + e]) : 0.0f;
+        for (int e = 0; e < 8; ++e) v[8 * k + e] = in && col + 8 * k + e < N ? h2f<kF16>(p[8 * k + e]) : 0.0f;
       }
     }
   }
 }
 
-template <int kEpi, bool kAMn, bool kBMn, bool kF16>
-__global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_constant__ Maps maps, const PairArgs g) {
+// kAnyA: A's layout is each problem's; else K-major. kBMn: B stored [K, N].
+template <int kEpi, bool kAnyA, bool kBMn, bool kF16>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    k_ffn_pair(const __grid_constant__ PairMaps maps, const __grid_constant__ PairArgs g) {
   constexpr int ST = stages(kEpi);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -401,7 +428,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 2 && lane < 7) prefetch_map(lane < 2 ? &maps.a[lane] : lane < 4 ? &maps.b[lane - 2] : &maps.o[lane - 4]);
+  if (warp == 2 && lane < g.nmaps) prefetch_map(&maps.m[lane]);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(kTmemCols)
@@ -418,27 +445,26 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     if (lane == 0) {
       pdl_wait();
       int kit = 0;
-      for (Items work(g.sched, unit); !*abort_flag && work.next(g.sched, item);) {
-        int prob, bm, bn;
-        tile_of(g, item.tile, prob, bm, bn);
-        const int arow = bm * 2 * BM + (int)rank * BM;
+      for (Items work(g.sched, unit); !*abort_flag && work.next(g, item);) {
+        const Problem& p = g.p[item.prob];
+        const int arow = item.bm * 2 * BM + (int)rank * BM;
         // gated tiles: 128 features from gate (even CTA) or up (odd CTA)
-        const int brow = is_plain(kEpi) ? bn * BN + (int)rank * (BN / 2) : bn * kFeat;
+        const int brow = is_plain(kEpi) ? item.bn * BN + (int)rank * (BN / 2) : item.bn * kFeat;
         for (int kb = item.k0; kb < item.k1; ++kb, ++kit) {
           const int s = kit % ST;
           if (!mbar_wait(&empty[s], ((kit / ST) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
           if (item.tile == g.fault.unit && kb == 0) continue;  // test-only: withhold; the MMA warp's wait expires
-          const int seg = kb >= g.kb ? 1 : 0;
-          const int k0 = (kb - seg * g.kb) * BK;
-          const CUtensorMap* ma = &maps.a[seg + prob];
-          const CUtensorMap* mb_ = &maps.b[is_plain(kEpi) ? seg : (int)rank];
+          const int seg = kb >= p.kb ? 1 : 0;
+          const int k0 = (kb - seg * p.kb) * BK;
+          const CUtensorMap* ma = &maps.m[p.a[seg]];
+          const CUtensorMap* mb_ = &maps.m[p.b[is_plain(kEpi) ? seg : (int)rank]];
           const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
           if (leader) mbar_expect_tx(&full[s], 2 * (kTileA + kTileB));
           uint8_t* a = sA + s * kTileA;
           uint8_t* b = sB + s * kTileB;
-          if constexpr (kAMn) {
-            load_2d_pair(a, ma, bar, arow, k0);
-            load_2d_pair(a + kBox, ma, bar, arow + 64, k0);
+          if constexpr (kAnyA) {  // 64 x 64 boxes serve both layouts
+            load_2d_pair(a, ma, bar, p.a_mn ? arow : k0, p.a_mn ? k0 : arow);
+            load_2d_pair(a + kBox, ma, bar, p.a_mn ? arow + 64 : k0, p.a_mn ? k0 : arow + 64);
           } else {
             load_2d_pair(a, ma, bar, k0, arow);
           }
@@ -460,9 +486,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     }
   } else if (warp == 1) {
     if (lane == 0 && leader) {
-      const uint32_t id = idesc(kF16, kAMn, kBMn, 2 * BM, BN);
       int kit = 0, it = 0;
-      for (Items work(g.sched, unit); !*abort_flag && work.next(g.sched, item); ++it) {
+      for (Items work(g.sched, unit); !*abort_flag && work.next(g, item); ++it) {
+        const bool a_mn = kAnyA && g.p[item.prob].a_mn;
+        const uint32_t id = idesc(kF16, a_mn, kBMn, 2 * BM, BN);
         const int a = it & 1;
         if (!mbar_wait_cluster(&acc_empty[a], ((it >> 1) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
         tc_fence_after();
@@ -474,7 +501,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
           const uint32_t a0 = smem_u32(sA + s * kTileA), b0 = smem_u32(sB + s * kTileB);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            umma_pair(acc, tile_desc<kAMn>(a0, k), tile_desc<kBMn>(b0, k), id, kb != item.k0 || k != 0 ? 1u : 0u);
+            umma_pair(acc, a_mn ? tile_desc<true>(a0, k) : tile_desc<false>(a0, k), tile_desc<kBMn>(b0, k), id,
+                      kb != item.k0 || k != 0 ? 1u : 0u);
           umma_commit_both(&empty[s]);
         }
         // an aborted tile is not handed over: the odd CTA cannot see this CTA's abort flag
@@ -494,13 +522,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
     uint8_t* out = sOut + (warp - 2) * warp_bytes(kEpi);
     int it = 0;
     pdl_wait();
-    for (Items work(g.sched, unit); work.next(g.sched, item); ++it) {
+    for (Items work(g.sched, unit); work.next(g, item); ++it) {
       const int a = it & 1;
-      int prob, bm, bn;
-      tile_of(g, item.tile, prob, bm, bn);
-      const int row0 = bm * 2 * BM + (int)rank * BM + q * 32;
-      const int col0 = is_plain(kEpi) ? bn * BN + half * kWarpCols : bn * kFeat + half * (kFeat / 2);
-      const bool in = row0 < g.M && col0 < g.N;  // some of this warp's outputs exist
+      const Problem& p = g.p[item.prob];
+      const int row0 = item.bm * 2 * BM + (int)rank * BM + q * 32;
+      const int col0 = is_plain(kEpi) ? item.bn * BN + half * kWarpCols : item.bn * kFeat + half * (kFeat / 2);
+      const bool in = row0 < p.M && col0 < p.N;  // some of this warp's outputs exist
       float dh[32];
       if constexpr (is_bwd(kEpi)) {
         if (in) load_dh<kEpi, kF16>(g, row0 + lane, col0, dh);  // arrives while the MMAs run
@@ -536,7 +563,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
       } else if (in) {
         if constexpr (kEpi == kPlainF32) {
           for (int b = 0; b < 4; ++b) {
-            if (col0 + 32 * b >= g.N) break;  // warp-uniform
+            if (col0 + 32 * b >= p.N) break;  // warp-uniform
             float v[32];
             fetch(b, v);
             if (lane == 0) store_wait_read<0>();  // the store before has read this tile
@@ -548,13 +575,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
             fence_async();
             __syncwarp();
             if (lane == 0) {
-              store_2d(&maps.o[prob], out, col0 + 32 * b, row0);
+              store_2d(&maps.m[p.o], out, col0 + 32 * b, row0);
               store_commit();
             }
           }
         } else if constexpr (kEpi == kPlain) {
           for (int b = 0; b < 4; b += 2) {
-            if (col0 + 32 * b >= g.N) break;  // warp-uniform
+            if (col0 + 32 * b >= p.N) break;  // warp-uniform
             float v[64];
             fetch(b, v);
             fetch(b + 1, v + 32);
@@ -565,7 +592,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
             fence_async();
             __syncwarp();
             if (lane == 0) {
-              store_2d(&maps.o[prob], out, col0 + 32 * b, row0);
+              store_2d(&maps.m[p.o], out, col0 + 32 * b, row0);
               store_commit();
             }
           }
@@ -584,7 +611,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
           fence_async();
           __syncwarp();
           if (lane == 0) {
-            store_2d(&maps.o[0], out, col0, row0);
+            store_2d(&maps.m[p.o], out, col0, row0);
             store_commit();
           }
         } else {
@@ -593,7 +620,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
           uint8_t* th = tdu + kOutBlock;
 #pragma unroll 1
           for (int b = 0; b < 2; ++b) {
-            if (col0 + 32 * b >= g.N) break;  // warp-uniform
+            if (col0 + 32 * b >= p.N) break;  // warp-uniform
             float v[64];
             fetch(b, v);
             fetch(b + 2, v + 32);
@@ -603,29 +630,29 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
             for (int k = 0; k < 4; ++k) {  // 8 features each
               uint32_t og[4], ou[4], oh[4];
 #pragma unroll
-              for (int p = 0; p < 4; ++p) {
+              for (int i = 0; i < 4; ++i) {
                 float dg[2], du[2], h[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const int j = k * 8 + p * 2 + e;
+                  const int j = k * 8 + i * 2 + e;
                   gated_bwd(v[j], v[32 + j], dh[j], g.act, dg[e], du[e], h[e]);
                 }
-                og[p] = pack2<kF16>(dg[0], dg[1]);
-                ou[p] = pack2<kF16>(du[0], du[1]);
-                oh[p] = pack2<kF16>(h[0], h[1]);
+                og[i] = pack2<kF16>(dg[0], dg[1]);
+                ou[i] = pack2<kF16>(du[0], du[1]);
+                oh[i] = pack2<kF16>(h[0], h[1]);
               }
               *block_chunk(tdg, lane, k) = make_uint4(og[0], og[1], og[2], og[3]);
               *block_chunk(tdu, lane, k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
               *block_chunk(th, lane, k) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
             }
-            if (b == 0 && col0 + 32 < g.N) load_dh<kEpi, kF16>(g, row0 + lane, col0 + 32, dh);
+            if (b == 0 && col0 + 32 < p.N) load_dh<kEpi, kF16>(g, row0 + lane, col0 + 32, dh);
             fence_async();
             __syncwarp();
             if (lane == 0) {
               const int col = col0 + 32 * b;
-              store_2d(&maps.o[0], tdg, col, row0);
-              store_2d(&maps.o[1], tdu, col, row0);
-              if (g.want_h) store_2d(&maps.o[2], th, col, row0);
+              store_2d(&maps.m[p.o], tdg, col, row0);
+              store_2d(&maps.m[p.o + 1], tdu, col, row0);
+              if (g.want_h) store_2d(&maps.m[p.o + 2], th, col, row0);
               store_commit();
             }
           }
@@ -647,12 +674,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) k_ffn_pair(const __grid_const
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ffn_err, 1);
 }
 
-// Completes the cut tiles of a pair launch: adds each one's pieces in contraction
+// Completes the cut tiles of a pair launch (all of its problem 0): adds each one's pieces in contraction
 // order and runs the product's epilogue. A warp takes 32 rows x 16 columns (features),
 // lane l row l as the pieces were written: it reads whole 512-byte lines, all of a
 // thread's in flight at once, and writes whole sectors.
 struct JoinArgs {
-  PairArgs p;
+  PairArgs g;
   void* o[3];
   int64_t ldo[3];
 };
@@ -679,25 +706,27 @@ __device__ __forceinline__ void store_cols(void* p, int64_t e, int n, const floa
 }
 
 template <int kEpi, bool kF16>
-__global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const JoinArgs j) {
+__global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const __grid_constant__ JoinArgs j) {
   pdl_trigger();
-  const PairArgs& g = j.p;
+  const PairArgs& g = j.g;
+  const Problem& p0 = g.p[0];
   constexpr int kGroups = (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;  // of a piece's warp
   constexpr int kParts = is_plain(kEpi) ? 1 : 2;                                 // value, or g and u
   const int lane = threadIdx.x & 31;
   const int item = (int)(blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5));
-  const int group = item % kGroups, w16 = item / kGroups % (2 * kEpiWarps), tile = item / kGroups / (2 * kEpiWarps);
-  int prob, bm, bn;
-  tile_of(g, tile, prob, bm, bn);
+  const int group = item % kGroups, w16 = item / kGroups % (2 * kEpiWarps);
+  Item it;
+  it.tile = item / kGroups / (2 * kEpiWarps);
+  place_tile(g, it);
   const int half = (w16 & (kEpiWarps - 1)) >> 2;
-  const int64_t row = (int64_t)bm * 2 * BM + w16 / kEpiWarps * BM + (w16 & 3) * 32 + lane;
+  const int64_t row = (int64_t)it.bm * 2 * BM + w16 / kEpiWarps * BM + (w16 & 3) * 32 + lane;
   const int col =
-      (is_plain(kEpi) ? bn * BN + half * kWarpCols : bn * kFeat + half * (kFeat / 2)) + kJoinCols * group;
-  if (row >= g.M || col >= g.N) return;
-  const int n = g.N - col < kJoinCols ? g.N - col : kJoinCols;
+      (is_plain(kEpi) ? it.bn * BN + half * kWarpCols : it.bn * kFeat + half * (kFeat / 2)) + kJoinCols * group;
+  if (row >= p0.M || col >= p0.N) return;
+  const int n = p0.N - col < kJoinCols ? p0.N - col : kJoinCols;
   pdl_wait();
   const float4* src = reinterpret_cast<const float4*>(g.partials) +
-                      ((int64_t)tile * g.sched.ways * 2 * kEpiWarps + w16) * (kWarpPartial / 4) +
+                      ((int64_t)it.tile * g.sched.ways * 2 * kEpiWarps + w16) * (kWarpPartial / 4) +
                       group * (kJoinCols / 4) * 32 + lane;
   constexpr int64_t kPiece = (int64_t)2 * kEpiWarps * kWarpPartial / 4;
   float v[kParts][kJoinCols];
@@ -717,9 +746,9 @@ __global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const JoinArgs j) {
       }
   }
   if constexpr (kEpi == kPlain) {
-    store_cols<kF16>(j.o[prob], row * j.ldo[prob] + col, n, v[0]);
+    store_cols<kF16>(j.o[0], row * j.ldo[0] + col, n, v[0]);
   } else if constexpr (kEpi == kPlainF32) {
-    float* o = static_cast<float*>(j.o[prob]) + row * j.ldo[prob] + col;
+    float* o = static_cast<float*>(j.o[0]) + row * j.ldo[0] + col;
 #pragma unroll
     for (int c = 0; c < kJoinCols; c += 4) {
       if (c + 4 <= n) {
@@ -752,6 +781,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const JoinArgs j) {
 }
 
 // ---------------------------------------------------------- skinny kernel --
+
+struct Maps {
+  CUtensorMap a[2], b[2];  // weights (K segments, or gate and up), tokens
+};
 
 constexpr int kSkinnyThreads = 128;
 constexpr int kSkinnyPitch = 132;  // floats between tokens' 128 partials in shared memory
@@ -990,12 +1023,14 @@ struct Mat {
 struct Product {
   int epi = kPlain;
   bool a_mn = false, b_mn = false;  // operand stored [K, M] / [K, N]
-  int nseg = 1, nprob = 1;
+  int nseg = 1;
   Mat a[2], b[2];    // gated: a[0] = x, b = gate, up
   Mat o[3];          // outputs (backward: dg, du, h or null)
   Mat dh;
   int64_t M = 0, N = 0, K = 0;  // N: features of a gated form
   int act = 0;
+
+  int64_t kblocks() const { return (K + BK - 1) / BK * nseg; }
 };
 
 constexpr int kMaxDevices = 64;
@@ -1057,25 +1092,79 @@ constexpr size_t kJoinBytes = (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial *
 // The workspace's joining part; a call whose products are all skinny has none.
 size_t join_bytes(int64_t tokens) { return tokens <= kSkinnyTokens ? 0 : kJoinBytes; }
 
-// Deal `tiles` tiles of kb k-blocks over at most `most` pairs: full rounds of whole
-// tiles, and the last round's tiles cut when that saves enough.
-Sched make_sched(int tiles, int kb, int most) {
-  Sched s{tiles, kb, tiles < most ? tiles : most, 0, 1};
+// One problem of `tiles` tiles of kb k-blocks over at most `most` pairs: full rounds of
+// whole tiles, and the last round's tiles cut when that saves enough.
+Sched deal_one(int tiles, int kb, int most) {
+  Sched s{tiles < most ? tiles : most, 0, 1, 0, tiles, 0, 0};
   const int rest = tiles % most;
   if (rest == 0) return s;
   int ways = most / rest;
   if (ways > kMaxWays) ways = kMaxWays;
   if (ways > kb / kMinPieceKb) ways = kb / kMinPieceKb;
   if (ways < 2 || kb - kb / ways < kMinSavedKb) return s;
-  s.cut_tiles = rest;
+  s.long_tiles = rest;
   s.ways = ways;
-  s.units = tiles > most ? most : rest * ways;
+  s.n_long = rest * ways;
+  s.n_rest = tiles - rest;
+  s.units = tiles > most ? most : s.n_long;
   return s;
 }
 
-template <int kEpi, bool kAMn, bool kBMn, bool kF16>
-int launch_pair(const Product& q, Ctx& ctx) {
-  auto kernel = &k_ffn_pair<kEpi, kAMn, kBMn, kF16>;
+// `first` tiles of long_kb k-blocks and `rest` tiles of kb: the long ones first, cut
+// when one of them is more than a pair's share of the whole, the others so that the
+// pairs end together.
+Sched deal_two(int first, int64_t long_kb, int rest, int kb, int most) {
+  const int64_t share = (first * long_kb + (int64_t)rest * kb + most - 1) / most;
+  int ways = 1;
+  if (long_kb > share && first < most) {
+    ways = (int)((long_kb + share - 1) / share);
+    if (ways > kMaxWays) ways = kMaxWays;
+    if (ways > most / first) ways = most / first;
+    if (ways > long_kb / kMinPieceKb) ways = (int)(long_kb / kMinPieceKb);
+    if (ways < 1) ways = 1;
+  }
+  Sched s{most, first, ways, first * ways, rest, 0, 0};
+  if (s.n_long + rest < most) s.units = s.n_long + rest;
+  s.late_units = s.n_long % s.units;
+  const int64_t lead = (long_kb / ways + kb / 2) / kb;  // tiles that make up for a long item
+  const int64_t early = (lead > 0 ? lead : 1) * (s.units - s.late_units);
+  if (s.late_units > 0) s.early = (int)(early < rest ? early : rest);
+  return s;
+}
+
+// The launch's maps: one for every matrix and box.
+struct MapSet {
+  struct Key {
+    Mat x;
+    int box_cols, box_rows;
+  };
+  PairMaps maps;
+  Key keys[kMaxMaps];
+  int n = 0;
+  bool ok = true;
+
+  int add(CUtensorMapDataType type, const Mat& x, int box_cols, int box_rows) {
+    for (int i = 0; i < n; ++i) {
+      const Key& k = keys[i];
+      if (k.x.p == x.p && k.x.rows == x.rows && k.x.cols == x.cols && k.x.ld == x.ld && k.box_cols == box_cols &&
+          k.box_rows == box_rows)
+        return i;
+    }
+    if (n == kMaxMaps) {
+      ok = false;
+      return 0;
+    }
+    keys[n] = {x, box_cols, box_rows};
+    ok = ok && map_2d(&maps.m[n], type, x.p, x.rows, x.cols, x.ld, box_cols, box_rows);
+    return n++;
+  }
+};
+
+// `n` products of one kind in one launch; more than one only in the kAnyA form, the
+// first of them the one with the longest contraction, the others' alike.
+template <int kEpi, bool kAnyA, bool kBMn, bool kF16>
+int launch_pair(const Product* qs, int n, Ctx& ctx) {
+  auto kernel = &k_ffn_pair<kEpi, kAnyA, kBMn, kF16>;
   constexpr int smem = pair_smem(kEpi);
   constexpr CUtensorMapDataType t16 = kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   constexpr CUtensorMapDataType t32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
@@ -1094,49 +1183,55 @@ int launch_pair(const Product& q, Ctx& ctx) {
     entry.rc[dev] = MB_OK;
   });
   if (entry.rc[dev] != MB_OK) return entry.rc[dev];
-  Maps m;
-  bool ok = true;
-  const int na = is_plain(kEpi) ? (q.nseg > q.nprob ? q.nseg : q.nprob) : 1;
-  const int nb = is_plain(kEpi) ? q.nseg : 2;
-  for (int i = 0; i < na; ++i)
-    ok = ok && map_2d(&m.a[i], t16, q.a[i].p, q.a[i].rows, q.a[i].cols, q.a[i].ld, 64, kAMn ? 64 : BM);
-  for (int i = 0; i < nb; ++i)
-    ok = ok && map_2d(&m.b[i], t16, q.b[i].p, q.b[i].rows, q.b[i].cols, q.b[i].ld, 64, kBMn ? 64 : BN / 2);
-  constexpr bool f32_out = kEpi == kPlainF32;
-  for (int i = 0; i < 3; ++i)
-    if (q.o[i].p)
-      ok = ok && map_2d(&m.o[i], f32_out ? t32 : t16, q.o[i].p, q.o[i].rows, q.o[i].cols, q.o[i].ld,
-                        f32_out || is_bwd(kEpi) ? 32 : 64, 32);
-  if (!ok) return MB_ERR_CUDA;
-  for (int i = na; i < 2; ++i) m.a[i] = m.a[0];  // every map the kernel prefetches is one
-  for (int i = nb; i < 2; ++i) m.b[i] = m.b[0];
-  for (int i = 0; i < 3; ++i)
-    if (!q.o[i].p) m.o[i] = m.o[0];
-  const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), cols = is_plain(kEpi) ? BN : kFeat;
-  const int64_t nt = (q.N + cols - 1) / cols;
-  const int64_t work = mt * nt * q.nprob;
-  const int64_t kb = (q.K + BK - 1) / BK;
-  if (work > ((int64_t)1 << 30) || kb * q.nseg > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+  MapSet maps;
   PairArgs g{};
-  g.M = (int)q.M; g.N = (int)q.N;
-  g.kb = (int)kb; g.nseg = q.nseg; g.nprob = q.nprob;
-  g.mt = (int)mt; g.nt = (int)nt;
+  int64_t tiles = 0;
+  for (int i = 0; i < n; ++i) {
+    const Product& q = qs[i];
+    Problem& p = g.p[i];
+    p.M = (int)q.M; p.N = (int)q.N;
+    p.nseg = q.nseg;
+    p.a_mn = q.a_mn ? 1 : 0;
+    const int64_t cols = is_plain(kEpi) ? BN : kFeat;
+    const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), nt = (q.N + cols - 1) / cols;
+    if (q.kblocks() > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+    p.kb = (int)((q.K + BK - 1) / BK);
+    p.mt = (int)mt; p.nt = (int)nt; p.tile0 = (int)tiles;
+    tiles += mt * nt;
+    if (tiles > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+    const int nb = is_plain(kEpi) ? q.nseg : 2;
+    for (int k = 0; k < q.nseg; ++k) p.a[k] = maps.add(t16, q.a[k], 64, kAnyA ? 64 : BM);
+    for (int k = 0; k < nb; ++k) p.b[k] = maps.add(t16, q.b[k], 64, kBMn ? 64 : BN / 2);
+  }
+  constexpr bool f32_out = kEpi == kPlainF32;
+  for (int i = 0; i < n; ++i)
+    for (int k = 0; k < 3; ++k) {
+      if (!qs[i].o[k].p) continue;
+      const int m = maps.add(f32_out ? t32 : t16, qs[i].o[k], f32_out || is_bwd(kEpi) ? 32 : 64, 32);
+      if (k == 0) g.p[i].o = m;
+    }
+  if (!maps.ok) return MB_ERR_CUDA;
+  const Product& q = qs[0];
+  const int first = g.p[0].mt * g.p[0].nt;
+  g.nprob = n;
+  g.nmaps = maps.n;
   g.act = q.act; g.want_h = q.o[2].p != nullptr;
   g.dh = q.dh.p; g.lddh = q.dh.ld;
   take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
-  g.sched = make_sched((int)work, (int)(kb * q.nseg), entry.pairs[dev]);
+  g.sched = n == 1 ? deal_one(first, (int)q.kblocks(), entry.pairs[dev])
+                   : deal_two(first, q.kblocks(), (int)tiles - first, (int)qs[1].kblocks(), entry.pairs[dev]);
   g.partials = ctx.partials;
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t cfg = launch_config(at, 2 * g.sched.units, kPairThreads, smem, 2, &ctx);
-  if (cudaLaunchKernelEx(&cfg, kernel, m, g) != cudaSuccess) return MB_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, kernel, maps.maps, g) != cudaSuccess) return MB_ERR_CUDA;
   ctx.chained = true;
-  if (g.sched.cut_tiles == 0) return MB_OK;
+  if (g.sched.ways == 1) return MB_OK;
   JoinArgs j{g, {}, {}};
   for (int i = 0; i < 3; ++i) {
     j.o[i] = const_cast<void*>(q.o[i].p);
     j.ldo[i] = q.o[i].ld;
   }
-  const int warps = g.sched.cut_tiles * 2 * kEpiWarps * (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;
+  const int warps = g.sched.long_tiles * 2 * kEpiWarps * (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;
   cudaLaunchAttribute jat[2];
   cudaLaunchConfig_t join = launch_config(jat, warps / (kJoinThreads / 32), kJoinThreads, 0, 1, &ctx);
   return cudaLaunchKernelEx(&join, k_ffn_join<kEpi, kF16>, j) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
@@ -1211,23 +1306,36 @@ int launch_skinny(const Product& q, Ctx& ctx) {
 }
 
 template <bool kF16>
-int run_product(const Product& q, Ctx& st) {
-  const bool skinny = !q.a_mn && q.M <= kSkinnyTokens;
-  if (q.epi == kGated) return skinny ? launch_skinny<kGated, false, kF16>(q, st) : launch_pair<kGated, false, false, kF16>(q, st);
-  if (q.epi == kGatedBwd)
-    return skinny ? launch_skinny<kGatedBwd, false, kF16>(q, st) : launch_pair<kGatedBwd, false, false, kF16>(q, st);
-  if (q.epi == kGatedBwdF32)
-    return skinny ? launch_skinny<kGatedBwdF32, false, kF16>(q, st)
-                  : launch_pair<kGatedBwdF32, false, false, kF16>(q, st);
-  if (q.epi == kPlainF32)
-    return skinny ? launch_skinny<kPlainF32, true, kF16>(q, st) : launch_pair<kPlainF32, false, true, kF16>(q, st);
-  if (q.a_mn) return launch_pair<kPlain, true, true, kF16>(q, st);
-  if (q.b_mn) return skinny ? launch_skinny<kPlain, true, kF16>(q, st) : launch_pair<kPlain, false, true, kF16>(q, st);
-  return skinny ? launch_skinny<kPlain, false, kF16>(q, st) : launch_pair<kPlain, false, false, kF16>(q, st);
+int run_product(const Product& q, Ctx& ctx) {
+  const bool skinny = q.M <= kSkinnyTokens;
+  switch (q.epi) {
+    case kGated:
+      return skinny ? launch_skinny<kGated, false, kF16>(q, ctx) : launch_pair<kGated, false, false, kF16>(&q, 1, ctx);
+    case kGatedBwd:
+      return skinny ? launch_skinny<kGatedBwd, false, kF16>(q, ctx)
+                    : launch_pair<kGatedBwd, false, false, kF16>(&q, 1, ctx);
+    case kGatedBwdF32:
+      return skinny ? launch_skinny<kGatedBwdF32, false, kF16>(q, ctx)
+                    : launch_pair<kGatedBwdF32, false, false, kF16>(&q, 1, ctx);
+    case kPlainF32:
+      return skinny ? launch_skinny<kPlainF32, true, kF16>(q, ctx)
+                    : launch_pair<kPlainF32, false, true, kF16>(&q, 1, ctx);
+    default:
+      if (q.b_mn)
+        return skinny ? launch_skinny<kPlain, true, kF16>(q, ctx) : launch_pair<kPlain, true, true, kF16>(&q, 1, ctx);
+      return skinny ? launch_skinny<kPlain, false, kF16>(q, ctx) : launch_pair<kPlain, false, false, kF16>(&q, 1, ctx);
+  }
 }
 
 int product(int dtype, const Product& q, Ctx& ctx) {
   return dtype == MB_F16 ? run_product<true>(q, ctx) : run_product<false>(q, ctx);
+}
+
+// Products over 16-bit B stored [K, N], in one launch.
+int products(int dtype, const Product* q, int n, Ctx& ctx) {
+  if (n == 0) return MB_OK;
+  return dtype == MB_F16 ? launch_pair<kPlain, true, true, true>(q, n, ctx)
+                         : launch_pair<kPlain, true, true, false>(q, n, ctx);
 }
 
 // The call's context over the joining part of its workspace (its first kJoinBytes).
@@ -1403,6 +1511,10 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     rc = product(a->dtype, q, ctx);
     if (rc != MB_OK) return rc;
   }
+  // dx and the weight gradients need each other's results for nothing: one launch (a
+  // few tokens' dx is a stream over the weights, for the skinny kernel)
+  Product grads[kMaxProblems];
+  int n = 0;
   if (r->dx) {
     Product q;
     q.nseg = 2;
@@ -1412,36 +1524,26 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     q.b_mn = true;
     q.o[0] = {r->dx, T, d, r->lddx};
     q.M = T; q.N = d; q.K = f;
-    rc = product(a->dtype, q, ctx);
-    if (rc != MB_OK) return rc;
-  }
-  if (r->dgate || r->dup) {
-    Product q;
-    q.a_mn = q.b_mn = true;
-    q.nprob = 0;
-    if (r->dgate) {
-      q.a[q.nprob] = dg;
-      q.o[q.nprob++] = {r->dgate, f, d, r->ld_dgate};
+    if (T > kSkinnyTokens) {
+      grads[n++] = q;
+    } else {
+      rc = product(a->dtype, q, ctx);
+      if (rc != MB_OK) return rc;
     }
-    if (r->dup) {
-      q.a[q.nprob] = du;
-      q.o[q.nprob++] = {r->dup, f, d, r->ld_dup};
-    }
-    q.b[0] = x;
-    q.M = f; q.N = d; q.K = T;
-    rc = product(a->dtype, q, ctx);
-    if (rc != MB_OK) return rc;
   }
-  if (r->ddown) {
-    Product q;
+  auto weight = [&](const Mat& left, const Mat& right, void* out, int64_t ld) {  // out = left^T right
+    if (!out) return;
+    Product& q = grads[n++];
     q.a_mn = q.b_mn = true;
-    q.a[0] = dy;
-    q.b[0] = h;
-    q.o[0] = {r->ddown, d, f, r->ld_ddown};
-    q.M = d; q.N = f; q.K = T;
-    rc = product(a->dtype, q, ctx);
-  }
-  return rc;
+    q.a[0] = left;
+    q.b[0] = right;
+    q.o[0] = {out, left.cols, right.cols, ld};
+    q.M = left.cols; q.N = right.cols; q.K = T;
+  };
+  weight(dg, x, r->dgate, r->ld_dgate);
+  weight(du, x, r->dup, r->ld_dup);
+  weight(dy, h, r->ddown, r->ld_ddown);
+  return products(a->dtype, grads, n, ctx);
 }
 
 MB_API int mb_ffn_status(void) {
