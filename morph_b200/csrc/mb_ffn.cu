@@ -1045,6 +1045,13 @@ int current_device(int* sms) {
   static std::atomic<int> count[kMaxDevices];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -1;
+  // a thread that has made no call of the runtime yet (autograd's, say) has no context,
+  // and the tensor-map encoder is a driver call
+  static thread_local int bound = -1;
+  if (bound != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return -1;
+    bound = dev;
+  }
   int n = count[dev].load(std::memory_order_relaxed);
   if (n == 0) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return -1;
@@ -1084,6 +1091,7 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
   return cfg;
 }
 
+constexpr int kTileKb = 6;
 constexpr int kMaxPairs = 96;  // pairs a launch may have, for the size of its workspace
 // Tokens up to which the weight-streaming kernel runs.
 constexpr int64_t kSkinnyTokens = 128;
@@ -1112,11 +1120,13 @@ Sched deal_one(int tiles, int kb, int most) {
 
 // `first` tiles of long_kb k-blocks and `rest` tiles of kb: the long ones first, cut
 // when one of them is more than a pair's share of the whole, the others so that the
-// pairs end together.
+// pairs end together. A tile costs about kTileKb k-blocks' time beside its own
+// (filling the ring, storing).
 Sched deal_two(int first, int64_t long_kb, int rest, int kb, int most) {
-  const int64_t share = (first * long_kb + (int64_t)rest * kb + most - 1) / most;
+  const int64_t cost = kb + kTileKb;
+  const int64_t share = (first * (long_kb + kTileKb) + rest * cost + most - 1) / most;
   int ways = 1;
-  if (long_kb > share && first < most) {
+  if (long_kb > share) {
     ways = (int)((long_kb + share - 1) / share);
     if (ways > kMaxWays) ways = kMaxWays;
     if (ways > most / first) ways = most / first;
@@ -1126,7 +1136,7 @@ Sched deal_two(int first, int64_t long_kb, int rest, int kb, int most) {
   Sched s{most, first, ways, first * ways, rest, 0, 0};
   if (s.n_long + rest < most) s.units = s.n_long + rest;
   s.late_units = s.n_long % s.units;
-  const int64_t lead = (long_kb / ways + kb / 2) / kb;  // tiles that make up for a long item
+  const int64_t lead = (long_kb / ways + kTileKb + cost / 2) / cost;  // tiles that make up for a long item
   const int64_t early = (lead > 0 ? lead : 1) * (s.units - s.late_units);
   if (s.late_units > 0) s.early = (int)(early < rest ? early : rest);
   return s;
