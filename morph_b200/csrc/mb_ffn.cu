@@ -27,7 +27,7 @@
 //   * dx as one contraction over both (dg, Wg) and (du, Wu): one accumulator;
 //   * dWg and dWu as one launch;
 //   * stores through swizzled shared tiles and TMA, which clips ragged edges.
-// Tiles run in groups of kGroupM row tiles, so that what the ~74 pairs read at one
+// Tiles run in groups of 8 row tiles, so that what the ~74 pairs read at one
 // time (about 8 x 9 tiles' operands) stays in L2.
 //
 // Its grid is persistent: whole tiles in turn, and where the last round would leave
@@ -74,7 +74,7 @@ constexpr int kTileA = BM * BK * 2;         // 16 KiB: this CTA's rows of A
 constexpr int kTileB = (BN / 2) * BK * 2;   // 16 KiB: this CTA's half of B
 constexpr int kBox = 64 * 64 * 2;           // 8 KiB: one 64 x 64 MN-major box
 constexpr int kStoreTile = 32 * 64 * 2;     // 4 KiB: a warp's 32 rows x 64 columns
-constexpr int kGroupM = 8;
+constexpr int kGroupLog2 = 3;  // row tiles of a group: 8
 constexpr int kBarBytes = 512;
 constexpr uint32_t kTmemCols = 512;
 
@@ -84,16 +84,30 @@ enum Epi { kPlain = 0, kGated = 1, kGatedBwd = 2, kPlainF32 = 3, kGatedBwdF32 = 
 constexpr bool is_plain(int epi) { return epi == kPlain || epi == kPlainF32; }
 constexpr bool is_bwd(int epi) { return epi == kGatedBwd || epi == kGatedBwdF32; }
 
-// Ring stages and shared memory of an epilogue warp: one store tile, or in the
+// The ring, and shared memory of an epilogue warp: one store tile, or in the
 // backward form a 32 x 32 block each of dg, du and h.
 constexpr int kOutBlock = 32 * 32 * 2;
-constexpr int stages(int epi) { return is_bwd(epi) ? 5 : 6; }
+constexpr int ring_bytes(int epi) { return (is_bwd(epi) ? 5 : 6) * (kTileA + kTileB); }
 constexpr int warp_bytes(int epi) { return is_bwd(epi) ? 3 * kOutBlock : kStoreTile; }
 constexpr int pair_smem(int epi) {
-  return 1024 + stages(epi) * (kTileA + kTileB) + kEpiWarps * warp_bytes(epi) + kBarBytes;
+  return 1024 + ring_bytes(epi) + kEpiWarps * warp_bytes(epi) + kBarBytes;
 }
 static_assert(pair_smem(kPlain) <= 232448 && pair_smem(kGatedBwd) <= 232448, "shared memory of one SM");
 static_assert(warp_bytes(kGatedBwd) % 512 == 0, "swizzled blocks stay aligned");
+
+// Division of 0 <= x < 2^31 by a fixed d >= 1: floor(x m / 2^shift) with
+// m = ceil(2^shift / d), shift = 31 + ceil(log2 d), exact since m d - 2^shift < 2^(shift - 31).
+// The roles of a CTA find their next tile between two k-blocks: the compiler's
+// divisions by run-time values cost more there than a k-block takes.
+struct Div {
+  uint32_t m;
+  int shift;
+  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
+};
+
+template <int N> struct Int {
+  static constexpr int value = N;
+};
 
 // One problem of a pair launch: an output [M, N] (gated: N features) and up to two K
 // segments accumulated into it. Operands and output name the launch's maps.
@@ -104,6 +118,10 @@ struct Problem {
   int a[2], b[2];    // by segment; gated: b by CTA of the pair (gate, up)
   int o;             // backward: dg, du, h at o, o + 1, o + 2
   int mt, nt, tile0; // row and column tiles; its first tile's number
+  // groups of rows of tiles (of pairs of them with pairing 2): their number of rows
+  // (log2), the last one's, and the division by a group's tiles and by that last height
+  int group_log2, height, tail_rows;
+  Div by_group, by_tail;
 };
 
 constexpr int kMaxProblems = 4, kMaxMaps = 11;
@@ -112,17 +130,21 @@ struct PairMaps {
   CUtensorMap m[kMaxMaps];
 };
 
-// How a launch's tiles are dealt to its units (CTA pairs). The first long_tiles tiles
-// (all of problem 0) go first, whole (ways 1) or each cut into `ways` pieces: n_long
-// items in turn. Of the n_rest tiles after them, the first `early` go to the units from
-// `late_units` on, which had one long item less, and the others to all in turn.
+// How a launch's tiles are dealt to its units (CTA pairs). With pairing 2 the tiles
+// 2i and 2i + 1 are vertical neighbours, and a unit may take both as one item: they
+// share B's loads. The first long_tiles tiles (all of problem 0) go first: whole, in
+// items of long_step, or each cut into `ways` pieces: n_long items in turn. Of the
+// n_rest items after them (n_double double ones, then single tiles) the first `early`
+// go to the units from `late_units` on, which had one long item less, and the others
+// to all in turn.
 struct Sched {
-  int units, long_tiles, ways, n_long, n_rest, early, late_units;
+  int units, pairing, long_tiles, long_step, ways, n_long, n_rest, n_double, early, late_units;
 };
 
 struct PairArgs {
   Problem p[kMaxProblems];
   int nprob, nmaps;
+  int st, stage;  // ring stages and their bytes: A, B and, with pairing 2, the second tile's A
   Sched sched;
   float* partials;    // workspace of the pieces of cut tiles
   int act;
@@ -143,10 +165,10 @@ __device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint6
 }
 
 // Completes on the barrier at cluster address `bar` (the even CTA's); no multicast.
-__device__ __forceinline__ void load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-      "[%2];" ::"r"(smem_u32(dst)),
+      "[%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
@@ -183,12 +205,16 @@ __device__ __forceinline__ uint32_t idesc(bool f16, bool a_mn, bool b_mn, int m,
 // MN-major: boxes of 64 (MN) x 64 (K), one K index per 128-byte row: 8-K groups
 // 1024 B apart (SBO), the next 64 MN elements one box further (LBO); a 16-deep
 // slice is 16 rows = 2048 B further.
+__device__ __forceinline__ uint64_t desc_at(uint32_t saddr, bool mn) {
+  const uint64_t lbo = mn ? (uint64_t)(kBox >> 4) : 1u;
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (lbo << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+constexpr uint32_t desc_slice(bool mn) { return (mn ? 2048u : 32u) >> 4; }
+
 template <bool kMn>
 __device__ __forceinline__ uint64_t tile_desc(uint32_t saddr, int slice) {
-  const uint32_t a = saddr + (uint32_t)slice * (kMn ? 2048u : 32u);
-  const uint64_t lbo = kMn ? (uint64_t)(kBox >> 4) : 1u;
-  return (uint64_t)((a & 0x3FFFFu) >> 4) | (lbo << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)2 << 61);
+  return desc_at(saddr, kMn) + (uint32_t)slice * desc_slice(kMn);
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -278,31 +304,51 @@ __device__ __forceinline__ void store_quad(void* p, int64_t e, int n, const floa
 
 // ------------------------------------------------------------- scheduling --
 
+// Tiles go in twos (one load of B for both: 96 instead of 128 KB of operands) where the
+// contraction is long enough to cover that both epilogues end together, and there are
+// rounds enough: in k-blocks and rounds of tiles. Measured against single tiles: 4096
+// tokens, d 4096, f 11008: gate and up 478 -> 467 us, backward 2000 -> 1945; but the
+// backward of 2048 tokens, d 2048, f 5504 (8 rounds) 285 -> 292, of 1024 tokens, d 4096
+// (16 k-blocks) 549 -> 559. The backward projection's epilogue is too long for it
+// (417 -> 472 thousand cycles).
+constexpr int kTwosKb = 64, kTwosRounds = 2, kTwosKbGrads = 32, kTwosRoundsGrads = 16;
 // When a pair launch cuts its last round: pieces of at least kMinPieceKb k-blocks, at
 // most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time.
 constexpr int kMinPieceKb = 4, kMaxWays = 4, kMinSavedKb = 24;
 
-// One piece of work: k-blocks [k0, k1) of row tile bm, column tile bn of a problem;
-// `piece` of a cut tile, else -1.
+// One piece of work: k-blocks [k0, k1) of `count` tiles from row tile bm on, column
+// tile bn, of a problem; `piece` of a cut tile, else -1.
 struct Item {
-  int tile, prob, bm, bn, k0, k1, piece;
+  int tile, count, prob, bm, bn, k0, k1, piece;
 };
 
-// Tile -> problem and place: groups of kGroupM row tiles, row tiles fastest inside a group.
-__device__ __forceinline__ void place_tile(const PairArgs& g, Item& it) {
+// Tile -> problem and place: groups of 8 row tiles, row tiles fastest inside a
+// group. False for the tile below an odd number of row tiles.
+__device__ __forceinline__ bool place_tile(const PairArgs& g, Item& it) {
   it.prob = 0;
   for (int i = 1; i < kMaxProblems; ++i)
     if (i < g.nprob && it.tile >= g.p[i].tile0) it.prob = i;
   const Problem& p = g.p[it.prob];
+  const bool twos = g.sched.pairing == 2;
   const int t = it.tile - p.tile0;
-  const int first = t / (kGroupM * p.nt) * kGroupM;
-  const int rows = p.mt - first < kGroupM ? p.mt - first : kGroupM;
-  const int in = t - first * p.nt;
-  it.bm = first + in % rows;
-  it.bn = in / rows;
+  const int cell = twos ? t >> 1 : t;
+  const int group = p.by_group(cell), first = group << p.group_log2;
+  const int in = cell - first * p.nt;
+  int row;
+  if (p.height - first >= 1 << p.group_log2) {
+    row = in & ((1 << p.group_log2) - 1);
+    it.bn = in >> p.group_log2;
+  } else {
+    it.bn = p.by_tail(in);
+    row = in - it.bn * p.tail_rows;
+  }
+  row += first;
+  it.bm = twos ? 2 * row + (t & 1) : row;
   it.k0 = 0;
   it.k1 = p.kb * p.nseg;
   it.piece = -1;
+  if (it.bm + it.count > p.mt) it.count = p.mt - it.bm;
+  return it.count > 0;
 }
 
 struct Items {
@@ -311,30 +357,38 @@ struct Items {
       : unit(u), next_long(u), next_early(u >= s.late_units ? u - s.late_units : s.early), next_rest(s.early + u) {}
   __device__ __forceinline__ bool next(const PairArgs& g, Item& it) {
     const Sched& s = g.sched;
-    if (next_long < s.n_long) {
-      it.tile = next_long / s.ways;
-      place_tile(g, it);
-      if (s.ways > 1) {
-        const int kb = it.k1;
-        it.piece = next_long - it.tile * s.ways;
-        it.k0 = (int)((int64_t)kb * it.piece / s.ways);
-        it.k1 = (int)((int64_t)kb * (it.piece + 1) / s.ways);
+    while (true) {
+      if (next_long < s.n_long) {
+        int piece = 0;
+        it.tile = next_long * s.long_step;
+        if (s.ways > 1) {
+          it.tile = next_long / s.ways;
+          piece = next_long - it.tile * s.ways;
+        }
+        it.count = s.long_step;
+        next_long += s.units;
+        if (!place_tile(g, it)) continue;
+        if (s.ways > 1) {
+          const int kb = it.k1;
+          it.piece = piece;
+          it.k0 = (int)((int64_t)kb * piece / s.ways);
+          it.k1 = (int)((int64_t)kb * (piece + 1) / s.ways);
+        }
+        return true;
       }
-      next_long += s.units;
-      return true;
+      int j;
+      if (next_early < s.early) {
+        j = next_early;
+        next_early += s.units - s.late_units;
+      } else {
+        j = next_rest;
+        if (j >= s.n_rest) return false;
+        next_rest += s.units;
+      }
+      it.count = j < s.n_double ? 2 : 1;
+      it.tile = s.long_tiles + j + (j < s.n_double ? j : s.n_double);
+      if (place_tile(g, it)) return true;
     }
-    int j;
-    if (next_early < s.early) {
-      j = next_early;
-      next_early += s.units - s.late_units;
-    } else {
-      j = next_rest;
-      if (j >= s.n_rest) return false;
-      next_rest += s.units;
-    }
-    it.tile = s.long_tiles + j;
-    place_tile(g, it);
-    return true;
   }
 };
 
@@ -395,15 +449,13 @@ __device__ __forceinline__ void load_dh(const PairArgs& g, int64_t row, int col,
 template <int kEpi, bool kAnyA, bool kBMn, bool kF16>
 __global__ void __launch_bounds__(kPairThreads, 1)
     k_ffn_pair(const __grid_constant__ PairMaps maps, const __grid_constant__ PairArgs g) {
-  constexpr int ST = stages(kEpi);
+  constexpr int kMaxStages = ring_bytes(kEpi) / (kTileA + kTileB);
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sA = smem;
-  uint8_t* sB = sA + ST * kTileA;
-  uint8_t* sOut = sB + ST * kTileB;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sOut = ring + ring_bytes(kEpi);
   uint64_t* full = reinterpret_cast<uint64_t*>(sOut + kEpiWarps * warp_bytes(kEpi));
-  uint64_t* empty = full + ST;
-  uint64_t* acc_full = empty + ST;      // [2]
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* acc_full = empty + kMaxStages;  // [2]
   uint64_t* acc_empty = acc_full + 2;   // [2]: one arrival per epilogue warp of both CTAs
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -416,7 +468,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   Item item;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; ++s) {
+    for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -444,69 +496,148 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       pdl_wait();
-      int kit = 0;
+      // Issuing a stage must stay well under its MMAs' 512 cycles, so everything that an
+      // item fixes is out of the loop (two more loads under a run-time condition in it
+      // cost the weight gradients 11 %).
+      const int st = g.st;
+      const uint32_t stage = (uint32_t)g.stage;
+      const uint32_t full0 = mapa_u32(smem_u32(full), 0);  // the even CTA's barriers
+      const uint32_t ring0 = smem_u32(ring);
+      int s = 0, issued = 0;
+      uint32_t ph = 0;
       for (Items work(g.sched, unit); !*abort_flag && work.next(g, item);) {
         const Problem& p = g.p[item.prob];
         const int arow = item.bm * 2 * BM + (int)rank * BM;
         // gated tiles: 128 features from gate (even CTA) or up (odd CTA)
         const int brow = is_plain(kEpi) ? item.bn * BN + (int)rank * (BN / 2) : item.bn * kFeat;
-        for (int kb = item.k0; kb < item.k1; ++kb, ++kit) {
-          const int s = kit % ST;
-          if (!mbar_wait(&empty[s], ((kit / ST) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
-          if (item.tile == g.fault.unit && kb == 0) continue;  // test-only: withhold; the MMA warp's wait expires
-          const int seg = kb >= p.kb ? 1 : 0;
-          const int k0 = (kb - seg * p.kb) * BK;
-          const CUtensorMap* ma = &maps.m[p.a[seg]];
-          const CUtensorMap* mb_ = &maps.m[p.b[is_plain(kEpi) ? seg : (int)rank]];
-          const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
-          if (leader) mbar_expect_tx(&full[s], 2 * (kTileA + kTileB));
-          uint8_t* a = sA + s * kTileA;
-          uint8_t* b = sB + s * kTileB;
-          if constexpr (kAnyA) {  // 64 x 64 boxes serve both layouts
-            load_2d_pair(a, ma, bar, p.a_mn ? arow : k0, p.a_mn ? k0 : arow);
-            load_2d_pair(a + kBox, ma, bar, p.a_mn ? arow + 64 : k0, p.a_mn ? k0 : arow + 64);
-          } else {
-            load_2d_pair(a, ma, bar, k0, arow);
-          }
-          if constexpr (kBMn) {
-            load_2d_pair(b, mb_, bar, brow, k0);
-            load_2d_pair(b + kBox, mb_, bar, brow + 64, k0);
-          } else {
-            load_2d_pair(b, mb_, bar, k0, brow);
-          }
+        const bool a_mn = kAnyA && p.a_mn;
+        const uint32_t bytes = 2 * (item.count * kTileA + kTileB);
+        const int seg_kb = p.kb;
+        const CUtensorMap* ma = &maps.m[p.a[0]];
+        const CUtensorMap* mb_ = &maps.m[p.b[is_plain(kEpi) ? 0 : (int)rank]];
+        const CUtensorMap* ma1 = &maps.m[p.a[1]];
+        const CUtensorMap* mb1 = &maps.m[p.b[1]];
+        const bool withhold = item.tile == g.fault.unit && item.k0 == 0;  // test-only: the MMA warp's wait expires
+        int k0 = item.k0 * BK;
+        if (is_plain(kEpi) && item.k0 >= seg_kb) {
+          ma = ma1;
+          mb_ = mb1;
+          k0 -= seg_kb * BK;
         }
+        auto fill = [&](auto count) {  // one loop each for single and double tiles
+          constexpr bool two = decltype(count)::value == 2;
+          for (int kb = item.k0; kb < item.k1; ++kb) {
+            if (is_plain(kEpi) && kb == seg_kb) {  // the second segment
+              ma = ma1;
+              mb_ = mb1;
+              k0 = 0;
+            }
+            if (!mbar_wait(&empty[s], ph ^ 1, abort_flag, g.fault.limit_ns)) break;
+            if (!withhold || kb > 0) {
+              const uint32_t bar = full0 + 8u * (uint32_t)s;
+              const uint32_t a = ring0 + (uint32_t)s * stage, b = a + kTileA, a2 = b + kTileB;
+              if (leader) mbar_expect_tx(&full[s], bytes);
+              if constexpr (kAnyA) {  // 64 x 64 boxes serve both layouts
+                load_2d_pair(a, ma, bar, a_mn ? arow : k0, a_mn ? k0 : arow);
+                load_2d_pair(a + kBox, ma, bar, a_mn ? arow + 64 : k0, a_mn ? k0 : arow + 64);
+                if constexpr (two) {
+                  load_2d_pair(a2, ma, bar, a_mn ? arow + 256 : k0, a_mn ? k0 : arow + 256);
+                  load_2d_pair(a2 + kBox, ma, bar, a_mn ? arow + 320 : k0, a_mn ? k0 : arow + 320);
+                }
+              } else {
+                load_2d_pair(a, ma, bar, k0, arow);
+                if constexpr (two) load_2d_pair(a2, ma, bar, k0, arow + 256);
+              }
+              if constexpr (kBMn) {
+                load_2d_pair(b, mb_, bar, brow, k0);
+                load_2d_pair(b + kBox, mb_, bar, brow + 64, k0);
+              } else {
+                load_2d_pair(b, mb_, bar, k0, brow);
+              }
+            }
+            k0 += BK;
+            ++issued;
+            if (++s == st) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
+        };
+        if (item.count == 2) fill(Int<2>{});
+        else fill(Int<1>{});
       }
       if (*abort_flag && leader) {
         // bounded wait for both CTAs' loads still in flight (they land on the even CTA's barriers)
         const uint64_t t0 = globaltimer();
-        for (int k = kit - ST > 0 ? kit - ST : 0; k < kit; ++k)
-          while (!mbar_try_wait(&full[k % ST], (k / ST) & 1) && globaltimer() - t0 < g.fault.limit_ns) {
+        for (int k = issued - st > 0 ? issued - st : 0; k < issued; ++k)
+          while (!mbar_try_wait(&full[k % st], (k / st) & 1) && globaltimer() - t0 < g.fault.limit_ns) {
           }
       }
     }
   } else if (warp == 1) {
     if (lane == 0 && leader) {
-      int kit = 0, it = 0;
-      for (Items work(g.sched, unit); !*abort_flag && work.next(g, item); ++it) {
+      const int st = g.st;
+      const uint32_t ring0 = smem_u32(ring), stage16 = (uint32_t)g.stage >> 4;
+      int s = 0, it = 0;
+      uint32_t ph = 0;
+      for (Items work(g.sched, unit); !*abort_flag && work.next(g, item);) {
         const bool a_mn = kAnyA && g.p[item.prob].a_mn;
         const uint32_t id = idesc(kF16, a_mn, kBMn, 2 * BM, BN);
-        const int a = it & 1;
-        if (!mbar_wait_cluster(&acc_empty[a], ((it >> 1) & 1) ^ 1, abort_flag, g.fault.limit_ns)) break;
-        tc_fence_after();
-        const uint32_t acc = tmem + (uint32_t)(a * BN);
-        for (int kb = item.k0; kb < item.k1; ++kb, ++kit) {
-          const int s = kit % ST;
-          if (!mbar_wait(&full[s], (kit / ST) & 1, abort_flag, g.fault.limit_ns)) break;
-          tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + s * kTileA), b0 = smem_u32(sB + s * kTileB);
+        const uint64_t da0 = desc_at(ring0, a_mn), db0 = desc_at(ring0 + kTileA, kBMn);
+        const uint32_t a_slice = desc_slice(a_mn);
+        auto slot_free = [&](int i) {
+          return mbar_wait_cluster(&acc_empty[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, g.fault.limit_ns);
+        };
+        auto stage_here = [&] { return mbar_wait(&full[s], ph, abort_flag, g.fault.limit_ns); };
+        // stage s into accumulator slot i: tile m's A against B
+        auto multiply = [&](int stage, int m, int i, bool first) {
+          const uint32_t off = (uint32_t)stage * stage16;
+          const uint64_t da = da0 + off + (m == 0 ? 0 : (kTileA + kTileB) >> 4), db = db0 + off;
+          const uint32_t acc = tmem + (uint32_t)((i & 1) * BN);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            umma_pair(acc, a_mn ? tile_desc<true>(a0, k) : tile_desc<false>(a0, k), tile_desc<kBMn>(b0, k), id,
-                      kb != item.k0 || k != 0 ? 1u : 0u);
-          umma_commit_both(&empty[s]);
+            umma_pair(acc, da + (uint32_t)k * a_slice, db + (uint32_t)k * desc_slice(kBMn), id,
+                      first && k == 0 ? 0u : 1u);
+        };
+        auto advance = [&] {
+          if (++s == st) {
+            s = 0;
+            ph ^= 1;
+          }
+        };
+        const int n = item.k1 - item.k0;
+        if (!slot_free(it)) break;
+        tc_fence_after();
+        bool good = true;
+        if (item.count == 1) {
+          for (int kb = 0; kb < n; ++kb) {
+            if (!(good = stage_here())) break;
+            tc_fence_after();
+            multiply(s, 0, it, kb == 0);
+            umma_commit_both(&empty[s]);
+            advance();
+          }
+          // an aborted tile is not handed over: the odd CTA cannot see this CTA's abort flag
+          if (good) umma_commit_both(&acc_full[it & 1]);
+        } else {
+          // two tiles on the same B, stage by stage
+          for (int kb = 0; kb < n; ++kb) {
+            if (!(good = stage_here())) break;
+            tc_fence_after();
+            multiply(s, 0, it, kb == 0);
+            if (kb + 1 == n) umma_commit_both(&acc_full[it & 1]);
+            if (kb == 0) {  // the first tile starts while the epilogue still drains the second accumulator
+              if (!(good = slot_free(it + 1))) break;
+              tc_fence_after();
+            }
+            multiply(s, 1, it + 1, kb == 0);
+            umma_commit_both(&empty[s]);
+            advance();
+          }
+          if (good) umma_commit_both(&acc_full[(it + 1) & 1]);
         }
-        // an aborted tile is not handed over: the odd CTA cannot see this CTA's abort flag
-        if (!*abort_flag) umma_commit_both(&acc_full[a]);
+        if (!good) break;
+        it += item.count;
       }
       if (*abort_flag) {
         umma_commit_pair(drain);
@@ -520,20 +651,29 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int half = (warp - 2) >> 2;    // its half of the tile's columns (gated: features)
     const int w16 = (int)rank * kEpiWarps + half * 4 + q;
     uint8_t* out = sOut + (warp - 2) * warp_bytes(kEpi);
-    int it = 0;
+    int it = 0, ok = 1;
     pdl_wait();
-    for (Items work(g.sched, unit); work.next(g, item); ++it) {
+    Items work(g.sched, unit);
+    int m = 0;
+    item.count = 0;
+    while (true) {
+      if (m == item.count) {  // the next item's first tile, or this item's second
+        if (!work.next(g, item)) break;
+        m = 0;
+      }
       const int a = it & 1;
+      const uint32_t use = it >> 1;
+      ++it;
       const Problem& p = g.p[item.prob];
-      const int row0 = item.bm * 2 * BM + (int)rank * BM + q * 32;
+      const int row0 = (item.bm + m) * 2 * BM + (int)rank * BM + q * 32;
+      ++m;
       const int col0 = is_plain(kEpi) ? item.bn * BN + half * kWarpCols : item.bn * kFeat + half * (kFeat / 2);
       const bool in = row0 < p.M && col0 < p.N;  // some of this warp's outputs exist
       float dh[32];
       if constexpr (is_bwd(kEpi)) {
         if (in) load_dh<kEpi, kF16>(g, row0 + lane, col0, dh);  // arrives while the MMAs run
       }
-      int ok = 0;
-      if (lane == 0) ok = mbar_wait(&acc_full[a], (it >> 1) & 1, abort_flag, g.fault.limit_ns) && !*abort_flag;
+      if (lane == 0) ok = mbar_wait(&acc_full[a], use & 1, abort_flag, g.fault.limit_ns) && !*abort_flag;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
@@ -547,7 +687,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
       };
-      if (in && item.piece >= 0) {
+      // hand the accumulator back: every lane's loads of it are complete
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[a]), 0));
+      };
+      if (!in) {
+        release();
+      } else if (item.piece >= 0) {
         // the piece's partial: float4 j of lane l at j * 32 + l
         float4* mine = reinterpret_cast<float4*>(g.partials) +
                        ((int64_t)(item.tile * g.sched.ways + item.piece) * 2 * kEpiWarps + w16) * (kWarpPartial / 4) +
@@ -560,18 +708,24 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           for (int k = 0; k < 8; ++k)
             mine[(b * 8 + k) * 32] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
         }
-      } else if (in) {
+        release();
+      } else {
         if constexpr (kEpi == kPlainF32) {
+          float v[128];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) fetch(b, v + 32 * b);
+          release();
+#pragma unroll
           for (int b = 0; b < 4; ++b) {
             if (col0 + 32 * b >= p.N) break;  // warp-uniform
-            float v[32];
-            fetch(b, v);
             if (lane == 0) store_wait_read<0>();  // the store before has read this tile
             __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              *tile_chunk(out, lane, k) = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
-                                                     __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3]));
+            for (int k = 0; k < 8; ++k) {
+              const float* x = v + 32 * b + 4 * k;
+              *tile_chunk(out, lane, k) =
+                  make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+            }
             fence_async();
             __syncwarp();
             if (lane == 0) {
@@ -580,19 +734,29 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
           }
         } else if constexpr (kEpi == kPlain) {
-          for (int b = 0; b < 4; b += 2) {
-            if (col0 + 32 * b >= p.N) break;  // warp-uniform
-            float v[64];
+          uint32_t w[4][16];  // the warp's 128 columns, rounded
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            float v[32];
             fetch(b, v);
-            fetch(b + 1, v + 32);
-            if (lane == 0) store_wait_read<0>();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[b][k] = pack2<kF16>(v[2 * k], v[2 * k + 1]);
+          }
+          release();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (col0 + 64 * h >= p.N) break;  // warp-uniform
+            if (lane == 0) store_wait_read<0>();  // the store before has read this tile
             __syncwarp();
-            put_row<kF16>(out, lane, 0, v);
-            put_row<kF16>(out, lane, 4, v + 32);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint32_t* x = w[2 * h + c / 4] + 4 * (c % 4);
+              *tile_chunk(out, lane, c) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
             fence_async();
             __syncwarp();
             if (lane == 0) {
-              store_2d(&maps.m[p.o], out, col0 + 32 * b, row0);
+              store_2d(&maps.m[p.o], out, col0 + 64 * h, row0);
               store_commit();
             }
           }
@@ -604,6 +768,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             float v[64];
             fetch(b, v);
             fetch(b + 2, v + 32);
+            if (b == 1) release();
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = gated(v[j], v[32 + j], g.act);
             put_row<kF16>(out, lane, 4 * b, v);
@@ -620,10 +785,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           uint8_t* th = tdu + kOutBlock;
 #pragma unroll 1
           for (int b = 0; b < 2; ++b) {
-            if (col0 + 32 * b >= p.N) break;  // warp-uniform
+            const bool last = b == 1 || col0 + 32 >= p.N;  // warp-uniform
             float v[64];
             fetch(b, v);
             fetch(b + 2, v + 32);
+            if (last) release();
             if (lane == 0) store_wait_read<0>();  // the block before has been read out
             __syncwarp();
 #pragma unroll
@@ -645,7 +811,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
               *block_chunk(tdu, lane, k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
               *block_chunk(th, lane, k) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
             }
-            if (b == 0 && col0 + 32 < p.N) load_dh<kEpi, kF16>(g, row0 + lane, col0 + 32, dh);
+            if (!last) load_dh<kEpi, kF16>(g, row0 + lane, col0 + 32, dh);
             fence_async();
             __syncwarp();
             if (lane == 0) {
@@ -655,12 +821,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
               if (g.want_h) store_2d(&maps.m[p.o + 2], th, col, row0);
               store_commit();
             }
+            if (last) break;
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[a]), 0));
     }
     if (lane == 0) store_wait_read<0>();  // the stores have read their tiles; the kernel's end completes them
     __syncwarp();
@@ -717,7 +881,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const __grid_constant
   const int group = item % kGroups, w16 = item / kGroups % (2 * kEpiWarps);
   Item it;
   it.tile = item / kGroups / (2 * kEpiWarps);
-  place_tile(g, it);
+  it.count = 1;
+  if (!place_tile(g, it)) return;
   const int half = (w16 & (kEpiWarps - 1)) >> 2;
   const int64_t row = (int64_t)it.bm * 2 * BM + w16 / kEpiWarps * BM + (w16 & 3) * 32 + lane;
   const int col =
@@ -1092,6 +1257,7 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
 }
 
 constexpr int kTileKb = 6;
+constexpr int kLongDouble = 4;  // long tiles go in twos while one is at most this part of a pair's share
 constexpr int kMaxPairs = 96;  // pairs a launch may have, for the size of its workspace
 // Tokens up to which the weight-streaming kernel runs.
 constexpr int64_t kSkinnyTokens = 128;
@@ -1101,20 +1267,27 @@ constexpr size_t kJoinBytes = (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial *
 size_t join_bytes(int64_t tokens) { return tokens <= kSkinnyTokens ? 0 : kJoinBytes; }
 
 // One problem of `tiles` tiles of kb k-blocks over at most `most` pairs: full rounds of
-// whole tiles, and the last round's tiles cut when that saves enough.
-Sched deal_one(int tiles, int kb, int most) {
-  Sched s{tiles < most ? tiles : most, 0, 1, 0, tiles, 0, 0};
-  const int rest = tiles % most;
-  if (rest == 0) return s;
-  int ways = most / rest;
+// whole tiles (double ones with pairing 2), and the last round's tiles cut when that
+// saves enough.
+Sched deal_one(int tiles, int kb, int most, int pairing) {
+  Sched s{};
+  s.units = tiles < most ? tiles : most;
+  s.pairing = pairing;
+  s.long_step = s.ways = 1;
+  int rest = tiles % most;
+  int ways = rest ? most / rest : 1;
   if (ways > kMaxWays) ways = kMaxWays;
   if (ways > kb / kMinPieceKb) ways = kb / kMinPieceKb;
-  if (ways < 2 || kb - kb / ways < kMinSavedKb) return s;
-  s.long_tiles = rest;
-  s.ways = ways;
-  s.n_long = rest * ways;
-  s.n_rest = tiles - rest;
-  s.units = tiles > most ? most : s.n_long;
+  if (rest && pairing == 2 && (rest & 1)) ++rest;  // what follows starts on a pair
+  if (ways >= 2 && rest * ways <= most && kb - kb / ways >= kMinSavedKb) {
+    s.long_tiles = rest;
+    s.ways = ways;
+    s.n_long = rest * ways;
+    s.units = tiles > most ? most : s.n_long;
+  }
+  const int whole = tiles - s.long_tiles;
+  s.n_double = pairing == 2 ? whole / (2 * most) * most : 0;
+  s.n_rest = whole - s.n_double;
   return s;
 }
 
@@ -1122,24 +1295,44 @@ Sched deal_one(int tiles, int kb, int most) {
 // when one of them is more than a pair's share of the whole, the others so that the
 // pairs end together. A tile costs about kTileKb k-blocks' time beside its own
 // (filling the ring, storing).
-Sched deal_two(int first, int64_t long_kb, int rest, int kb, int most) {
+Sched deal_two(int first, int64_t long_kb, int rest, int kb, int most, int pairing) {
   const int64_t cost = kb + kTileKb;
   const int64_t share = (first * (long_kb + kTileKb) + rest * cost + most - 1) / most;
-  int ways = 1;
+  Sched s{};
+  s.pairing = pairing;
+  s.long_tiles = first;
+  s.ways = s.long_step = 1;
   if (long_kb > share) {
-    ways = (int)((long_kb + share - 1) / share);
+    int ways = (int)((long_kb + share - 1) / share);
     if (ways > kMaxWays) ways = kMaxWays;
     if (ways > most / first) ways = most / first;
     if (ways > long_kb / kMinPieceKb) ways = (int)(long_kb / kMinPieceKb);
-    if (ways < 1) ways = 1;
+    if (ways > 1) s.ways = ways;
+  } else if (pairing == 2 && kLongDouble * long_kb <= share) {
+    s.long_step = 2;
   }
-  Sched s{most, first, ways, first * ways, rest, 0, 0};
-  if (s.n_long + rest < most) s.units = s.n_long + rest;
+  s.n_long = first / s.long_step * s.ways;
+  // double tiles but for about the last two rounds
+  if (pairing == 2 && rest > 4 * most) s.n_double = (rest - 2 * most) / 2;
+  s.n_rest = rest - s.n_double;
+  s.units = s.n_long + s.n_rest < most ? s.n_long + s.n_rest : most;
   s.late_units = s.n_long % s.units;
-  const int64_t lead = (long_kb / ways + kTileKb + cost / 2) / cost;  // tiles that make up for a long item
-  const int64_t early = (lead > 0 ? lead : 1) * (s.units - s.late_units);
-  if (s.late_units > 0) s.early = (int)(early < rest ? early : rest);
+  if (s.late_units > 0) {
+    // items that make up for a long one
+    const int64_t one = s.n_double > 0 ? 2 * cost : cost;
+    const int64_t lead = (s.long_step * long_kb / s.ways + kTileKb + one / 2) / one;
+    const int64_t early = (lead > 0 ? lead : 1) * (s.units - s.late_units);
+    const int most_early = s.n_double > 0 ? s.n_double : rest;
+    s.early = (int)(early < most_early ? early : most_early);
+  }
   return s;
+}
+
+Div make_div(int64_t d) {
+  int log = 0;
+  while (((int64_t)1 << log) < d) ++log;
+  const int shift = 31 + log;
+  return {(uint32_t)((((uint64_t)1 << shift) + (uint64_t)d - 1) / (uint64_t)d), shift};
 }
 
 // The launch's maps: one for every matrix and box.
@@ -1204,11 +1397,11 @@ int launch_pair(const Product* qs, int n, Ctx& ctx) {
     p.a_mn = q.a_mn ? 1 : 0;
     const int64_t cols = is_plain(kEpi) ? BN : kFeat;
     const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), nt = (q.N + cols - 1) / cols;
+    tiles += mt * nt;
+    if (tiles > ((int64_t)1 << 29)) return MB_ERR_TOO_LARGE;
     if (q.kblocks() > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
     p.kb = (int)((q.K + BK - 1) / BK);
-    p.mt = (int)mt; p.nt = (int)nt; p.tile0 = (int)tiles;
-    tiles += mt * nt;
-    if (tiles > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+    p.mt = (int)mt; p.nt = (int)nt;
     const int nb = is_plain(kEpi) ? q.nseg : 2;
     for (int k = 0; k < q.nseg; ++k) p.a[k] = maps.add(t16, q.a[k], 64, kAnyA ? 64 : BM);
     for (int k = 0; k < nb; ++k) p.b[k] = maps.add(t16, q.b[k], 64, kBMn ? 64 : BN / 2);
@@ -1222,14 +1415,31 @@ int launch_pair(const Product* qs, int n, Ctx& ctx) {
     }
   if (!maps.ok) return MB_ERR_CUDA;
   const Product& q = qs[0];
-  const int first = g.p[0].mt * g.p[0].nt;
+  const int most = entry.pairs[dev];
+  const bool twos = !is_bwd(kEpi) && tiles >= (n > 1 ? kTwosRoundsGrads : kTwosRounds) * most &&
+                    qs[n - 1].kblocks() >= (n > 1 ? kTwosKbGrads : kTwosKb);
+  const int pairing = twos ? 2 : 1;
+  int total = 0, first = 0;
+  for (int i = 0; i < n; ++i) {
+    Problem& p = g.p[i];
+    p.tile0 = total;
+    p.group_log2 = pairing == 2 ? kGroupLog2 - 1 : kGroupLog2;
+    p.height = (p.mt + pairing - 1) / pairing;
+    p.tail_rows = p.height & ((1 << p.group_log2) - 1);
+    p.by_group = make_div(p.nt << p.group_log2);
+    p.by_tail = make_div(p.tail_rows > 0 ? p.tail_rows : 1);
+    total += (g.p[i].mt + pairing - 1) / pairing * pairing * g.p[i].nt;
+    if (i == 0) first = total;
+  }
+  g.stage = pairing * kTileA + kTileB;
+  g.st = ring_bytes(kEpi) / g.stage;
   g.nprob = n;
   g.nmaps = maps.n;
   g.act = q.act; g.want_h = q.o[2].p != nullptr;
   g.dh = q.dh.p; g.lddh = q.dh.ld;
   take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
-  g.sched = n == 1 ? deal_one(first, (int)q.kblocks(), entry.pairs[dev])
-                   : deal_two(first, q.kblocks(), (int)tiles - first, (int)qs[1].kblocks(), entry.pairs[dev]);
+  g.sched = n == 1 ? deal_one(first, (int)q.kblocks(), most, pairing)
+                   : deal_two(first, q.kblocks(), total - first, (int)qs[1].kblocks(), most, pairing);
   g.partials = ctx.partials;
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t cfg = launch_config(at, 2 * g.sched.units, kPairThreads, smem, 2, &ctx);
