@@ -422,9 +422,11 @@ MB_API int mb_act_unpack(const uint8_t* codes, const uint8_t* scales, int64_t ro
 
 /* One gated feed-forward block (the SwiGLU of morph/model/morph_model.py:23-28):
  * x [tokens, d], gate and up [f, d], down [d, f], all `dtype` (MB_BF16 or
- * MB_F16), row-major with row pitches ld (elements, multiples of 8) and 16-byte
- * aligned bases. Products accumulate in FP32; h and the gradients of x gate^T and
- * x up^T are rounded to `dtype` once each, as the next product's operand. */
+ * MB_F16), row-major with row pitches ld (elements). Products accumulate in FP32;
+ * h and the gradients of x gate^T and x up^T are rounded to `dtype` once each, as
+ * the next product's operand. Matrices whose rows do not start on 16 bytes (base,
+ * or a pitch that is no multiple of 8) are copied through the workspace, which then
+ * has to be mb_ffn_padding_bytes larger (else MB_ERR_ALIGN). */
 typedef struct mb_ffn_args {
   int32_t dtype;
   int32_t activation; /* MB_ACT_* */
@@ -442,6 +444,7 @@ typedef struct mb_ffn_args {
 /* h = act(x gate^T) * (x up^T), [tokens, f]. Workspaces (device, 256-byte aligned)
  * need no preparation and hold nothing after the call; calls that may overlap need
  * one each. */
+MB_API size_t mb_ffn_padding_bytes(int64_t tokens, int64_t d, int64_t f);
 MB_API size_t mb_gated_linear_workspace_bytes(int64_t tokens);
 MB_API int mb_gated_linear(const mb_ffn_args* args, void* h, int64_t ldh, void* workspace, size_t workspace_bytes,
                            mb_stream_t stream);

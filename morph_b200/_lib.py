@@ -114,6 +114,7 @@ SIGNATURES = {
     "mb_fp8_unpack": (ctypes.c_int, [_p, _p, _i64, _p, _i32, _p]),
     "mb_act_pack": (ctypes.c_int, [_p, _i32, _i64, _i64, _i64, _p, _p, _p]),
     "mb_act_unpack": (ctypes.c_int, [_p, _p, _i64, _i64, _p, _i32, _i64, _p]),
+    "mb_ffn_padding_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
     "mb_gated_linear_workspace_bytes": (ctypes.c_size_t, [_i64]),
     "mb_gated_linear": (ctypes.c_int, [_p, _p, _i64, _p, ctypes.c_size_t, _p]),
     "mb_feed_forward_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),

@@ -1160,6 +1160,44 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ffn_err, 1);
 }
 
+// -------------------------------------------------------------- alignment --
+
+// TMA takes rows that start on 16 bytes. A call's matrices whose rows do not are
+// copied to (outputs: from) padded rows of the workspace, all in one launch: a warp a
+// row, consecutive lanes consecutive elements.
+struct CopyJob {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t src_ld, dst_ld, rows, cols;
+};
+
+constexpr int kMaxCopies = 5;  // x, gate, up, down, dy; or the four gradients
+
+struct CopyJobs {
+  CopyJob j[kMaxCopies];
+};
+
+constexpr int kCopyThreads = 256;
+
+__global__ void __launch_bounds__(kCopyThreads) k_ffn_copy(const __grid_constant__ CopyJobs jobs) {
+  const CopyJob& j = jobs.j[blockIdx.y];
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = (int64_t)gridDim.x * (kCopyThreads / 32);
+  for (int64_t row = (int64_t)blockIdx.x * (kCopyThreads / 32) + (threadIdx.x >> 5); row < j.rows; row += warps) {
+    const uint16_t* src = j.src + row * j.src_ld;
+    uint16_t* dst = j.dst + row * j.dst_ld;
+    for (int64_t c = lane; c < j.cols; c += 32 * 8) {
+      uint16_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + 32 * i < j.cols) v[i] = src[c + 32 * i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + 32 * i < j.cols) dst[c + 32 * i] = v[i];
+    }
+  }
+}
+
 // ------------------------------------------------------------------ host --
 
 // 2-D tensor [rows][cols] of `type`, row pitch ld (elements); boxes of 64 or 128
@@ -1566,13 +1604,62 @@ constexpr int64_t kMaxDim = (int64_t)1 << 30;
 int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 size_t area(int64_t rows, int64_t cols) { return ((size_t)rows * (size_t)pad8(cols) * 2 + 255) / 256 * 256; }
 
-// A caller's matrix: 16-byte aligned rows, as TMA needs them.
+// A caller's matrix: whole elements, rows that do not overlap.
 int check_mat(const void* p, int64_t cols, int64_t ld) {
-  if (!p) return MB_ERR_ARG;
-  if (ld < cols) return MB_ERR_ARG;
-  if (ld % 8 || !aligned(p, 16) || ld >= ((int64_t)1 << 36)) return MB_ERR_ALIGN;
+  if (!p || ld < cols) return MB_ERR_ARG;
+  if (!aligned(p, 2) || ld >= ((int64_t)1 << 36)) return MB_ERR_ALIGN;
   return MB_OK;
 }
+
+// The end of a call's workspace, from which padded copies of unaligned matrices are cut.
+class Padding {
+ public:
+  Padding(void* base, size_t bytes) : next_(static_cast<uint8_t*>(base)), left_(bytes) {}
+
+  // The matrix as the kernels may read it.
+  Mat in(const void* p, int64_t rows, int64_t cols, int64_t ld) {
+    if (!p) return {};
+    return fits(p, rows, ld) ? Mat{p, rows, cols, rows > 1 ? ld : pad8(cols)} : copy(in_, n_in_, p, rows, cols, ld, false);
+  }
+  // The matrix as the kernels may write it.
+  Mat out(void* p, int64_t rows, int64_t cols, int64_t ld) {
+    if (!p) return {};
+    return fits(p, rows, ld) ? Mat{p, rows, cols, rows > 1 ? ld : pad8(cols)} : copy(out_, n_out_, p, rows, cols, ld, true);
+  }
+  int status() const { return rc_; }
+  int before(cudaStream_t st) const { return launch(in_, n_in_, st); }
+  int after(cudaStream_t st) const { return launch(out_, n_out_, st); }
+
+ private:
+  static bool fits(const void* p, int64_t rows, int64_t ld) { return aligned(p, 16) && (ld % 8 == 0 || rows <= 1); }
+
+  Mat copy(CopyJobs& jobs, int& n, const void* p, int64_t rows, int64_t cols, int64_t ld, bool back) {
+    const size_t need = area(rows, cols);
+    if (n == kMaxCopies || left_ < need) {
+      rc_ = MB_ERR_ALIGN;
+      return {};
+    }
+    const Mat m{next_, rows, cols, pad8(cols)};
+    next_ += need;
+    left_ -= need;
+    uint16_t *mine = static_cast<uint16_t*>(const_cast<void*>(m.p)), *theirs = static_cast<uint16_t*>(const_cast<void*>(p));
+    jobs.j[n++] = back ? CopyJob{mine, theirs, m.ld, ld, rows, cols} : CopyJob{theirs, mine, ld, m.ld, rows, cols};
+    return m;
+  }
+  static int launch(const CopyJobs& jobs, int n, cudaStream_t st) {
+    if (n == 0) return MB_OK;
+    int64_t rows = 0;
+    for (int i = 0; i < n; ++i) rows = jobs.j[i].rows > rows ? jobs.j[i].rows : rows;
+    const int64_t blocks = (rows + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
+    k_ffn_copy<<<dim3((unsigned)(blocks < 1184 ? blocks : 1184), (unsigned)n), kCopyThreads, 0, st>>>(jobs);
+    return cudaGetLastError() == cudaSuccess ? MB_OK : MB_ERR_CUDA;
+  }
+
+  uint8_t* next_;
+  size_t left_;
+  CopyJobs in_, out_;
+  int n_in_ = 0, n_out_ = 0, rc_ = MB_OK;
+};
 
 int check_args(const mb_ffn_args* a, bool need_x, bool need_down) {
   if (!a) return MB_ERR_ARG;
@@ -1588,12 +1675,12 @@ int check_args(const mb_ffn_args* a, bool need_x, bool need_down) {
   return rc;
 }
 
-Product gated_product(const mb_ffn_args* a, const Mat& x) {
+Product gated_product(const mb_ffn_args* a, const Mat& x, const Mat& gate, const Mat& up) {
   Product q;
   q.epi = kGated;
   q.a[0] = x;
-  q.b[0] = {a->gate, a->f, a->d, a->ld_gate};
-  q.b[1] = {a->up, a->f, a->d, a->ld_up};
+  q.b[0] = gate;
+  q.b[1] = up;
   q.M = a->tokens; q.N = a->f; q.K = a->d;
   q.act = a->activation;
   return q;
@@ -1611,24 +1698,14 @@ using namespace mb::ffn;
 
 extern "C" {
 
-MB_API size_t mb_gated_linear_workspace_bytes(int64_t tokens) {
-  return tokens <= 0 || tokens > kMaxDim ? 0 : join_bytes(tokens);
+MB_API size_t mb_ffn_padding_bytes(int64_t tokens, int64_t d, int64_t f) {
+  if (tokens <= 0 || d <= 0 || f <= 0 || tokens > kMaxDim || d > kMaxDim || f > kMaxDim) return 0;
+  // x, dy, dx or y over d; dh or h over f; the weights and their gradients
+  return 3 * area(tokens, d) + area(tokens, f) + 4 * area(f, d) + 2 * area(d, f);
 }
 
-MB_API int mb_gated_linear(const mb_ffn_args* a, void* h, int64_t ldh, void* workspace, size_t workspace_bytes,
-                           mb_stream_t stream) {
-  int rc = check_args(a, true, false);
-  if (rc != MB_OK) return rc;
-  if (a->tokens == 0) return MB_OK;
-  rc = check_mat(h, a->f, ldh);
-  if (rc != MB_OK) return rc;
-  const size_t need = mb_gated_linear_workspace_bytes(a->tokens);
-  if ((need > 0 && !workspace) || workspace_bytes < need) return MB_ERR_ARG;
-  if (!aligned(workspace, 256)) return MB_ERR_ALIGN;
-  Ctx ctx = make_ctx(workspace, (cudaStream_t)stream);
-  Product q = gated_product(a, {a->x, a->tokens, a->d, a->ldx});
-  q.o[0] = {h, a->tokens, a->f, ldh};
-  return product(a->dtype, q, ctx);
+MB_API size_t mb_gated_linear_workspace_bytes(int64_t tokens) {
+  return tokens <= 0 || tokens > kMaxDim ? 0 : join_bytes(tokens);
 }
 
 MB_API size_t mb_feed_forward_workspace_bytes(int64_t tokens, int64_t f) {
@@ -1636,27 +1713,48 @@ MB_API size_t mb_feed_forward_workspace_bytes(int64_t tokens, int64_t f) {
   return join_bytes(tokens) + area(tokens, f);
 }
 
+// Both forward entries: without down, y is h.
+static int forward(const mb_ffn_args* a, bool with_down, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                   cudaStream_t st) {
+  int rc = check_args(a, true, with_down);
+  if (rc != MB_OK) return rc;
+  const int64_t T = a->tokens, d = a->d, f = a->f, width = with_down ? d : f;
+  if (T == 0) return MB_OK;
+  rc = check_mat(y, width, ldy);
+  if (rc != MB_OK) return rc;
+  const size_t need = with_down ? mb_feed_forward_workspace_bytes(T, f) : mb_gated_linear_workspace_bytes(T);
+  if ((need > 0 && !workspace) || workspace_bytes < need) return MB_ERR_ARG;
+  if (!aligned(workspace, 256)) return MB_ERR_ALIGN;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Padding pad(ws + need, workspace ? workspace_bytes - need : 0);
+  const Mat x = pad.in(a->x, T, d, a->ldx), gate = pad.in(a->gate, f, d, a->ld_gate), up = pad.in(a->up, f, d, a->ld_up);
+  const Mat down = with_down ? pad.in(a->down, d, f, a->ld_down) : Mat{}, out = pad.out(y, T, width, ldy);
+  if (pad.status() != MB_OK) return pad.status();
+  rc = pad.before(st);
+  if (rc != MB_OK) return rc;
+  Ctx ctx = make_ctx(workspace, st);  // its first kernel is not chained to the copies: it reads them at once
+  Product q = gated_product(a, x, gate, up);
+  q.o[0] = with_down ? Mat{ws + join_bytes(T), T, f, pad8(f)} : out;
+  rc = product(a->dtype, q, ctx);
+  if (rc == MB_OK && with_down) {
+    Product p;
+    p.a[0] = q.o[0];
+    p.b[0] = down;
+    p.o[0] = out;
+    p.M = T; p.N = d; p.K = f;
+    rc = product(a->dtype, p, ctx);
+  }
+  return rc == MB_OK ? pad.after(st) : rc;
+}
+
+MB_API int mb_gated_linear(const mb_ffn_args* a, void* h, int64_t ldh, void* workspace, size_t workspace_bytes,
+                           mb_stream_t stream) {
+  return forward(a, false, h, ldh, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
 MB_API int mb_feed_forward(const mb_ffn_args* a, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
                            mb_stream_t stream) {
-  int rc = check_args(a, true, true);
-  if (rc != MB_OK) return rc;
-  if (a->tokens == 0) return MB_OK;
-  rc = check_mat(y, a->d, ldy);
-  if (rc != MB_OK) return rc;
-  if (!workspace || workspace_bytes < mb_feed_forward_workspace_bytes(a->tokens, a->f)) return MB_ERR_ARG;
-  if (!aligned(workspace, 256)) return MB_ERR_ALIGN;
-  Ctx ctx = make_ctx(workspace, (cudaStream_t)stream);
-  const Mat h{static_cast<uint8_t*>(workspace) + join_bytes(a->tokens), a->tokens, a->f, pad8(a->f)};
-  Product q = gated_product(a, {a->x, a->tokens, a->d, a->ldx});
-  q.o[0] = h;
-  rc = product(a->dtype, q, ctx);
-  if (rc != MB_OK) return rc;
-  Product p;
-  p.a[0] = h;
-  p.b[0] = {a->down, a->d, a->f, a->ld_down};
-  p.o[0] = {y, a->tokens, a->d, ldy};
-  p.M = a->tokens; p.N = a->d; p.K = a->f;
-  return product(a->dtype, p, ctx);
+  return forward(a, true, y, ldy, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 MB_API size_t mb_feed_forward_backward_workspace_bytes(int64_t tokens, int64_t d, int64_t f, int32_t from_codes,
@@ -1669,14 +1767,14 @@ MB_API size_t mb_feed_forward_backward_workspace_bytes(int64_t tokens, int64_t d
 MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r, void* workspace,
                                     size_t workspace_bytes, mb_stream_t stream) {
   if (!a || !r) return MB_ERR_ARG;
-  const bool from_codes = r->codes != nullptr, down = a->down != nullptr;
-  int rc = check_args(a, !from_codes, down);
+  const bool from_codes = r->codes != nullptr, with_down = a->down != nullptr;
+  int rc = check_args(a, !from_codes, with_down);
   if (rc != MB_OK) return rc;
   const int64_t T = a->tokens, d = a->d, f = a->f;
   if (r->dx && T > 0) rc = check_mat(r->dx, d, r->lddx);
   if (rc == MB_OK && r->dgate) rc = check_mat(r->dgate, d, r->ld_dgate);
   if (rc == MB_OK && r->dup) rc = check_mat(r->dup, d, r->ld_dup);
-  if (rc == MB_OK && r->ddown) rc = down ? check_mat(r->ddown, f, r->ld_ddown) : MB_ERR_ARG;
+  if (rc == MB_OK && r->ddown) rc = with_down ? check_mat(r->ddown, f, r->ld_ddown) : MB_ERR_ARG;
   if (rc != MB_OK) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   if (T == 0) {  // sums over no tokens
@@ -1686,36 +1784,43 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     return rc;
   }
   if (!r->dx && !r->dgate && !r->dup && !r->ddown) return MB_OK;
-  rc = check_mat(r->dy, down ? d : f, r->lddy);
+  rc = check_mat(r->dy, with_down ? d : f, r->lddy);
   if (rc != MB_OK) return rc;
   if (from_codes && !r->scales) return MB_ERR_ARG;
-  if (!workspace ||
-      workspace_bytes < mb_feed_forward_backward_workspace_bytes(T, d, f, from_codes ? 1 : 0, down ? 1 : 0))
-    return MB_ERR_ARG;
+  const size_t need = mb_feed_forward_backward_workspace_bytes(T, d, f, from_codes ? 1 : 0, with_down ? 1 : 0);
+  if (!workspace || workspace_bytes < need) return MB_ERR_ARG;
   if (!aligned(workspace, 256)) return MB_ERR_ALIGN;
-  uint8_t* ws = static_cast<uint8_t*>(workspace) + kJoinBytes;
-  Ctx ctx = make_ctx(workspace, st);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Padding pad(ws + need, workspace_bytes - need);
+  ws += kJoinBytes;
   const int64_t fp = pad8(f);
   const Mat dg{ws, T, f, fp}, du{ws + area(T, f), T, f, fp};
-  Mat dh{r->dy, T, f, r->lddy}, h;
   ws += 2 * area(T, f);
-  if (down) {
+  const Mat dy = pad.in(r->dy, T, with_down ? d : f, r->lddy);
+  Mat dh = dy, h;
+  if (with_down) {
     h = {ws, T, f, fp};
     dh = {ws + area(T, f), T, f, fp};
     ws += 3 * area(T, f);
   }
-  Mat x{a->x, T, d, a->ldx};
+  const Mat x = from_codes ? Mat{ws, T, d, pad8(d)} : pad.in(a->x, T, d, a->ldx);
+  const Mat gate = pad.in(a->gate, f, d, a->ld_gate), up = pad.in(a->up, f, d, a->ld_up);
+  const Mat down = with_down ? pad.in(a->down, d, f, a->ld_down) : Mat{};
+  const Mat dx = pad.out(r->dx, T, d, r->lddx), dgate = pad.out(r->dgate, f, d, r->ld_dgate);
+  const Mat dup = pad.out(r->dup, f, d, r->ld_dup), ddown = pad.out(r->ddown, d, f, r->ld_ddown);
+  if (pad.status() != MB_OK) return pad.status();
+  rc = pad.before(st);
+  if (rc != MB_OK) return rc;
   if (from_codes) {
-    x = {ws, T, d, pad8(d)};
-    rc = act_unpack(r->codes, r->scales, T, d, ws, a->dtype, pad8(d), st);
+    rc = act_unpack(r->codes, r->scales, T, d, const_cast<void*>(x.p), a->dtype, pad8(d), st);
     if (rc != MB_OK) return rc;
   }
-  const Mat dy{r->dy, T, d, r->lddy};
-  if (down) {
+  Ctx ctx = make_ctx(workspace, st);
+  if (with_down) {
     Product q;
     q.epi = kPlainF32;
     q.a[0] = dy;
-    q.b[0] = {a->down, d, f, a->ld_down};
+    q.b[0] = down;
     q.b_mn = true;
     q.o[0] = dh;
     q.M = T; q.N = f; q.K = d;
@@ -1723,8 +1828,8 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     if (rc != MB_OK) return rc;
   }
   {
-    Product q = gated_product(a, x);
-    q.epi = down ? kGatedBwdF32 : kGatedBwd;
+    Product q = gated_product(a, x, gate, up);
+    q.epi = with_down ? kGatedBwdF32 : kGatedBwd;
     q.dh = dh;
     q.o[0] = dg; q.o[1] = du;
     if (r->ddown) q.o[2] = h;
@@ -1739,10 +1844,9 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     Product q;
     q.nseg = 2;
     q.a[0] = dg; q.a[1] = du;
-    q.b[0] = {a->gate, f, d, a->ld_gate};
-    q.b[1] = {a->up, f, d, a->ld_up};
+    q.b[0] = gate; q.b[1] = up;
     q.b_mn = true;
-    q.o[0] = {r->dx, T, d, r->lddx};
+    q.o[0] = dx;
     q.M = T; q.N = d; q.K = f;
     if (T > kSkinnyTokens) {
       grads[n++] = q;
@@ -1751,19 +1855,20 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
       if (rc != MB_OK) return rc;
     }
   }
-  auto weight = [&](const Mat& left, const Mat& right, void* out, int64_t ld) {  // out = left^T right
-    if (!out) return;
+  auto weight = [&](const Mat& left, const Mat& right, const Mat& out) {  // out = left^T right
+    if (!out.p) return;
     Product& q = grads[n++];
     q.a_mn = q.b_mn = true;
     q.a[0] = left;
     q.b[0] = right;
-    q.o[0] = {out, left.cols, right.cols, ld};
+    q.o[0] = out;
     q.M = left.cols; q.N = right.cols; q.K = T;
   };
-  weight(dg, x, r->dgate, r->ld_dgate);
-  weight(du, x, r->dup, r->ld_dup);
-  weight(dy, h, r->ddown, r->ld_ddown);
-  return products(a->dtype, grads, n, ctx);
+  weight(dg, x, dgate);
+  weight(du, x, dup);
+  weight(dy, h, ddown);
+  rc = products(a->dtype, grads, n, ctx);
+  return rc == MB_OK ? pad.after(st) : rc;
 }
 
 MB_API int mb_ffn_status(void) {

@@ -20,8 +20,9 @@ are the same backward pass for engines that replay stages themselves
 
 Calls run on the current stream of the tensors' device, allocate their outputs
 and workspace from torch's caching allocator and never synchronise, so they can
-be captured in a CUDA graph. Rows whose start is not 16-byte aligned (d or f not
-a multiple of 8, odd views) are copied to padded rows first.
+be captured in a CUDA graph. Matrices whose rows do not start on 16 bytes (d or f
+not a multiple of 8, odd views) are copied to padded rows of the workspace by one
+launch before and, for outputs, one after; transposed and broadcast ones by torch.
 """
 from __future__ import annotations
 
@@ -70,32 +71,21 @@ def _check_weights(gate, up, down, d):
     return f
 
 
-def _pad8(n: int) -> int:
-    return (n + 7) // 8 * 8
-
-
 def _rows(t, rows, cols):
-    """(tensor, address, pitch) of a [rows, cols] tensor with 16-byte aligned rows:
-    itself, or a padded copy."""
-    address = t.data_ptr()
-    if address % 16 == 0:
-        if t.is_contiguous():
-            if cols % 8 == 0:
-                return t, address, cols
-            if rows <= 1:
-                return t, address, _pad8(cols)
-        else:
-            ld, inner = t.stride()
-            if (inner == 1 or cols == 1) and ld % 8 == 0 and ld >= cols:
-                return t, address, ld
-    buf = t.new_empty((rows, _pad8(cols)))
-    buf[:, :cols].copy_(t.detach())
-    return buf, buf.data_ptr(), buf.shape[1]
+    """(tensor, address, pitch) of a [rows, cols] tensor whose rows are contiguous and
+    apart: itself, or a copy. The pitch of a single row is its length."""
+    if t.is_contiguous():
+        return t, t.data_ptr(), cols
+    ld, inner = t.stride()
+    if (inner == 1 or cols == 1) and (ld >= cols or rows <= 1):
+        return t, t.data_ptr(), ld if rows > 1 else cols
+    t = t.detach().contiguous()
+    return t, t.data_ptr(), cols
 
 
-def _out(rows, cols, like):
-    """A buffer for a [rows, cols] output, its rows padded to 16 bytes."""
-    return like.new_empty((rows, _pad8(cols)))
+def _unaligned(*rows):
+    """True if TMA cannot take some (address, pitch): the library then copies."""
+    return any([address % 16 or ld % 8 for address, ld in rows])
 
 
 def _workspace(nbytes, like):
@@ -107,16 +97,12 @@ def _workspace(nbytes, like):
     return ws, ws.data_ptr()
 
 
-def _crop(buf, cols):
-    return buf if cols % 8 == 0 else buf[:, :cols].contiguous()
-
-
 def _two_d(t):
     return t if t.dim() == 2 else t.detach().reshape(-1, t.shape[-1])
 
 
 def _args(code, tokens, d, f, x, gate, up, down):
-    """The C arguments, and the tensors they point into."""
+    """The C arguments, the tensors they point into, and whether some are unaligned."""
     dtype = DTYPES[gate.dtype]
     gate, at_gate, ld_gate = _rows(gate, f, d)
     up, at_up, ld_up = _rows(up, f, d)
@@ -126,7 +112,8 @@ def _args(code, tokens, d, f, x, gate, up, down):
     if down is not None:
         down, at_down, ld_down = _rows(down, d, f)
     return (_lib.FfnArgs(dtype, code, tokens, d, f, at_x, ldx, at_gate, ld_gate, at_up, ld_up, at_down, ld_down),
-            (x, gate, up, down))
+            (x, gate, up, down),
+            d % 8 or f % 8 or _unaligned((at_gate, ld_gate), (at_up, ld_up), (at_x or 0, ldx), (at_down or 0, ld_down)))
 
 
 def _input(x, gate):
@@ -144,19 +131,20 @@ def _forward(x, gate, up, down, code):
         x2 = _two_d(x)
         tokens = x2.shape[0]
         width = f if down is None else d
-        a, keep = _args(code, tokens, d, f, x2, gate, up, down)
-        out = _out(tokens, width, x)
+        a, keep, pad = _args(code, tokens, d, f, x2, gate, up, down)
+        out = x.new_empty((tokens, width))
         L = _lib.lib()
         if down is None:
             name, run, nbytes = "gated_linear", L.mb_gated_linear, L.mb_gated_linear_workspace_bytes(tokens)
         else:
             name, run, nbytes = "feed_forward", L.mb_feed_forward, L.mb_feed_forward_workspace_bytes(tokens, f)
+        if pad:
+            nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
         ws, address = _workspace(nbytes, x)
-        rc = run(ctypes.byref(a), out.data_ptr(), _pad8(width), address, nbytes, stream)
+        rc = run(ctypes.byref(a), out.data_ptr(), width, address, nbytes, stream)
         if rc:
             _lib.check(rc, name)
         del keep, ws
-        out = _crop(out, width)
         return out if x.dim() == 2 else out.view(x.shape[:-1] + (width,))
 
 
@@ -176,25 +164,27 @@ def _backward(grad, saved, gate, up, down, code, needs):
     with _lib.on_device(gate.device) as stream:
         g2 = _two_d(grad)
         tokens = g2.shape[0]
-        a, keep = _args(code, tokens, d, f, None if codes is not None else _two_d(saved), gate, up, down)
+        a, keep, pad = _args(code, tokens, d, f, None if codes is not None else _two_d(saved), gate, up, down)
         r = _lib.FfnGrads()
         if codes is not None:
             r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
         g2, r.dy, r.lddy = _rows(g2, tokens, f if down is None else d)
+        pad = pad or _unaligned((r.dy or 0, r.lddy))
         grads = [None] * len(needs)
         for i, (need, rows, cols) in enumerate(zip(needs, (tokens, f, f, d), (d, d, d, f))):
             if need:
-                grads[i] = buf = _out(rows, cols, gate)
+                grads[i] = buf = gate.new_empty((rows, cols))
                 setattr(r, GRADS[i], buf.data_ptr())
-                setattr(r, PITCHES[i], _pad8(cols))
+                setattr(r, PITCHES[i], cols)
         L = _lib.lib()
         nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, codes is not None, down is not None)
+        if pad:
+            nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
         ws, address = _workspace(nbytes, gate)
         rc = L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), address, nbytes, stream)
         if rc:
             _lib.check(rc, "feed_forward_backward")
         del keep, ws
-        grads = [None if buf is None else _crop(buf, cols) for buf, cols in zip(grads, (d, d, d, f))]
         if grads[0] is not None and like.dim() != 2:
             grads[0] = grads[0].view(like.shape)
         return tuple(grads)

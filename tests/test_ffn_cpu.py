@@ -26,6 +26,9 @@ def test_workspace_sizes():
         m = L.mb_feed_forward_backward_workspace_bytes(tokens, 4096, 11008, 1, 1)
         assert n >= tokens * 11008 * 10 and m - n >= tokens * 4096 * 2
     assert L.mb_feed_forward_backward_workspace_bytes(1 << 31, 1, 1, 0, 0) == 0
+    # x, dy, dx; gate, up, down and their gradients; h
+    assert L.mb_ffn_padding_bytes(5, 33, 65) >= 2 * (3 * 5 * 40 + 5 * 72 + 4 * 65 * 40 + 2 * 33 * 72)
+    assert L.mb_ffn_padding_bytes(0, 33, 65) == 0
 
 
 def _args(**over):
@@ -44,12 +47,14 @@ def _args(**over):
     (dict(x=4098), _lib.MB_ERR_ALIGN), (dict(down=4104), _lib.MB_ERR_ALIGN), (dict(ld_down=88), _lib.MB_ERR_ARG)])
 def test_c_entries_refuse_bad_arguments(over, status):
     L = _lib.lib()
-    a = _args(**over)
-    assert L.mb_feed_forward(ctypes.byref(a), 4096, 64, 4096, 1 << 40, None) == status
+    a = _args(**over)  # workspaces without room for padded copies: unaligned rows are refused
+    need = L.mb_feed_forward_workspace_bytes(4, 96)
+    assert L.mb_feed_forward(ctypes.byref(a), 4096, 64, 4096, need, None) == status
     r = _lib.FfnGrads(dy=4096, lddy=64, dx=4096, lddx=64)
     if "down" not in over and "ld_down" not in over:
-        assert L.mb_gated_linear(ctypes.byref(a), 4096, 96, 4096, 1 << 40, None) == status
-    assert L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), 4096, 1 << 40, None) == status
+        assert L.mb_gated_linear(ctypes.byref(a), 4096, 96, None, 0, None) == status
+    need = L.mb_feed_forward_backward_workspace_bytes(4, 64, 96, 0, 1)
+    assert L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), 4096, need, None) == status
 
 
 def test_c_entries_refuse_bad_outputs_and_workspaces():
@@ -58,8 +63,9 @@ def test_c_entries_refuse_bad_outputs_and_workspaces():
     assert L.mb_feed_forward(None, 4096, 64, 4096, 1 << 40, None) == _lib.MB_ERR_ARG
     assert L.mb_feed_forward(ctypes.byref(a), None, 64, 4096, 1 << 40, None) == _lib.MB_ERR_ARG
     assert L.mb_feed_forward(ctypes.byref(a), 4096, 60, 4096, 1 << 40, None) == _lib.MB_ERR_ARG
-    assert L.mb_feed_forward(ctypes.byref(a), 4096, 68, 4096, 1 << 40, None) == _lib.MB_ERR_ALIGN
     need = L.mb_feed_forward_workspace_bytes(4, 96)
+    assert L.mb_feed_forward(ctypes.byref(a), 4096, 68, 4096, need, None) == _lib.MB_ERR_ALIGN
+    assert L.mb_feed_forward(ctypes.byref(a), 4097, 64, 4096, 1 << 40, None) == _lib.MB_ERR_ALIGN
     assert L.mb_feed_forward(ctypes.byref(a), 4096, 64, None, 1 << 40, None) == _lib.MB_ERR_ARG
     assert L.mb_feed_forward(ctypes.byref(a), 4096, 64, 4096, need - 1, None) == _lib.MB_ERR_ARG
     assert L.mb_feed_forward(ctypes.byref(a), 4096, 64, 4096 + 16, 1 << 40, None) == _lib.MB_ERR_ALIGN
@@ -68,7 +74,8 @@ def test_c_entries_refuse_bad_outputs_and_workspaces():
     assert L.mb_feed_forward_backward(ctypes.byref(a), None, 4096, 1 << 40, None) == _lib.MB_ERR_ARG
     for bad in (dict(dy=None), dict(lddy=56), dict(dx=4100), dict(ld_dgate=1, dgate=4096), dict(codes=4096, scales=None)):
         r = _lib.FfnGrads(**{**dict(dy=4096, lddy=64, dx=4096, lddx=64), **bad})
-        assert L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), 4096, 1 << 40, None) in (
+        need = L.mb_feed_forward_backward_workspace_bytes(4, 64, 96, "codes" in bad, 1)
+        assert L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), 4096, need, None) in (
             _lib.MB_ERR_ARG, _lib.MB_ERR_ALIGN)
     r = _lib.FfnGrads(dy=4096, lddy=96, ddown=4096, ld_ddown=96)  # ddown of a block without down
     b = _args(down=None)
