@@ -190,6 +190,18 @@ def _backward(grad, saved, gate, up, down, code, needs):
         return tuple(grads)
 
 
+def _block_grads(ctx, grad):
+    gate, up, *rest = ctx.saved_tensors
+    down = rest.pop(0) if ctx.has_down else None
+    saved = tuple(rest) if ctx.checkpoint == "fp8" else rest[0]
+    needs = ctx.needs_input_grad[:4 if ctx.has_down else 3]
+    grads = _backward(grad, saved, gate, up, down, ctx.code, needs)
+    return (*grads, None, None) if ctx.has_down else (*grads, None, None, None)
+
+
+_block_grads_once = once_differentiable(_block_grads)
+
+
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, up, down, code, checkpoint):
@@ -200,14 +212,10 @@ class _Block(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        gate, up, *rest = ctx.saved_tensors
-        down = rest.pop(0) if ctx.has_down else None
-        saved = tuple(rest) if ctx.checkpoint == "fp8" else rest[0]
-        needs = ctx.needs_input_grad[:4 if ctx.has_down else 3]
-        grads = _backward(grad, saved, gate, up, down, ctx.code, needs)
-        return (*grads, None, None) if ctx.has_down else (*grads, None, None, None)
+        # the wrapper that refuses a second derivative costs 30 us; only a backward pass
+        # that records a graph (create_graph=True) needs it
+        return _block_grads_once(ctx, grad) if torch.is_grad_enabled() else _block_grads(ctx, grad)
 
 
 def _block(x, gate, up, down, activation, checkpoint):

@@ -183,6 +183,18 @@ def test_autograd_equals_the_functions(cuda, down, checkpoint):
     assert torch.equal(leaves[1].grad, want[1] + want[1])
 
 
+def test_a_second_derivative_is_refused(cuda):
+    from morph_b200 import ffn
+    v = _inputs(10, 64, 96, BF16, cuda)
+    leaves = _leaves(v, "x", "gate", "up", "down")
+    y = ffn.feed_forward(*leaves)
+    plain = torch.autograd.grad(y, leaves, v["grad"], retain_graph=True)
+    grads = torch.autograd.grad(y, leaves, v["grad"], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+    with pytest.raises(RuntimeError):
+        grads[0].float().sum().backward()
+
+
 @pytest.mark.parametrize("needs", [(True, False, False, False), (False, True, False, False), (False, False, True, False),
                                    (False, False, False, True), (False, True, True, True), (True, False, True, True),
                                    (False, False, False, False)])
