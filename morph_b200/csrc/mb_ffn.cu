@@ -14,7 +14,7 @@
 //
 // Two kernels do every product:
 //
-// k_ffn_pair (T > kSkinnyTokens, and all weight gradients): the CTA-pair tcgen05
+// k_ffn_pair (more tokens, and all weight gradients): the CTA-pair tcgen05
 // form of mb_gemm.cu's header (256 x 256 output tile over two SMs, M = 256,
 // TMA-fed ring, two TMEM accumulators so that a tile's epilogue overlaps the next
 // tile's MMAs), with
@@ -23,10 +23,16 @@
 //   * gate and up as the two halves of one tile's B operand: the even CTA loads 128
 //     gate rows, the odd one the same 128 up rows, so a lane's TMEM row holds g in
 //     columns 0-127 and u of the same features in 128-255, and h (or dg, du, h from
-//     the dh tile, which TMA brings in meanwhile) is formed where they lie;
+//     dh, which each lane fetches for its row while the MMAs run) is formed where they
+//     lie;
 //   * dx as one contraction over both (dg, Wg) and (du, Wu): one accumulator;
-//   * dWg and dWu as one launch;
-//   * stores through swizzled shared tiles and TMA, which clips ragged edges.
+//   * dx and the three weight gradients as one launch, dealt so that the pairs end
+//     together (deal_two);
+//   * long contractions in double tiles: 512 x 256, both accumulators, one load of B.
+//     A single tile moves 64 KB of operands per 64-deep k-block into a pair, which at
+//     the ~54 bytes a clock that L2 gives an SM takes 596 cycles against its MMAs' 512;
+//   * eight epilogue warps that hand the accumulator back as soon as they hold it, and
+//     stores through swizzled shared tiles and TMA, which clips ragged edges.
 // Tiles run in groups of 8 row tiles, so that what the ~74 pairs read at one
 // time (about 8 x 9 tiles' operands) stays in L2.
 //
@@ -38,7 +44,7 @@
 // while the SM's TMA loads keep coming: 54.9 us against 49 for 256 tokens, d 4096,
 // f 11008.)
 //
-// k_ffn_skinny (T <= kSkinnyTokens): weights are the MMA's M side (128 rows per CTA:
+// k_ffn_skinny (few tokens, kSkinnyTokens): weights are the MMA's M side (128 rows per CTA:
 // 64 gate and 64 up rows in the gated forms), tokens its N side (16 ..), so each
 // weight is read once and the kernel is a stream over them, bound by HBM. Clusters of
 // 1-8 CTAs split the contraction; their FP32 partials are summed over distributed
@@ -576,6 +582,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 1) {
     if (lane == 0 && leader) {
+      pdl_wait();  // so that its waits' bounds count from here
       const int st = g.st;
       const uint32_t ring0 = smem_u32(ring), stage16 = (uint32_t)g.stage >> 4;
       int s = 0, it = 0;
@@ -1065,6 +1072,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     }
   } else if (warp == 1 && lane == 0) {
     const uint32_t id = idesc(kF16, kAMn, false, 128, g.n);
+    pdl_wait();  // so that its waits' bounds count from here
     int kit = 0;
     for (int k = k_lo; k < k_hi; ++k, ++kit) {
       const int s = kit % g.st;
@@ -1079,6 +1087,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     umma_commit(acc_full);  // also on abort: completion of every MMA issued
   }
   __syncwarp();
+  pdl_wait();  // before the first access to what the kernels before may write or read
   // Every thread waits for the last MMA: then the ring is idle and its memory holds
   // the partials. An aborting CTA takes part in the cluster steps below and stores nothing.
   mbar_wait(acc_full, 0, abort_flag, g.fault.limit_ns);
@@ -1105,7 +1114,6 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
   }
   if (!*abort_flag) {
-    pdl_wait();  // before the first access to what the kernels before may write or read
     // the tile's (token, 4 features) groups, dealt to the cluster's threads; a group's
     // partials are added in rank order
     constexpr int kPer = is_plain(kEpi) ? 32 : 16;
@@ -1237,6 +1245,9 @@ struct Product {
 };
 
 constexpr int kMaxDevices = 64;
+// Longest contraction, in k-blocks (1.3e8 elements): a tile's MMAs then end well inside
+// the 2 s that its epilogue waits for them.
+constexpr int64_t kMaxKb = (int64_t)1 << 21;
 
 struct KernelEntry {
   std::once_flag once[kMaxDevices];
@@ -1297,11 +1308,15 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
 constexpr int kTileKb = 6;
 constexpr int kLongDouble = 4;  // long tiles go in twos while one is at most this part of a pair's share
 constexpr int kMaxPairs = 96;  // pairs a launch may have, for the size of its workspace
-// Tokens up to which the weight-streaming kernel runs.
-constexpr int64_t kSkinnyTokens = 128;
+// Tokens up to which the weight-streaming kernel runs: the gated forms (at d 4096, f
+// 11008 and 100 tokens 45.6 us against the pair kernel's 50.0; from 129 on two of its
+// CTAs share an SM instead of three, and it is behind: d 1200, f 8000, 130 tokens 17.6
+// against 15.8), and the plain ones (160 tokens: 25.5 against 30.0, 11.1 against 11.4 at
+// d 1024, f 2816; 192 tokens at d 2048, f 5504: 27.7 against 15.6).
+constexpr int64_t kSkinnyTokens = 128, kSkinnyTokensPlain = 160;
 constexpr size_t kJoinBytes = (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial * 4;  // one piece a pair
 
-// The workspace's joining part; a call whose products are all skinny has none.
+// The workspace's joining part; a forward call whose products are all skinny has none.
 size_t join_bytes(int64_t tokens) { return tokens <= kSkinnyTokens ? 0 : kJoinBytes; }
 
 // One problem of `tiles` tiles of kb k-blocks over at most `most` pairs: full rounds of
@@ -1437,7 +1452,7 @@ int launch_pair(const Product* qs, int n, Ctx& ctx) {
     const int64_t mt = (q.M + 2 * BM - 1) / (2 * BM), nt = (q.N + cols - 1) / cols;
     tiles += mt * nt;
     if (tiles > ((int64_t)1 << 29)) return MB_ERR_TOO_LARGE;
-    if (q.kblocks() > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+    if (q.kblocks() > kMaxKb) return MB_ERR_TOO_LARGE;
     p.kb = (int)((q.K + BK - 1) / BK);
     p.mt = (int)mt; p.nt = (int)nt;
     const int nb = is_plain(kEpi) ? q.nseg : 2;
@@ -1519,7 +1534,7 @@ int launch_skinny(const Product& q, Ctx& ctx) {
   g.rows = (int)q.N;
   constexpr int kPer = is_plain(kEpi) ? 128 : 64;
   const int64_t kb = (q.K + BK - 1) / BK, tiles = (q.N + kPer - 1) / kPer, KB = kb * q.nseg;
-  if (KB > ((int64_t)1 << 30)) return MB_ERR_TOO_LARGE;
+  if (KB > kMaxKb) return MB_ERR_TOO_LARGE;
   g.kb = (int)kb; g.nseg = q.nseg;
   const int stage = kTileA + g.n * BK * 2, partials = (int)q.M * kSkinnyPitch * 4;  // the ring's memory holds both
   g.tmem_cols = 32;
@@ -1565,7 +1580,7 @@ int launch_skinny(const Product& q, Ctx& ctx) {
 
 template <bool kF16>
 int run_product(const Product& q, Ctx& ctx) {
-  const bool skinny = q.M <= kSkinnyTokens;
+  const bool skinny = q.M <= (is_plain(q.epi) ? kSkinnyTokensPlain : kSkinnyTokens);
   switch (q.epi) {
     case kGated:
       return skinny ? launch_skinny<kGated, false, kF16>(q, ctx) : launch_pair<kGated, false, false, kF16>(&q, 1, ctx);
@@ -1848,7 +1863,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     q.b_mn = true;
     q.o[0] = dx;
     q.M = T; q.N = d; q.K = f;
-    if (T > kSkinnyTokens) {
+    if (T > kSkinnyTokensPlain) {
       grads[n++] = q;
     } else {
       rc = product(a->dtype, q, ctx);

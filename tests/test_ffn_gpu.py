@@ -20,11 +20,12 @@ def _inputs(tokens, d, f, dtype, device, seed=0, grad="dy"):
                 grad=r(tokens, d if grad == "dy" else f, std=0.5))
 
 
-# tokens cross the weight-streaming kernel's paddings (16) and limit (256) and the
-# pair kernel's row tiles (256); widths end inside k-blocks (64), feature tiles
+# tokens cross the weight-streaming kernel's paddings (16) and limits (128, 160) and
+# the pair kernel's row tiles (256); widths end inside k-blocks (64), feature tiles
 # (64, 128) and store chunks (64), and need not be multiples of 8
-SHAPES = [(1, 64, 64), (1, 1024, 2816), (2, 8, 8), (5, 136, 200), (15, 256, 512), (16, 512, 264), (17, 320, 64),
-          (33, 1000, 1111), (64, 256, 1024), (100, 72, 328), (129, 640, 384), (200, 512, 1000), (256, 256, 512),
+SHAPES = [(1, 1, 1), (3, 1, 40), (200, 3, 1), (1, 64, 64), (1, 1024, 2816), (2, 8, 8), (5, 136, 200), (15, 256, 512), (16, 512, 264), (17, 320, 64),
+          (33, 1000, 1111), (64, 256, 1024), (100, 72, 328), (128, 192, 456), (129, 640, 384), (160, 264, 512),
+          (161, 512, 264), (200, 512, 1000), (256, 256, 512),
           (257, 256, 512), (300, 200, 328), (513, 1024, 640), (777, 136, 1096), (1025, 64, 2048), (600, 333, 777)]
 
 
