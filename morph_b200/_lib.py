@@ -200,14 +200,14 @@ def stream_handle(stream=None) -> ctypes.c_void_p:
 
 
 class on_device:
-    """``with on_device(device) as stream``: the device is current inside, and
+    """``with on_device(index) as stream``: that CUDA device is current inside, and
     ``stream`` is the handle of its current stream. Leaves the device alone where
     it is current already (the usual case, at a fraction of the cost of switching)."""
 
     __slots__ = ("index", "before")
 
-    def __init__(self, device):
-        self.index = device.index
+    def __init__(self, index):
+        self.index = index
 
     def __enter__(self):
         from torch import _C

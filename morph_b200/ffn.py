@@ -50,7 +50,7 @@ def _activation_code(activation) -> int:
 def _check(tensor, what, shape, like) -> None:
     if not isinstance(tensor, torch.Tensor) or tensor.shape != shape:
         raise ValueError(f"{what} must be a tensor of shape {list(shape)}")
-    if tensor.dtype != like.dtype or tensor.device != like.device:
+    if tensor.dtype is not like.dtype or tensor.get_device() != like.get_device():
         raise ValueError(f"{what} is {tensor.dtype} on {tensor.device}, expected {like.dtype} on {like.device}")
 
 
@@ -83,11 +83,6 @@ def _rows(t, rows, cols):
     return t, t.data_ptr(), cols
 
 
-def _unaligned(*rows):
-    """True if TMA cannot take some (address, pitch): the library then copies."""
-    return any([address % 16 or ld % 8 for address, ld in rows])
-
-
 def _workspace(nbytes, like):
     """(tensor, address): a buffer from the caching allocator, which a captured
     graph keeps for itself; none for an empty one."""
@@ -102,24 +97,25 @@ def _two_d(t):
 
 
 def _args(code, tokens, d, f, x, gate, up, down):
-    """The C arguments, the tensors they point into, and whether some are unaligned."""
+    """The C arguments, the tensors they point into, and whether TMA cannot take some of
+    their rows (the library then copies them)."""
     dtype = DTYPES[gate.dtype]
     gate, at_gate, ld_gate = _rows(gate, f, d)
     up, at_up, ld_up = _rows(up, f, d)
-    at_x, ldx, at_down, ld_down = None, 0, None, 0
+    at_x, ldx, at_down, ld_down = 0, 0, 0, 0
     if x is not None:
         x, at_x, ldx = _rows(x, tokens, d)
     if down is not None:
         down, at_down, ld_down = _rows(down, d, f)
+    pad = (at_gate | at_up | at_x | at_down) % 16 or (ld_gate | ld_up | ldx | ld_down | d | f) % 8
     return (_lib.FfnArgs(dtype, code, tokens, d, f, at_x, ldx, at_gate, ld_gate, at_up, ld_up, at_down, ld_down),
-            (x, gate, up, down),
-            d % 8 or f % 8 or _unaligned((at_gate, ld_gate), (at_up, ld_up), (at_x or 0, ldx), (at_down or 0, ld_down)))
+            (x, gate, up, down), pad)
 
 
 def _input(x, gate):
     if not isinstance(x, torch.Tensor) or x.dim() == 0:
         raise ValueError("x must be a tensor [..., d]")
-    if not isinstance(gate, torch.Tensor) or x.dtype != gate.dtype or x.device != gate.device:
+    if not isinstance(gate, torch.Tensor) or x.dtype is not gate.dtype or x.get_device() != gate.get_device():
         raise ValueError("x and the weights must have one dtype and one device")
     return x.shape[-1]
 
@@ -127,7 +123,7 @@ def _input(x, gate):
 def _forward(x, gate, up, down, code):
     d = _input(x, gate)
     f = _check_weights(gate, up, down, d)
-    with _lib.on_device(x.device) as stream:
+    with _lib.on_device(x.get_device()) as stream:
         x2 = _two_d(x)
         tokens = x2.shape[0]
         width = f if down is None else d
@@ -156,12 +152,12 @@ def _backward(grad, saved, gate, up, down, code, needs):
         check_activation(codes, scales)
         d, like = codes.shape[-1], codes
     f = _check_weights(gate, up, down, d)
-    if gate.device != like.device:
+    if gate.get_device() != like.get_device():
         raise ValueError("the checkpoint and the weights are on different devices")
     _check(grad, "the output's gradient", like.shape[:-1] + (f if down is None else d,), gate)
     if len(needs) != (3 if down is None else 4):
         raise ValueError("needs names one truth value for x and each weight")
-    with _lib.on_device(gate.device) as stream:
+    with _lib.on_device(gate.get_device()) as stream:
         g2 = _two_d(grad)
         tokens = g2.shape[0]
         a, keep, pad = _args(code, tokens, d, f, None if codes is not None else _two_d(saved), gate, up, down)
@@ -169,7 +165,7 @@ def _backward(grad, saved, gate, up, down, code, needs):
         if codes is not None:
             r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
         g2, r.dy, r.lddy = _rows(g2, tokens, f if down is None else d)
-        pad = pad or _unaligned((r.dy or 0, r.lddy))
+        pad = pad or (r.dy or 0) % 16 or r.lddy % 8
         grads = [None] * len(needs)
         for i, (need, rows, cols) in enumerate(zip(needs, (tokens, f, f, d), (d, d, d, f))):
             if need:

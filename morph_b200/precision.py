@@ -184,7 +184,7 @@ def pack_activation(x: torch.Tensor):
         ld = d
     codes = x.new_empty(shape, dtype=torch.uint8)
     scales = x.new_empty(shape[:-1] + (-(-d // ACTIVATION_BLOCK),), dtype=torch.uint8)
-    with _lib.on_device(x.device) as stream:
+    with _lib.on_device(x.get_device()) as stream:
         _lib.check(_lib.lib().mb_act_pack(flat.data_ptr(), code, rows, d, ld, codes.data_ptr(), scales.data_ptr(),
                                           stream), "pack_activation")
     return codes, scales
@@ -215,7 +215,7 @@ def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfl
         raise ValueError(f"unsupported dtype {dtype}")
     d = codes.shape[-1]
     out = codes.new_empty(codes.shape, dtype=dtype)
-    with _lib.on_device(codes.device) as stream:
+    with _lib.on_device(codes.get_device()) as stream:
         _lib.check(_lib.lib().mb_act_unpack(codes.data_ptr(), scales.data_ptr(), codes.numel() // d, d,
                                             out.data_ptr(), code, d, stream), "unpack_activation")
     return out
