@@ -33,8 +33,10 @@
 //     the ~54 bytes a clock that L2 gives an SM takes 596 cycles against its MMAs' 512;
 //   * eight epilogue warps that hand the accumulator back as soon as they hold it, and
 //     stores through swizzled shared tiles and TMA, which clips ragged edges.
-// Tiles run in groups of 8 row tiles, so that what the ~74 pairs read at one
-// time (about 8 x 9 tiles' operands) stays in L2.
+// Tiles run in groups of 16 row tiles, row tiles fastest, so that what the ~74 pairs
+// read at one time (about 16 x 5 tiles' operands) stays in L2. Large products run at the
+// 1000 W limit, so traffic costs clock: with groups of 8 the sustained forward pass of
+// 8192 tokens (d 4096, f 11008) takes 1682 us against 1613-1650, with 4 1704.
 //
 // Its grid is persistent: whole tiles in turn, and where the last round would leave
 // most pairs idle, that round's tiles are cut along the contraction into equal
@@ -80,7 +82,7 @@ constexpr int kTileA = BM * BK * 2;         // 16 KiB: this CTA's rows of A
 constexpr int kTileB = (BN / 2) * BK * 2;   // 16 KiB: this CTA's half of B
 constexpr int kBox = 64 * 64 * 2;           // 8 KiB: one 64 x 64 MN-major box
 constexpr int kStoreTile = 32 * 64 * 2;     // 4 KiB: a warp's 32 rows x 64 columns
-constexpr int kGroupLog2 = 3;  // row tiles of a group: 8
+constexpr int kGroupLog2 = 4;  // row tiles of a group: 16 (see tile order in the header comment)
 constexpr int kBarBytes = 512;
 constexpr uint32_t kTmemCols = 512;
 
@@ -328,7 +330,7 @@ struct Item {
   int tile, count, prob, bm, bn, k0, k1, piece;
 };
 
-// Tile -> problem and place: groups of 8 row tiles, row tiles fastest inside a
+// Tile -> problem and place: groups of 16 row tiles, row tiles fastest inside a
 // group. False for the tile below an odd number of row tiles.
 __device__ __forceinline__ bool place_tile(const PairArgs& g, Item& it) {
   it.prob = 0;
