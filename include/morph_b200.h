@@ -27,6 +27,12 @@
  *   mb_grad_accumulate
  *       the microbatch accumulation g.float() / loss_scale into the FP32 gradient
  *       window of streamtrain/sparse_disk.py:82-110, with the norm statistics.
+ *   mb_gated_linear / mb_feed_forward / mb_feed_forward_backward
+ *       the SwiGLU block of morph/model/morph_model.py:23-28, whose weights the
+ *       optimizer entries update.
+ *   mb_act_pack / mb_act_unpack
+ *       an 8-bit form of the forward boundaries that streamtrain/engine.py:165-211
+ *       keeps for its replay.
  *   mb_export_f16
  *       the FP16 export cast and range check of streamtrain/export.py:30-35.
  *   mb_cast_f32

@@ -11,7 +11,10 @@ Public drop-ins (same names and behaviour as the reference's interfaces):
   morph_b200.export   the FP16 export writer (export_fp16)
   morph_b200.offload  row state in pinned host memory (OffloadedRowTable, ShardedRowTable)
   morph_b200.zero     one process per GPU: ZeroAdamW, ZeroHybridMuonAdamW
-  morph_b200.precision pack_fp8 / unpack_fp8 (FP8 block transport)
+  morph_b200.precision pack_fp8 / unpack_fp8 (FP8 block transport); pack_activation /
+                      unpack_activation (8-bit activation checkpoints)
+  morph_b200.ffn      the gated feed-forward block (SwiGLU) of morph/model/morph_model.py:23-28,
+                      forward and backward: GatedFeedForward, feed_forward, gated_linear
 
 All compute goes through the C-ABI library libmorph_b200.so (include/morph_b200.h);
 importing a class that needs it raises ImportError when the library is missing.

@@ -25,7 +25,7 @@ def _inputs(tokens, d, f, dtype, device, seed=0, grad="dy"):
 # (64, 128) and store chunks (64), and need not be multiples of 8
 SHAPES = [(1, 1, 1), (3, 1, 40), (200, 3, 1), (1, 64, 64), (1, 1024, 2816), (2, 8, 8), (5, 136, 200), (15, 256, 512), (16, 512, 264), (17, 320, 64),
           (33, 1000, 1111), (64, 256, 1024), (100, 72, 328), (128, 192, 456), (129, 640, 384), (160, 264, 512),
-          (161, 512, 264), (200, 512, 1000), (256, 256, 512),
+          (161, 512, 264), (150, 333, 777), (200, 512, 1000), (256, 256, 512),
           (257, 256, 512), (300, 200, 328), (513, 1024, 640), (777, 136, 1096), (1025, 64, 2048), (600, 333, 777)]
 
 
@@ -88,10 +88,10 @@ def test_gated_linear_backward_from_the_checkpoint(cuda, tokens, d, f, dtype):
 
 
 @pytest.mark.parametrize("tokens,d,f", [(1, 4096, 11008), (128, 2048, 5504), (130, 4096, 11008), (1021, 2048, 5504),
-                                        (2500, 1536, 4096)])
+                                        (2500, 1536, 4096), (2300, 4096, 8192), (2500, 4096, 8200)])
 def test_served_and_trained_sizes(cuda, tokens, d, f):
-    """The sizes of a 7B-shaped block and of a smaller one: every way a launch's last
-    round is cut and joined."""
+    """The sizes of a 7B-shaped block and of smaller ones: every way a launch's last
+    round is cut and joined, and double tiles over odd and even numbers of row tiles."""
     from morph_b200 import ffn
     v = _inputs(tokens, d, f, BF16, cuda)
     args = (v["x"], v["gate"], v["up"], v["down"], "silu")
