@@ -199,28 +199,18 @@ def stream_handle(stream=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(s.cuda_stream)
 
 
-class on_device:
-    """``with on_device(index) as stream``: that CUDA device is current inside, and
-    ``stream`` is the handle of its current stream. Leaves the device alone where
-    it is current already (the usual case, at a fraction of the cost of switching)."""
+_CUDA = None  # torch's current-device and current-stream lookups
 
-    __slots__ = ("index", "before")
 
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
+def raw_stream(index: int):
+    """The handle of CUDA device ``index``'s current stream, or None when another
+    device is current (the caller then switches and comes again): a fraction of the
+    cost of a ``torch.cuda.device`` block around every call."""
+    global _CUDA
+    if _CUDA is None:
         from torch import _C
-        self.before = _C._cuda_getDevice()
-        if self.before != self.index:
-            _C._cuda_setDevice(self.index)
-        return _C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            from torch import _C
-            _C._cuda_setDevice(self.before)
-        return False
+        _CUDA = _C._cuda_getDevice, _C._cuda_getCurrentRawStream
+    return _CUDA[1](index) if _CUDA[0]() == index else None
 
 
 def ptr(t) -> ctypes.c_void_p:

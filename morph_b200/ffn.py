@@ -123,25 +123,29 @@ def _input(x, gate):
 def _forward(x, gate, up, down, code):
     d = _input(x, gate)
     f = _check_weights(gate, up, down, d)
-    with _lib.on_device(x.get_device()) as stream:
-        x2 = _two_d(x)
-        tokens = x2.shape[0]
-        width = f if down is None else d
-        a, keep, pad = _args(code, tokens, d, f, x2, gate, up, down)
-        out = x.new_empty((tokens, width))
-        L = _lib.lib()
-        if down is None:
-            name, run, nbytes = "gated_linear", L.mb_gated_linear, L.mb_gated_linear_workspace_bytes(tokens)
-        else:
-            name, run, nbytes = "feed_forward", L.mb_feed_forward, L.mb_feed_forward_workspace_bytes(tokens, f)
-        if pad:
-            nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
-        ws, address = _workspace(nbytes, x)
-        rc = run(ctypes.byref(a), out.data_ptr(), width, address, nbytes, stream)
-        if rc:
-            _lib.check(rc, name)
-        del keep, ws
-        return out if x.dim() == 2 else out.view(x.shape[:-1] + (width,))
+    index = x.get_device()
+    stream = _lib.raw_stream(index)
+    if stream is None:
+        with torch.cuda.device(index):
+            return _forward(x, gate, up, down, code)
+    x2 = _two_d(x)
+    tokens = x2.shape[0]
+    width = f if down is None else d
+    a, keep, pad = _args(code, tokens, d, f, x2, gate, up, down)
+    out = x.new_empty((tokens, width))
+    L = _lib.lib()
+    if down is None:
+        name, run, nbytes = "gated_linear", L.mb_gated_linear, L.mb_gated_linear_workspace_bytes(tokens)
+    else:
+        name, run, nbytes = "feed_forward", L.mb_feed_forward, L.mb_feed_forward_workspace_bytes(tokens, f)
+    if pad:
+        nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
+    ws, address = _workspace(nbytes, x)
+    rc = run(ctypes.byref(a), out.data_ptr(), width, address, nbytes, stream)
+    if rc:
+        _lib.check(rc, name)
+    del keep, ws
+    return out if x.dim() == 2 else out.view(x.shape[:-1] + (width,))
 
 
 def _backward(grad, saved, gate, up, down, code, needs):
@@ -157,33 +161,37 @@ def _backward(grad, saved, gate, up, down, code, needs):
     _check(grad, "the output's gradient", like.shape[:-1] + (f if down is None else d,), gate)
     if len(needs) != (3 if down is None else 4):
         raise ValueError("needs names one truth value for x and each weight")
-    with _lib.on_device(gate.get_device()) as stream:
-        g2 = _two_d(grad)
-        tokens = g2.shape[0]
-        a, keep, pad = _args(code, tokens, d, f, None if codes is not None else _two_d(saved), gate, up, down)
-        r = _lib.FfnGrads()
-        if codes is not None:
-            r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
-        g2, r.dy, r.lddy = _rows(g2, tokens, f if down is None else d)
-        pad = pad or (r.dy or 0) % 16 or r.lddy % 8
-        grads = [None] * len(needs)
-        for i, (need, rows, cols) in enumerate(zip(needs, (tokens, f, f, d), (d, d, d, f))):
-            if need:
-                grads[i] = buf = gate.new_empty((rows, cols))
-                setattr(r, GRADS[i], buf.data_ptr())
-                setattr(r, PITCHES[i], cols)
-        L = _lib.lib()
-        nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, codes is not None, down is not None)
-        if pad:
-            nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
-        ws, address = _workspace(nbytes, gate)
-        rc = L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), address, nbytes, stream)
-        if rc:
-            _lib.check(rc, "feed_forward_backward")
-        del keep, ws
-        if grads[0] is not None and like.dim() != 2:
-            grads[0] = grads[0].view(like.shape)
-        return tuple(grads)
+    index = gate.get_device()
+    stream = _lib.raw_stream(index)
+    if stream is None:
+        with torch.cuda.device(index):
+            return _backward(grad, saved, gate, up, down, code, needs)
+    g2 = _two_d(grad)
+    tokens = g2.shape[0]
+    a, keep, pad = _args(code, tokens, d, f, None if codes is not None else _two_d(saved), gate, up, down)
+    r = _lib.FfnGrads()
+    if codes is not None:
+        r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
+    g2, r.dy, r.lddy = _rows(g2, tokens, f if down is None else d)
+    pad = pad or (r.dy or 0) % 16 or r.lddy % 8
+    grads = [None] * len(needs)
+    for i, (need, rows, cols) in enumerate(zip(needs, (tokens, f, f, d), (d, d, d, f))):
+        if need:
+            grads[i] = buf = gate.new_empty((rows, cols))
+            setattr(r, GRADS[i], buf.data_ptr())
+            setattr(r, PITCHES[i], cols)
+    L = _lib.lib()
+    nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, codes is not None, down is not None)
+    if pad:
+        nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
+    ws, address = _workspace(nbytes, gate)
+    rc = L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), address, nbytes, stream)
+    if rc:
+        _lib.check(rc, "feed_forward_backward")
+    del keep, ws
+    if grads[0] is not None and like.dim() != 2:
+        grads[0] = grads[0].view(like.shape)
+    return tuple(grads)
 
 
 def _block_grads(ctx, grad):

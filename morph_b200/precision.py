@@ -174,6 +174,11 @@ def pack_activation(x: torch.Tensor):
     shape = x.shape
     if len(shape) == 0 or shape[-1] == 0:
         raise ValueError("pack_activation expects [..., d] with d >= 1")
+    index = x.get_device()
+    stream = _lib.raw_stream(index)
+    if stream is None:
+        with torch.cuda.device(index):
+            return pack_activation(x)
     d = shape[-1]
     flat = x if len(shape) == 2 else x.detach().reshape(-1, d)
     rows = flat.shape[0]
@@ -184,22 +189,22 @@ def pack_activation(x: torch.Tensor):
         ld = d
     codes = x.new_empty(shape, dtype=torch.uint8)
     scales = x.new_empty(shape[:-1] + (-(-d // ACTIVATION_BLOCK),), dtype=torch.uint8)
-    with _lib.on_device(x.get_device()) as stream:
-        _lib.check(_lib.lib().mb_act_pack(flat.data_ptr(), code, rows, d, ld, codes.data_ptr(), scales.data_ptr(),
-                                          stream), "pack_activation")
+    _lib.check(_lib.lib().mb_act_pack(flat.data_ptr(), code, rows, d, ld, codes.data_ptr(), scales.data_ptr(), stream),
+               "pack_activation")
     return codes, scales
 
 
 def check_activation(codes: torch.Tensor, scales: torch.Tensor):
     """Raise ValueError unless (codes, scales) have the layout of ``pack_activation``."""
     for t, what in ((codes, "codes"), (scales, "scales")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or not t.is_contiguous():
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype is not torch.uint8 or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous uint8 on a CUDA device")
-    if codes.dim() == 0 or codes.shape[-1] == 0:
+    shape = codes.shape
+    if len(shape) == 0 or shape[-1] == 0:
         raise ValueError("codes must be [..., d] with d >= 1")
-    if scales.device != codes.device:
+    if scales.get_device() != codes.get_device():
         raise ValueError("codes and scales are on different devices")
-    want = codes.shape[:-1] + (-(-codes.shape[-1] // ACTIVATION_BLOCK),)
+    want = shape[:-1] + (-(-shape[-1] // ACTIVATION_BLOCK),)
     if scales.shape != want:
         raise ValueError(f"scales must be {tuple(want)}, one per {ACTIVATION_BLOCK} features of a row")
 
@@ -213,11 +218,16 @@ def unpack_activation(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfl
     code = _DTYPE_CODES.get(dtype)
     if code is None:
         raise ValueError(f"unsupported dtype {dtype}")
-    d = codes.shape[-1]
-    out = codes.new_empty(codes.shape, dtype=dtype)
-    with _lib.on_device(codes.get_device()) as stream:
-        _lib.check(_lib.lib().mb_act_unpack(codes.data_ptr(), scales.data_ptr(), codes.numel() // d, d,
-                                            out.data_ptr(), code, d, stream), "unpack_activation")
+    index = codes.get_device()
+    stream = _lib.raw_stream(index)
+    if stream is None:
+        with torch.cuda.device(index):
+            return unpack_activation(codes, scales, dtype)
+    shape = codes.shape
+    d = shape[-1]
+    out = codes.new_empty(shape, dtype=dtype)
+    _lib.check(_lib.lib().mb_act_unpack(codes.data_ptr(), scales.data_ptr(), codes.numel() // d, d, out.data_ptr(), code,
+                                        d, stream), "unpack_activation")
     return out
 
 

@@ -122,3 +122,11 @@ def test_module_parameters():
     assert all(fp8_eligible(n) and p.dtype == torch.float32 for n, p in names.items())
     muon, adam = partition(m)
     assert len(muon) == 3 and not adam
+
+
+def test_raw_stream_only_for_the_current_device(monkeypatch):
+    """Another current device gives None: the callers then switch to the tensors' one."""
+    monkeypatch.setattr(_lib, "_CUDA", (lambda: 1, lambda index: 70 + index))
+    assert _lib.raw_stream(1) == 71 and _lib.raw_stream(0) is None
+    monkeypatch.setattr(_lib, "_CUDA", (lambda: 0, lambda index: 0))
+    assert _lib.raw_stream(0) == 0  # the legacy stream's handle
