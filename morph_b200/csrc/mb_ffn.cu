@@ -86,6 +86,10 @@ constexpr int kGroupLog2 = 4;  // row tiles of a group: 16 (see tile order in th
 constexpr int kBarBytes = 512;
 constexpr uint32_t kTmemCols = 512;
 
+template <int N> struct Int {
+  static constexpr int value = N;
+};
+
 // What a product's epilogue does. kPlainF32: FP32 output (dh); kGatedBwd reads a
 // 16-bit dh (the caller's), kGatedBwdF32 an FP32 one.
 enum Epi { kPlain = 0, kGated = 1, kGatedBwd = 2, kPlainF32 = 3, kGatedBwdF32 = 4 };
@@ -111,10 +115,6 @@ struct Div {
   uint32_t m;
   int shift;
   __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
-};
-
-template <int N> struct Int {
-  static constexpr int value = N;
 };
 
 // One problem of a pair launch: an output [M, N] (gated: N features) and up to two K
@@ -237,35 +237,90 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 
 // ------------------------------------------------------------- arithmetic --
 
-// sigma(z) in FP32; exp(-z) of a very negative z is infinite and sigma 0.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// Two FP32 values in a register pair: sm_100 multiplies and adds both at once, which
+// halves the epilogues' arithmetic.
+struct Two {
+  uint64_t v;
+};
+
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ Two two(float x) { return two(x, x); }
+__device__ __forceinline__ void split(Two a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// sigma(z) = 1 / (1 + 2^(-z log2 e)); 2^.. of a very negative z is infinite and sigma 0.
+__device__ __forceinline__ Two sigmoid(Two z) {
+  float x, y;
+  split(z * two(-1.4426950408889634f), x, y);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+  split(two(x, y) + two(1.0f), x, y);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(y));
+  return two(x, y);
+}
 
 constexpr float kGeluC = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float kGeluA = 0.044715f;
 
-// Past |g| = 64 sigma(z) is 0 or 1 to the last bit of FP32; stopping there keeps g^3
-// finite, so that z' times a zero is not a NaN.
-__device__ __forceinline__ float gelu_arg(float g) { return fminf(fmaxf(g, -64.0f), 64.0f); }
-
-__device__ __forceinline__ float act_z(float g, int act) {
-  if (act == MB_ACT_SILU) return g;
-  const float c = gelu_arg(g);
-  return kGeluC * (c + kGeluA * c * c * c);
+// Past |g| = 64 GELU's sigma(z) is 0 or 1 to the last bit of FP32; stopping there keeps
+// g^3 finite, so that z' times a zero is not a NaN.
+__device__ __forceinline__ Two gelu_arg(Two g) {
+  float x, y;
+  split(g, x, y);
+  return two(fminf(fmaxf(x, -64.0f), 64.0f), fminf(fmaxf(y, -64.0f), 64.0f));
 }
 
-__device__ __forceinline__ float gated(float g, float u, int act) {
-  return g * sigmoid(act_z(g, act)) * u;
+template <int kAct>
+__device__ __forceinline__ Two gated(Two g, Two u) {
+  Two z = g;
+  if constexpr (kAct == MB_ACT_GELU_TANH) {
+    const Two c = gelu_arg(g);
+    z = c * fma2(c * c, two(kGeluC * kGeluA), two(kGeluC));
+  }
+  return g * sigmoid(z) * u;
 }
 
-// dg, du and h at one element.
-__device__ __forceinline__ void gated_bwd(float g, float u, float dh, int act, float& dg, float& du, float& h) {
-  const float s = sigmoid(act_z(g, act));
-  const float c = gelu_arg(g);
-  const float zp = act == MB_ACT_SILU ? 1.0f : kGeluC * (1.0f + 3.0f * kGeluA * c * c);
-  const float a = g * s;
+// dg, du and h of two elements.
+template <int kAct>
+__device__ __forceinline__ void gated_bwd(Two g, Two u, Two dh, Two& dg, Two& du, Two& h) {
+  Two z = g, zp;
+  if constexpr (kAct == MB_ACT_GELU_TANH) {
+    const Two c = gelu_arg(g), c2 = c * c;
+    z = c * fma2(c2, two(kGeluC * kGeluA), two(kGeluC));
+    zp = fma2(c2, two(3.0f * kGeluC * kGeluA), two(kGeluC));
+  }
+  const Two s = sigmoid(z), a = g * s;
   h = a * u;
   du = dh * a;
-  dg = dh * u * (s + a * (1.0f - s) * zp);
+  Two slope = fma2(s, two(-1.0f), two(1.0f));  // s + a (1 - s) z'
+  if constexpr (kAct == MB_ACT_GELU_TANH) slope = slope * zp;
+  dg = dh * u * fma2(a, slope, s);
+}
+
+// f(Int<activation>): one copy of a loop for each, with no test inside.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  if (act == MB_ACT_SILU) f(Int<MB_ACT_SILU>{});
+  else f(Int<MB_ACT_GELU_TANH>{});
 }
 
 template <bool kF16>
@@ -277,6 +332,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&t);
   }
+}
+
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack2(Two a) {
+  float x, y;
+  split(a, x, y);
+  return pack2<kF16>(x, y);
 }
 
 // 16-byte chunk `c` (0..7) of row `r` of a 128-byte-swizzled store tile.
@@ -778,8 +840,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             fetch(b, v);
             fetch(b + 2, v + 32);
             if (b == 1) release();
+            with_act(g.act, [&](auto act) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = gated(v[j], v[32 + j], g.act);
+              for (int j = 0; j < 32; j += 2)
+                split(gated<decltype(act)::value>(two(v[j], v[j + 1]), two(v[32 + j], v[33 + j])), v[j], v[j + 1]);
+            });
             put_row<kF16>(out, lane, 4 * b, v);
           }
           fence_async();
@@ -801,25 +866,25 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             if (last) release();
             if (lane == 0) store_wait_read<0>();  // the block before has been read out
             __syncwarp();
+            with_act(g.act, [&](auto act) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {  // 8 features each
-              uint32_t og[4], ou[4], oh[4];
+              for (int k = 0; k < 4; ++k) {  // 8 features each
+                uint32_t og[4], ou[4], oh[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float dg[2], du[2], h[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int j = k * 8 + i * 2 + e;
-                  gated_bwd(v[j], v[32 + j], dh[j], g.act, dg[e], du[e], h[e]);
+                for (int i = 0; i < 4; ++i) {
+                  const int j = k * 8 + i * 2;
+                  Two dg, du, h;
+                  gated_bwd<decltype(act)::value>(two(v[j], v[j + 1]), two(v[32 + j], v[33 + j]), two(dh[j], dh[j + 1]),
+                                                  dg, du, h);
+                  og[i] = pack2<kF16>(dg);
+                  ou[i] = pack2<kF16>(du);
+                  oh[i] = pack2<kF16>(h);
                 }
-                og[i] = pack2<kF16>(dg[0], dg[1]);
-                ou[i] = pack2<kF16>(du[0], du[1]);
-                oh[i] = pack2<kF16>(h[0], h[1]);
+                *block_chunk(tdg, lane, k) = make_uint4(og[0], og[1], og[2], og[3]);
+                *block_chunk(tdu, lane, k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
+                *block_chunk(th, lane, k) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
               }
-              *block_chunk(tdg, lane, k) = make_uint4(og[0], og[1], og[2], og[3]);
-              *block_chunk(tdu, lane, k) = make_uint4(ou[0], ou[1], ou[2], ou[3]);
-              *block_chunk(th, lane, k) = make_uint4(oh[0], oh[1], oh[2], oh[3]);
-            }
+            });
             if (!last) load_dh<kEpi, kF16>(g, row0 + lane, col0 + 32, dh);
             fence_async();
             __syncwarp();
@@ -934,20 +999,33 @@ __global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const __grid_constant
       }
     }
   } else if constexpr (kEpi == kGated) {
+    with_act(g.act, [&](auto act) {
 #pragma unroll
-    for (int c = 0; c < kJoinCols; ++c) v[0][c] = gated(v[0][c], v[1][c], g.act);
+      for (int c = 0; c < kJoinCols; c += 2)
+        split(gated<decltype(act)::value>(two(v[0][c], v[0][c + 1]), two(v[1][c], v[1][c + 1])), v[0][c], v[0][c + 1]);
+    });
     store_cols<kF16>(j.o[0], row * j.ldo[0] + col, n, v[0]);
   } else {
-    float dg[kJoinCols], du[kJoinCols], h[kJoinCols];
+    float dg[kJoinCols], du[kJoinCols], h[kJoinCols], dh[kJoinCols];
 #pragma unroll
     for (int c = 0; c < kJoinCols; ++c) {
-      float dh = 0.0f;
+      dh[c] = 0.0f;
       if (c < n) {
-        if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[row * g.lddh + col + c];
-        else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[row * g.lddh + col + c]);
+        if constexpr (kEpi == kGatedBwdF32) dh[c] = static_cast<const float*>(g.dh)[row * g.lddh + col + c];
+        else dh[c] = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[row * g.lddh + col + c]);
       }
-      gated_bwd(v[0][c], v[1][c], dh, g.act, dg[c], du[c], h[c]);
     }
+    with_act(g.act, [&](auto act) {
+#pragma unroll
+      for (int c = 0; c < kJoinCols; c += 2) {
+        Two a, b, e;
+        gated_bwd<decltype(act)::value>(two(v[0][c], v[0][c + 1]), two(v[1][c], v[1][c + 1]), two(dh[c], dh[c + 1]), a,
+                                        b, e);
+        split(a, dg[c], dg[c + 1]);
+        split(b, du[c], du[c + 1]);
+        split(e, h[c], h[c + 1]);
+      }
+    });
     store_cols<kF16>(j.o[0], row * j.ldo[0] + col, n, dg);
     store_cols<kF16>(j.o[1], row * j.ldo[1] + col, n, du);
     if (g.want_h) store_cols<kF16>(j.o[2], row * j.ldo[2] + col, n, h);
@@ -1146,20 +1224,32 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
         for (int e = 0; e < 4; ++e)
           if (e < n) o[e] = v[e];
       } else if constexpr (kEpi == kGated) {
+        with_act(g.act, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = gated(v[e], w[e], g.act);
+          for (int e = 0; e < 4; e += 2)
+            split(gated<decltype(act)::value>(two(v[e], v[e + 1]), two(w[e], w[e + 1])), v[e], v[e + 1]);
+        });
         store_quad<kF16>(g.o0, tok * g.ldo + col, n, v);
       } else {
-        float dg[4], du[4], h[4];
+        float dg[4], du[4], h[4], dh[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float dh = 0.0f;
+          dh[e] = 0.0f;
           if (e < n) {
-            if constexpr (kEpi == kGatedBwdF32) dh = static_cast<const float*>(g.dh)[tok * g.lddh + col + e];
-            else dh = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col + e]);
+            if constexpr (kEpi == kGatedBwdF32) dh[e] = static_cast<const float*>(g.dh)[tok * g.lddh + col + e];
+            else dh[e] = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col + e]);
           }
-          gated_bwd(v[e], w[e], dh, g.act, dg[e], du[e], h[e]);
         }
+        with_act(g.act, [&](auto act) {
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            Two a, b, c;
+            gated_bwd<decltype(act)::value>(two(v[e], v[e + 1]), two(w[e], w[e + 1]), two(dh[e], dh[e + 1]), a, b, c);
+            split(a, dg[e], dg[e + 1]);
+            split(b, du[e], du[e + 1]);
+            split(c, h[e], h[e + 1]);
+          }
+        });
         store_quad<kF16>(g.o0, tok * g.ldo + col, n, dg);
         store_quad<kF16>(g.o1, tok * g.ldu + col, n, du);
         if (g.o2 != nullptr) store_quad<kF16>(g.o2, tok * g.ldh + col, n, h);
