@@ -1980,6 +1980,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
 
 MB_API int mb_ffn_status(void) {
   int32_t err = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return MB_ERR_CUDA;
   if (cudaMemcpyFromSymbol(&err, g_ffn_err, sizeof(err)) != cudaSuccess) return MB_ERR_CUDA;
   if (err == 0) return MB_OK;
   err = 0;

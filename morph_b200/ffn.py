@@ -20,9 +20,11 @@ are the same backward pass for engines that replay stages themselves
 
 Calls run on the current stream of the tensors' device, allocate their outputs
 and workspace from torch's caching allocator and never synchronise, so they can
-be captured in a CUDA graph. Matrices whose rows do not start on 16 bytes (d or f
-not a multiple of 8, odd views) are copied to padded rows of the workspace by one
-launch before and, for outputs, one after; transposed and broadcast ones by torch.
+be captured in a CUDA graph (a captured autograd backward pass, as with any torch
+operator, must find no eager graph of the same leaves alive). Matrices whose rows
+do not start on 16 bytes (d or f not a multiple of 8, odd views) are copied to
+padded rows of the workspace by one launch before and, for outputs, one after;
+transposed and broadcast ones by torch.
 """
 from __future__ import annotations
 
@@ -269,7 +271,6 @@ def check(device=None) -> None:
     block kernel there gave up a bounded wait since the last check; what it wrote
     is then not valid."""
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
-        torch.cuda.synchronize()  # mb_ffn_status reads behind the default stream only
         _lib.check(_lib.lib().mb_ffn_status(), "feed_forward")
 
 

@@ -378,6 +378,55 @@ def test_streams_graphs_and_overlapping_calls(cuda, tokens):
     ffn.check()
 
 
+def test_a_captured_training_step(cuda):
+    """Forward and backward through autograd in one graph, replayed on other data."""
+    from morph_b200 import ffn
+    from morph_b200.precision import pack_activation
+    names = ("x", "gate", "up", "down")
+    v, w = (_inputs(300, 256, 512, BF16, cuda, seed=s) for s in (5, 6))
+    leaves = _leaves(v, *names)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ffn.feed_forward(*leaves, checkpoint="fp8")
+        grads = torch.autograd.grad(y, leaves, v["grad"])
+    with torch.no_grad():
+        for leaf, n in zip(leaves, names):
+            leaf.copy_(w[n])
+        v["grad"].copy_(w["grad"])
+    graph.replay()
+    assert torch.equal(y, ffn.feed_forward(*(w[n] for n in names)))
+    want = ffn.feed_forward_backward(w["grad"], pack_activation(w["x"]), *(w[n] for n in names[1:]))
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import torch
+from morph_b200 import ffn, precision
+r = lambda *s: torch.randn(*s, device="cuda").bfloat16()
+for tokens in (300, 3):
+    x, gate, up, down, dy = r(tokens, 256), r(512, 256), r(512, 256), r(256, 512), r(tokens, 256)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ffn.feed_forward(x, gate, up, down)
+        grads = ffn.feed_forward_backward(dy, precision.pack_activation(x), gate, up, down)
+    graph.replay()
+    want = ffn.feed_forward_backward(dy, precision.pack_activation(x), gate, up, down)
+    assert torch.equal(y, ffn.feed_forward(x, gate, up, down))
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+print("captured")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured(cuda):
+    import os
+    import subprocess
+    import sys
+    repo = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], cwd=repo, capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr
+
+
 def test_a_thread_without_a_context(cuda):
     """The first CUDA call of a fresh thread may be the block's."""
     import threading
