@@ -1087,6 +1087,27 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   const int k_lo = (int)((int64_t)KB * rank / g.split), k_hi = (int)((int64_t)KB * (rank + 1) / g.split);
   const int feat0 = tile * (is_plain(kEpi) ? 128 : 64);
 
+  const bool withhold = (int)blockIdx.x == g.fault.unit;  // test-only; the MMA thread's wait expires
+  auto load_weights = [&](int s, int k) {
+    const int seg = k >= g.kb ? 1 : 0, k0 = (k - seg * g.kb) * BK;
+    mbar_expect_tx(&full[s], kTileA + tile_b);
+    uint8_t* a = sA + s * kTileA;
+    if constexpr (kAMn) {
+      load_2d(a, &maps.a[seg], &full[s], feat0, k0);
+      load_2d(a + kBox, &maps.a[seg], &full[s], feat0 + 64, k0);
+    } else if constexpr (is_plain(kEpi)) {
+      load_2d(a, &maps.a[seg], &full[s], k0, feat0);
+    } else {  // 64 gate rows, then the same 64 up rows
+      load_2d(a, &maps.a[0], &full[s], k0, feat0);
+      load_2d(a + kBox, &maps.a[1], &full[s], k0, feat0);
+    }
+  };
+  auto load_tokens = [&](int s, int k) {
+    const int seg = k >= g.kb ? 1 : 0;
+    load_2d(sB + s * tile_b, &maps.b[seg], &full[s], (k - seg * g.kb) * BK, 0);
+  };
+  const int head = k_hi - k_lo < g.st ? k_hi - k_lo : g.st;
+
   if (threadIdx.x == 0) {
     for (int s = 0; s < g.st; ++s) {
       mbar_init(&full[s], 1);
@@ -1095,6 +1116,9 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     mbar_init(acc_full, 1);
     *abort_flag = 0;
     mbar_fence_init();
+    // the ring's first round: weights before anything else is set up, tokens when the
+    // kernels before have written them
+    for (int i = withhold ? 1 : 0; i < head; ++i) load_weights(i, k_lo + i);
   }
   if (warp == 2 && lane < 4) prefetch_map(lane < 2 ? &maps.a[lane] : &maps.b[lane - 2]);
   if (warp == 1) {
@@ -1110,28 +1134,6 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   pdl_trigger();
 
   if (warp == 0 && lane == 0) {
-    const bool withhold = (int)blockIdx.x == g.fault.unit;  // test-only; the MMA thread's wait expires
-    auto load_weights = [&](int s, int k) {
-      const int seg = k >= g.kb ? 1 : 0, k0 = (k - seg * g.kb) * BK;
-      mbar_expect_tx(&full[s], kTileA + tile_b);
-      uint8_t* a = sA + s * kTileA;
-      if constexpr (kAMn) {
-        load_2d(a, &maps.a[seg], &full[s], feat0, k0);
-        load_2d(a + kBox, &maps.a[seg], &full[s], feat0 + 64, k0);
-      } else if constexpr (is_plain(kEpi)) {
-        load_2d(a, &maps.a[seg], &full[s], k0, feat0);
-      } else {  // 64 gate rows, then the same 64 up rows
-        load_2d(a, &maps.a[0], &full[s], k0, feat0);
-        load_2d(a + kBox, &maps.a[1], &full[s], k0, feat0);
-      }
-    };
-    auto load_tokens = [&](int s, int k) {
-      const int seg = k >= g.kb ? 1 : 0;
-      load_2d(sB + s * tile_b, &maps.b[seg], &full[s], (k - seg * g.kb) * BK, 0);
-    };
-    // the ring's first round: weights at once, tokens when the kernels before have written them
-    const int head = k_hi - k_lo < g.st ? k_hi - k_lo : g.st;
-    for (int i = withhold ? 1 : 0; i < head; ++i) load_weights(i, k_lo + i);
     pdl_wait();
     int kit = 0;
     for (int k = k_lo; k < k_hi; ++k, ++kit) {
