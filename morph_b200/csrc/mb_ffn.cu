@@ -913,17 +913,23 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 }
 
 // Completes the cut tiles of a pair launch (all of its problem 0): adds each one's pieces in contraction
-// order and runs the product's epilogue. A warp takes 32 rows x 16 columns (features),
-// lane l row l as the pieces were written: it reads whole 512-byte lines, all of a
-// thread's in flight at once, and writes whole sectors.
+// order and runs the product's epilogue. A warp takes 16 rows x 16 columns (features), a
+// lane a row's 8: it reads 256 contiguous bytes of a piece at a time, all of a thread's
+// loads in flight at once, and writes whole sectors. A CTA's warps take different rows
+// of the tile, so that those past the last token are spread evenly.
+// Gated, d 4096, f 11008: 256 tokens 58.0 -> 53.7 us against 32 rows x 16 columns a warp
+// with one piece's loads in flight at a time; f 4736: 28.8 -> 27.
 struct JoinArgs {
   PairArgs g;
   void* o[3];
   int64_t ldo[3];
 };
 
-constexpr int kJoinThreads = 128;
-constexpr int kJoinCols = 16;
+// What an SM has left beside a pair kernel's CTA (registers, 1.5 KB of shared memory) takes
+// one CTA of this many threads, which is there when the pair kernel ends: 0.5 us less
+// than CTAs of 128.
+constexpr int join_threads(int epi) { return epi == kGated ? 384 : is_bwd(epi) ? 192 : 256; }
+constexpr int kJoinCols = 8;
 
 // kJoinCols 16-bit values from element e on, the first n of them (rows are 16-byte
 // aligned and kJoinCols divides e's column).
@@ -932,7 +938,7 @@ __device__ __forceinline__ void store_cols(void* p, int64_t e, int n, const floa
   uint16_t* o = static_cast<uint16_t*>(p) + e;
   if (n == kJoinCols) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < kJoinCols / 8; ++h)
       reinterpret_cast<uint4*>(o)[h] =
           make_uint4(pack2<kF16>(v[8 * h], v[8 * h + 1]), pack2<kF16>(v[8 * h + 2], v[8 * h + 3]),
                      pack2<kF16>(v[8 * h + 4], v[8 * h + 5]), pack2<kF16>(v[8 * h + 6], v[8 * h + 7]));
@@ -943,20 +949,28 @@ __device__ __forceinline__ void store_cols(void* p, int64_t e, int n, const floa
   }
 }
 
+// volatile, so that a thread's loads are all issued before it adds
+__device__ __forceinline__ float4 ld_partial(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+
 template <int kEpi, bool kF16>
-__global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const __grid_constant__ JoinArgs j) {
+__global__ void __launch_bounds__(join_threads(kEpi)) k_ffn_join(const __grid_constant__ JoinArgs j) {
   pdl_trigger();
   const PairArgs& g = j.g;
   const Problem& p0 = g.p[0];
   constexpr int kGroups = (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;  // of a piece's warp
   constexpr int kParts = is_plain(kEpi) ? 1 : 2;                                 // value, or g and u
-  const int lane = threadIdx.x & 31;
-  const int item = (int)(blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5));
-  const int group = item % kGroups, w16 = item / kGroups % (2 * kEpiWarps);
+  const int item = (int)(blockIdx.x * (join_threads(kEpi) / 32) + (threadIdx.x >> 5));
+  const int w16 = item % (2 * kEpiWarps), g0 = item / (2 * kEpiWarps) % kGroups;
+  const int lane = (g0 & 1) * 16 + (threadIdx.x & 15);  // of the pieces' warp: its row
+  const int group = (g0 & ~1) + ((threadIdx.x >> 4) & 1);
   Item it;
   it.tile = item / kGroups / (2 * kEpiWarps);
   it.count = 1;
-  if (!place_tile(g, it)) return;
+  if (it.tile >= g.sched.long_tiles || !place_tile(g, it)) return;
   const int half = (w16 & (kEpiWarps - 1)) >> 2;
   const int64_t row = (int64_t)it.bm * 2 * BM + w16 / kEpiWarps * BM + (w16 & 3) * 32 + lane;
   const int col =
@@ -969,21 +983,31 @@ __global__ void __launch_bounds__(kJoinThreads) k_ffn_join(const __grid_constant
                       group * (kJoinCols / 4) * 32 + lane;
   constexpr int64_t kPiece = (int64_t)2 * kEpiWarps * kWarpPartial / 4;
   float v[kParts][kJoinCols];
+  auto add = [&](auto ways) {
+    float4 x[decltype(ways)::value][kParts][kJoinCols / 4];
 #pragma unroll
-  for (int p = 0; p < kParts; ++p)
+    for (int i = 0; i < decltype(ways)::value; ++i)
 #pragma unroll
-    for (int c = 0; c < kJoinCols; ++c) v[p][c] = 0.0f;
+      for (int p = 0; p < kParts; ++p)
 #pragma unroll
-  for (int i = 0; i < kMaxWays; ++i) {
-    if (i >= g.sched.ways) break;
+        for (int c = 0; c < kJoinCols / 4; ++c)
+          x[i][p][c] = ld_partial(src + i * kPiece + (p * (kFeat / 2) / 4 + c) * 32);
 #pragma unroll
     for (int p = 0; p < kParts; ++p)
 #pragma unroll
       for (int c = 0; c < kJoinCols / 4; ++c) {
-        const float4 x = __ldcg(src + i * kPiece + (p * (kFeat / 2) / 4 + c) * 32);
-        v[p][4 * c] += x.x; v[p][4 * c + 1] += x.y; v[p][4 * c + 2] += x.z; v[p][4 * c + 3] += x.w;
+        float4 t = x[0][p][c];
+#pragma unroll
+        for (int i = 1; i < decltype(ways)::value; ++i) {
+          t.x += x[i][p][c].x; t.y += x[i][p][c].y; t.z += x[i][p][c].z; t.w += x[i][p][c].w;
+        }
+        v[p][4 * c] = t.x; v[p][4 * c + 1] = t.y; v[p][4 * c + 2] = t.z; v[p][4 * c + 3] = t.w;
       }
-  }
+  };
+  static_assert(kMaxWays == 4);
+  if (g.sched.ways == 2) add(std::integral_constant<int, 2>{});
+  else if (g.sched.ways == 3) add(std::integral_constant<int, 3>{});
+  else add(std::integral_constant<int, 4>{});
   if constexpr (kEpi == kPlain) {
     store_cols<kF16>(j.o[0], row * j.ldo[0] + col, n, v[0]);
   } else if constexpr (kEpi == kPlainF32) {
@@ -1599,8 +1623,9 @@ int launch_pair(const Product* qs, int n, Ctx& ctx) {
     j.ldo[i] = q.o[i].ld;
   }
   const int warps = g.sched.long_tiles * 2 * kEpiWarps * (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;
+  constexpr int per = join_threads(kEpi) / 32;
   cudaLaunchAttribute jat[2];
-  cudaLaunchConfig_t join = launch_config(jat, warps / (kJoinThreads / 32), kJoinThreads, 0, 1, &ctx);
+  cudaLaunchConfig_t join = launch_config(jat, (warps + per - 1) / per, 32 * per, 0, 1, &ctx);
   return cudaLaunchKernelEx(&join, k_ffn_join<kEpi, kF16>, j) == cudaSuccess ? MB_OK : MB_ERR_CUDA;
 }
 
