@@ -1213,13 +1213,16 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     for (int j = 0; j < 16; ++j)
       if (c + j < g.tokens) part[(c + j) * kSkinnyPitch + warp * 32 + lane] = __uint_as_float(r[j]);
   }
+  // The columns go back before the cluster barrier: a CTA that held them there while its
+  // peer waits for columns of another stream's kernel, whose own pair waits for these,
+  // would wait for good.
   tc_fence_before();
-  if (g.split > 1) cluster_sync();
-  else __syncthreads();
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
   }
+  if (g.split > 1) cluster_sync();
   if (!*abort_flag) {
     // the tile's (token, 4 features) groups, dealt to the cluster's threads; a group's
     // partials are added in rank order
