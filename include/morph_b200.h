@@ -487,8 +487,11 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* args, const mb_ffn_grads*
                                     size_t workspace_bytes, mb_stream_t stream);
 
 /* Waits for the current device and reports whether a block kernel gave up one of
- * its bounded waits since the last call: MB_ERR_TIMEOUT (its outputs are not
- * valid) or MB_OK. Not for use during stream capture. */
+ * its bounded waits since the last call: MB_ERR_TIMEOUT or MB_OK. Such a kernel
+ * leaves NaN for every result that it does not have, and a call's later kernels
+ * carry them into its outputs, so a caller who never asks sees them too (the
+ * optimizers' gates refuse such gradients). The word is one per device. Not for use
+ * during stream capture. */
 MB_API int mb_ffn_status(void);
 
 #ifdef __cplusplus

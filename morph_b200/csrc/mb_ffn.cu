@@ -57,7 +57,9 @@
 // of the call writes) while the previous one finishes.
 //
 // Waits are bounded as in mb_gemm.cu: on expiry a CTA raises the device's error word
-// (mb_ffn_status), waits (bounded) for its own copies, frees TMEM and returns.
+// (mb_ffn_status), waits (bounded) for its own copies, leaves NaN for the results it
+// does not have, frees TMEM and returns. The NaN pass through the call's later kernels
+// into its outputs, where the gates of the optimizers find them.
 #include <atomic>
 #include <mutex>
 
@@ -516,6 +518,40 @@ __device__ __forceinline__ void load_dh(const PairArgs& g, int64_t row, int col,
   }
 }
 
+// A NaN in either 16-bit type and, as a word, in FP32.
+constexpr uint32_t kNanWord = 0x7fff7fffu;
+
+// What a warp whose wait expired leaves of a tile: NaN in all outputs that it would have
+// written, or in its partial of a cut tile, so that what reads them sees it.
+template <int kEpi>
+__device__ __noinline__ void store_nan(const PairMaps& maps, const PairArgs& g, int prob, float4* partial, uint8_t* out,
+                                       int row0, int col0) {
+  const int lane = threadIdx.x & 31;
+  const uint4 nan = make_uint4(kNanWord, kNanWord, kNanWord, kNanWord);
+  if (partial) {
+    for (int i = 0; i < kWarpPartial / 128; ++i) reinterpret_cast<uint4*>(partial)[i * 32] = nan;
+    return;
+  }
+  const Problem& p = g.p[prob];
+  if (lane == 0) store_wait_read<0>();
+  __syncwarp();
+  for (int i = lane; i < warp_bytes(kEpi) / 16; i += 32) reinterpret_cast<uint4*>(out)[i] = nan;
+  fence_async();
+  __syncwarp();
+  if (lane == 0) {
+    constexpr int kCols = kEpi == kPlainF32 || is_bwd(kEpi) ? 32 : 64;  // of a store's box
+    constexpr int kWide = is_plain(kEpi) ? kWarpCols : kFeat / 2;
+    for (int c = 0; c < kWide && col0 + c < p.N; c += kCols) {
+      store_2d(&maps.m[p.o], out, col0 + c, row0);
+      if constexpr (is_bwd(kEpi)) {
+        store_2d(&maps.m[p.o + 1], out, col0 + c, row0);
+        if (g.want_h) store_2d(&maps.m[p.o + 2], out, col0 + c, row0);
+      }
+    }
+    store_commit();
+  }
+}
+
 // kAnyA: A's layout is each problem's; else K-major. kBMn: B stored [K, N].
 template <int kEpi, bool kAnyA, bool kBMn, bool kF16>
 __global__ void __launch_bounds__(kPairThreads, 1)
@@ -725,6 +761,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint8_t* out = sOut + (warp - 2) * warp_bytes(kEpi);
     int it = 0, ok = 1;
     pdl_wait();
+    // a cut tile's partial of this warp: float4 j of lane l at j * 32 + l
+    auto my_partial = [&](const Item& it) {
+      return reinterpret_cast<float4*>(g.partials) +
+             ((int64_t)(it.tile * g.sched.ways + it.piece) * 2 * kEpiWarps + w16) * (kWarpPartial / 4) + lane;
+    };
     Items work(g.sched, unit);
     int m = 0;
     item.count = 0;
@@ -745,9 +786,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if constexpr (is_bwd(kEpi)) {
         if (in) load_dh<kEpi, kF16>(g, row0 + lane, col0, dh);  // arrives while the MMAs run
       }
-      if (lane == 0) ok = mbar_wait(&acc_full[a], use & 1, abort_flag, g.fault.limit_ns) && !*abort_flag;
+      if (ok && lane == 0) ok = mbar_wait(&acc_full[a], use & 1, abort_flag, g.fault.limit_ns) && !*abort_flag;
       ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok) break;
+      if (!ok) {  // this tile and the unit's others will not come: NaN stands for them
+        if (in) store_nan<kEpi>(maps, g, item.prob, item.piece >= 0 ? my_partial(item) : nullptr, out, row0, col0);
+        continue;
+      }
       tc_fence_after();
       // this warp's accumulator columns: plain 0..127 from here; gated g at 0..63, u at kFeat..
       const uint32_t acc = tmem + (uint32_t)(a * BN) + ((uint32_t)(q * 32) << 16) +
@@ -768,10 +812,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!in) {
         release();
       } else if (item.piece >= 0) {
-        // the piece's partial: float4 j of lane l at j * 32 + l
-        float4* mine = reinterpret_cast<float4*>(g.partials) +
-                       ((int64_t)(item.tile * g.sched.ways + item.piece) * 2 * kEpiWarps + w16) * (kWarpPartial / 4) +
-                       lane;
+        float4* mine = my_partial(item);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
           float v[32];
@@ -1196,7 +1237,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   __syncwarp();
   pdl_wait();  // before the first access to what the kernels before may write or read
   // Every thread waits for the last MMA: then the ring is idle and its memory holds
-  // the partials. An aborting CTA takes part in the cluster steps below and stores nothing.
+  // the partials. An aborting CTA's are NaN, and so is what the cluster makes of them.
   mbar_wait(acc_full, 0, abort_flag, g.fault.limit_ns);
   if (*abort_flag) {
     const uint64_t t0 = globaltimer();
@@ -1206,12 +1247,13 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
   __syncthreads();  // the producer's and the MMA thread's waits have ended too
   tc_fence_after();
   float* part = reinterpret_cast<float*>(smem);
+  const bool lost = *abort_flag;
   for (int c = 0; c < g.tokens; c += 16) {
     uint32_t r[16];
     tmem_ld16(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, r);
 #pragma unroll
     for (int j = 0; j < 16; ++j)
-      if (c + j < g.tokens) part[(c + j) * kSkinnyPitch + warp * 32 + lane] = __uint_as_float(r[j]);
+      if (c + j < g.tokens) part[(c + j) * kSkinnyPitch + warp * 32 + lane] = __uint_as_float(lost ? kNanWord : r[j]);
   }
   // The columns go back before the cluster barrier: a CTA that held them there while its
   // peer waits for columns of another stream's kernel, whose own pair waits for these,
@@ -1223,67 +1265,65 @@ __global__ void __launch_bounds__(kSkinnyThreads) k_ffn_skinny(const __grid_cons
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
   }
   if (g.split > 1) cluster_sync();
-  if (!*abort_flag) {
-    // the tile's (token, 4 features) groups, dealt to the cluster's threads; a group's
-    // partials are added in rank order
-    constexpr int kPer = is_plain(kEpi) ? 32 : 16;
-    const int items = g.tokens * kPer;
-    const uint32_t base = smem_u32(part);
-    for (int i = rank * kSkinnyThreads + (int)threadIdx.x; i < items; i += g.split * kSkinnyThreads) {
-      const int j = i / kPer, f4 = (i % kPer) * 4;
-      const int64_t tok = j, col = feat0 + f4;
-      const int n = g.rows - (feat0 + f4) < 4 ? g.rows - (feat0 + f4) : 4;
-      if (n <= 0) continue;
-      float v[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
-      const uint32_t at = base + (uint32_t)(j * kSkinnyPitch + f4) * 4u;
+  // the tile's (token, 4 features) groups, dealt to the cluster's threads; a group's
+  // partials are added in rank order
+  constexpr int kPer = is_plain(kEpi) ? 32 : 16;
+  const int items = g.tokens * kPer;
+  const uint32_t base = smem_u32(part);
+  for (int i = rank * kSkinnyThreads + (int)threadIdx.x; i < items; i += g.split * kSkinnyThreads) {
+    const int j = i / kPer, f4 = (i % kPer) * 4;
+    const int64_t tok = j, col = feat0 + f4;
+    const int n = g.rows - (feat0 + f4) < 4 ? g.rows - (feat0 + f4) : 4;
+    if (n <= 0) continue;
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, w[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t at = base + (uint32_t)(j * kSkinnyPitch + f4) * 4u;
 #pragma unroll 4
-      for (int r = 0; r < g.split; ++r) {
-        const uint32_t p = g.split > 1 ? mapa_u32(at, (uint32_t)r) : at;
-        const float4 x = ld_cluster_f32x4(p);
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-        if constexpr (!is_plain(kEpi)) {
-          const float4 y = ld_cluster_f32x4(p + 64 * 4);
-          w[0] += y.x; w[1] += y.y; w[2] += y.z; w[3] += y.w;
+    for (int r = 0; r < g.split; ++r) {
+      const uint32_t p = g.split > 1 ? mapa_u32(at, (uint32_t)r) : at;
+      const float4 x = ld_cluster_f32x4(p);
+      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+      if constexpr (!is_plain(kEpi)) {
+        const float4 y = ld_cluster_f32x4(p + 64 * 4);
+        w[0] += y.x; w[1] += y.y; w[2] += y.z; w[3] += y.w;
+      }
+    }
+    if constexpr (kEpi == kPlain) {
+      store_quad<kF16>(g.o0, tok * g.ldo + col, n, v);
+    } else if constexpr (kEpi == kPlainF32) {
+      float* o = static_cast<float*>(g.o0) + tok * g.ldo + col;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < n) o[e] = v[e];
+    } else if constexpr (kEpi == kGated) {
+      with_act(g.act, [&](auto act) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+          split(gated<decltype(act)::value>(two(v[e], v[e + 1]), two(w[e], w[e + 1])), v[e], v[e + 1]);
+      });
+      store_quad<kF16>(g.o0, tok * g.ldo + col, n, v);
+    } else {
+      float dg[4], du[4], h[4], dh[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dh[e] = 0.0f;
+        if (e < n) {
+          if constexpr (kEpi == kGatedBwdF32) dh[e] = static_cast<const float*>(g.dh)[tok * g.lddh + col + e];
+          else dh[e] = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col + e]);
         }
       }
-      if constexpr (kEpi == kPlain) {
-        store_quad<kF16>(g.o0, tok * g.ldo + col, n, v);
-      } else if constexpr (kEpi == kPlainF32) {
-        float* o = static_cast<float*>(g.o0) + tok * g.ldo + col;
+      with_act(g.act, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < n) o[e] = v[e];
-      } else if constexpr (kEpi == kGated) {
-        with_act(g.act, [&](auto act) {
-#pragma unroll
-          for (int e = 0; e < 4; e += 2)
-            split(gated<decltype(act)::value>(two(v[e], v[e + 1]), two(w[e], w[e + 1])), v[e], v[e + 1]);
-        });
-        store_quad<kF16>(g.o0, tok * g.ldo + col, n, v);
-      } else {
-        float dg[4], du[4], h[4], dh[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          dh[e] = 0.0f;
-          if (e < n) {
-            if constexpr (kEpi == kGatedBwdF32) dh[e] = static_cast<const float*>(g.dh)[tok * g.lddh + col + e];
-            else dh[e] = h2f<kF16>(static_cast<const uint16_t*>(g.dh)[tok * g.lddh + col + e]);
-          }
+        for (int e = 0; e < 4; e += 2) {
+          Two a, b, c;
+          gated_bwd<decltype(act)::value>(two(v[e], v[e + 1]), two(w[e], w[e + 1]), two(dh[e], dh[e + 1]), a, b, c);
+          split(a, dg[e], dg[e + 1]);
+          split(b, du[e], du[e + 1]);
+          split(c, h[e], h[e + 1]);
         }
-        with_act(g.act, [&](auto act) {
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            Two a, b, c;
-            gated_bwd<decltype(act)::value>(two(v[e], v[e + 1]), two(w[e], w[e + 1]), two(dh[e], dh[e + 1]), a, b, c);
-            split(a, dg[e], dg[e + 1]);
-            split(b, du[e], du[e + 1]);
-            split(c, h[e], h[e + 1]);
-          }
-        });
-        store_quad<kF16>(g.o0, tok * g.ldo + col, n, dg);
-        store_quad<kF16>(g.o1, tok * g.ldu + col, n, du);
-        if (g.o2 != nullptr) store_quad<kF16>(g.o2, tok * g.ldh + col, n, h);
-      }
+      });
+      store_quad<kF16>(g.o0, tok * g.ldo + col, n, dg);
+      store_quad<kF16>(g.o1, tok * g.ldu + col, n, du);
+      if (g.o2 != nullptr) store_quad<kF16>(g.o2, tok * g.ldh + col, n, h);
     }
   }
   if (g.split > 1) cluster_sync();  // no CTA leaves while a peer reads its partials

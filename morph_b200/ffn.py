@@ -268,8 +268,9 @@ def feed_forward_backward(dy, x, gate, up, down, activation="silu", needs=(True,
 
 def check(device=None) -> None:
     """Wait for ``device`` (default: the current one) and raise TimeoutError if a
-    block kernel there gave up a bounded wait since the last check; what it wrote
-    is then not valid."""
+    block kernel there gave up a bounded wait since the last check. The results that
+    it does not have are NaN, and so are the outputs made from them: an optimizer's
+    finiteness gate refuses such gradients without this call."""
     with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
         _lib.check(_lib.lib().mb_ffn_status(), "feed_forward")
 

@@ -39,3 +39,63 @@ def test_few_tokens_beside_other_tensor_core_kernels(cuda, tokens):
     for out, w in zip(got, want):
         assert all(torch.equal(o, w) for o in out)
     ffn.check()
+
+
+def _stale_memory(like):
+    """Leave blocks of these tensors' sizes in the allocator that hold finite values."""
+    junk = [torch.full_like(t, 7.0) for t in like] * 2
+    del junk
+
+
+# few tokens (split and unsplit contractions), whole tiles, cut tiles with a join, double
+# tiles; the tile or CTA whose load is withheld
+FAULTS = [(0, 1, 512, 1024), (3, 20, 512, 1024), (5, 120, 512, 6000), (0, 300, 512, 1024), (5, 700, 512, 1024),
+          (2, 256, 2048, 5504), (7, 2500, 4096, 4096)]
+
+
+def _assert_right_or_nan(got, want):
+    lost = torch.isnan(got)
+    assert torch.equal(torch.where(lost, want, got), want)
+    return bool(lost.any())
+
+
+@pytest.mark.parametrize("unit,tokens,d,f", FAULTS)
+def test_an_expired_wait_leaves_nan_in_the_outputs(cuda, unit, tokens, d, f):
+    """Every element of a call whose kernel gave up a wait is right or NaN, never what
+    the memory held before."""
+    from morph_b200 import _lib, ffn
+    v = _inputs(tokens, d, f, BF16, cuda)
+    args = [v[n] for n in NAMES]
+    calls = [lambda: (ffn.gated_linear(*args[:3]),), lambda: (ffn.feed_forward(*args),),
+             lambda: ffn.feed_forward_backward(v["grad"], *args)]
+    ffn.check()
+    for call in calls:
+        want = call()
+        _stale_memory(want)
+        _lib.check(_lib.lib().mb_debug_arm_fault(_lib.MB_FAULT_FFN, unit, 5_000_000))
+        got = call()
+        with pytest.raises(TimeoutError):
+            ffn.check()
+        assert any([_assert_right_or_nan(a, b) for a, b in zip(got, want)])
+        assert all(torch.equal(a, b) for a, b in zip(call(), want))
+    ffn.check()
+
+
+def test_an_optimizer_refuses_a_step_after_an_expired_wait(cuda):
+    """Nobody calls ffn.check: the gradients' NaN make the gate refuse the step."""
+    from morph_b200 import HybridMuonAdamW, _lib, ffn
+    torch.manual_seed(1)
+    stage = torch.nn.Module()
+    stage.norm = torch.nn.LayerNorm(256, device=cuda)
+    stage.ffn = ffn.GatedFeedForward(256, 704, device=cuda)
+    x = torch.randn(300, 256, device=cuda)
+    opt = HybridMuonAdamW(stage, lr=1e-3, muon_lr=1e-2)
+    y = stage.ffn(stage.norm(x))
+    _lib.check(_lib.lib().mb_debug_arm_fault(_lib.MB_FAULT_FFN, 0, 5_000_000))
+    y.square().mean().backward()
+    before = {n: p.detach().clone() for n, p in stage.named_parameters()}
+    with pytest.raises(FloatingPointError):
+        opt.step()
+    assert all(torch.equal(before[n], p) for n, p in stage.named_parameters())
+    with pytest.raises(TimeoutError):
+        ffn.check()
