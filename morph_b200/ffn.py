@@ -11,7 +11,8 @@ float16; products accumulate in FP32, and h and the gradients of the two
 projections' outputs are rounded to 16 bits once each, as the next product's
 operand.
 
-Both functions are differentiable. What they keep for the backward pass is the
+Both functions are differentiable, once and in reverse mode (a tensor with a
+forward-mode tangent is refused). What they keep for the backward pass is the
 block's input only, as it is (``checkpoint="x"``) or in 8 bits
 (``checkpoint="fp8"``, ``precision.pack_activation``: 1 + 1/128 bytes per
 element); the projections are recomputed from it. The ``*_backward`` functions
@@ -34,7 +35,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .precision import check_activation, pack_activation
+from .precision import check_activation, pack_activation, refuse_tangents
 
 ACTIVATIONS = {"silu": _lib.MB_ACT_SILU, "gelu_tanh": _lib.MB_ACT_GELU_TANH}
 CHECKPOINTS = ("x", "fp8")
@@ -151,6 +152,7 @@ def _forward(x, gate, up, down, code):
 
 
 def _backward(grad, saved, gate, up, down, code, needs):
+    refuse_tangents(grad, saved, gate, up, down)
     if isinstance(saved, torch.Tensor):
         d, like, codes = _input(saved, gate), saved, None
     else:
@@ -231,6 +233,7 @@ def _block(x, gate, up, down, activation, checkpoint):
     leaves = (x, gate, up) if down is None else (x, gate, up, down)
     if not all([isinstance(t, torch.Tensor) for t in leaves]):
         raise ValueError("x and the weights must be tensors")
+    refuse_tangents(*leaves)
     if torch.is_grad_enabled() and any([t.requires_grad for t in leaves]):
         return _Block.apply(x, gate, up, down, code, checkpoint)
     return _forward(x, gate, up, down, code)

@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -151,6 +152,17 @@ def unpack_fp8(encoded: torch.Tensor, scales: torch.Tensor, dtype=torch.float16,
     return out
 
 
+def refuse_tangents(*tensors) -> None:
+    """Raise NotImplementedError if a tensor carries a forward-mode tangent: a kernel
+    reads its primal alone, and an output without a tangent stands for a derivative of
+    zero."""
+    if forward_ad._current_level < 0:  # no dual_level() is open
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("no forward-mode derivative (torch.autograd.forward_ad)")
+
+
 ACTIVATION_BLOCK = 128  # features per scale of an activation checkpoint
 _DTYPE_CODES = {torch.float32: _lib.MB_F32, torch.float16: _lib.MB_F16, torch.bfloat16: _lib.MB_BF16}
 
@@ -166,6 +178,7 @@ def pack_activation(x: torch.Tensor):
     [..., ceil(d / 128)]. Nonfinite elements become NaN; their neighbours keep
     their values. The relative error of a value within 2^-14 of its block's
     largest is at most 2^-4; smaller ones round at a fixed step of their block."""
+    refuse_tangents(x)
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("pack_activation expects a CUDA tensor")
     code = _DTYPE_CODES.get(x.dtype)
