@@ -99,3 +99,67 @@ def test_an_optimizer_refuses_a_step_after_an_expired_wait(cuda):
     assert all(torch.equal(before[n], p) for n, p in stage.named_parameters())
     with pytest.raises(TimeoutError):
         ffn.check()
+
+
+@pytest.mark.parametrize("param_dtype", [torch.float32, BF16])
+@pytest.mark.parametrize("checkpoint", ["x", "fp8"])
+def test_the_module_keeps_its_parameters_and_its_input_only(cuda, checkpoint, param_dtype):
+    """FP32 masters: no 16-bit copy of a weight lives from the forward to the backward
+    pass, and the gradients are those of the block on the cast weights, bit for bit."""
+    from morph_b200 import ffn
+    from morph_b200.precision import pack_activation
+    d, f, tokens = 512, 1408, 70
+    torch.manual_seed(2)
+    m = ffn.GatedFeedForward(d, f, checkpoint=checkpoint, device=cuda, param_dtype=param_dtype)
+    x = torch.randn(2, tokens // 2, d, device=cuda, requires_grad=True)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (kept.append(t), t)[1], lambda t: t):
+        y = m(x)
+    params = {w.data_ptr() for w in m.parameters()}
+    block = [t for t in kept if t.dtype != torch.float32 or t.data_ptr() in params]
+    assert len(kept) == len(block)  # nothing of the casts around it
+    own = [t for t in block if t.data_ptr() not in params]
+    want = tokens * d * 2 if checkpoint == "x" else tokens * (d + d // 128)
+    assert sum(t.numel() * t.element_size() for t in own) == want
+    del kept, block, own
+    torch.cuda.synchronize()
+    y = m(x)
+    del y
+    base = torch.cuda.memory_allocated()
+    y = m(x)
+    held = torch.cuda.memory_allocated() - base
+    assert held <= want + 2 * y.numel() * 4 + 16384  # the output, and its 16-bit form
+    dy = torch.randn(2, tokens // 2, d, device=cuda)
+    y.backward(dy)
+    weights = [w.weight.detach().to(BF16) for w in (m.gate, m.up, m.down)]
+    x16 = x.detach().to(BF16)
+    saved = pack_activation(x16) if checkpoint == "fp8" else x16
+    dx, *grads = ffn.feed_forward_backward(dy.to(BF16), saved, *weights)
+    assert torch.equal(y, ffn.feed_forward(x16, *weights).float())
+    assert x.grad.dtype == torch.float32 and torch.equal(x.grad, dx.float())
+    for w, g in zip((m.gate, m.up, m.down), grads):
+        assert w.weight.grad.dtype == param_dtype and torch.equal(w.weight.grad, g.to(param_dtype))
+
+
+def test_a_module_with_frozen_parts(cuda):
+    """Only the gradients asked for, with FP32 masters: input alone, one weight alone."""
+    from morph_b200 import ffn
+    torch.manual_seed(4)
+    m = ffn.GatedFeedForward(128, 192, device=cuda)
+    x = torch.randn(30, 128, device=cuda)
+    m(x).sum().backward()
+    full = {n: p.grad.clone() for n, p in m.named_parameters()}
+    for keep in full:
+        for n, p in m.named_parameters():
+            p.grad = None
+            p.requires_grad_(n == keep)
+        m(x).sum().backward()
+        for n, p in m.named_parameters():
+            assert (p.grad is None) == (n != keep)
+        got = dict(m.named_parameters())[keep].grad
+        ref.assert_close(got.to(BF16), full[keep].double(), 1e-5 * full[keep].double().std(), keep)
+    for p in m.parameters():
+        p.requires_grad_(False)
+    x.requires_grad_(True)
+    m(x).sum().backward()
+    assert x.grad.dtype == torch.float32 and torch.isfinite(x.grad).all() and (x.grad != 0).any()
