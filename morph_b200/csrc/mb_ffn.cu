@@ -27,7 +27,7 @@
 //     lie;
 //   * dx as one contraction over both (dg, Wg) and (du, Wu): one accumulator;
 //   * dx and the three weight gradients as one launch, dealt so that the pairs end
-//     together (deal_two);
+//     together (mb_ffn_deal.cuh);
 //   * long contractions in double tiles: 512 x 256, both accumulators, one load of B.
 //     A single tile moves 64 KB of operands per 64-deep k-block into a pair, which at
 //     the ~54 bytes a clock that L2 gives an SM takes 596 cycles against its MMAs' 512;
@@ -65,6 +65,7 @@
 
 #include "mb_async.cuh"
 #include "mb_common.cuh"
+#include "mb_ffn_deal.cuh"
 #include "mb_tc.cuh"
 
 namespace mb {
@@ -84,7 +85,6 @@ constexpr int kTileA = BM * BK * 2;         // 16 KiB: this CTA's rows of A
 constexpr int kTileB = (BN / 2) * BK * 2;   // 16 KiB: this CTA's half of B
 constexpr int kBox = 64 * 64 * 2;           // 8 KiB: one 64 x 64 MN-major box
 constexpr int kStoreTile = 32 * 64 * 2;     // 4 KiB: a warp's 32 rows x 64 columns
-constexpr int kGroupLog2 = 4;  // row tiles of a group: 16 (see tile order in the header comment)
 constexpr int kBarBytes = 512;
 constexpr uint32_t kTmemCols = 512;
 
@@ -109,53 +109,15 @@ constexpr int pair_smem(int epi) {
 static_assert(pair_smem(kPlain) <= 232448 && pair_smem(kGatedBwd) <= 232448, "shared memory of one SM");
 static_assert(warp_bytes(kGatedBwd) % 512 == 0, "swizzled blocks stay aligned");
 
-// Division of 0 <= x < 2^31 by a fixed d >= 1: floor(x m / 2^shift) with
-// m = ceil(2^shift / d), shift = 31 + ceil(log2 d), exact since m d - 2^shift < 2^(shift - 31).
-// The roles of a CTA find their next tile between two k-blocks: the compiler's
-// divisions by run-time values cost more there than a k-block takes.
-struct Div {
-  uint32_t m;
-  int shift;
-  __device__ __forceinline__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * m) >> shift); }
-};
-
-// One problem of a pair launch: an output [M, N] (gated: N features) and up to two K
-// segments accumulated into it. Operands and output name the launch's maps.
-struct Problem {
-  int M, N;
-  int kb, nseg;      // 64-deep blocks of one segment; segments
-  int a_mn;          // A is stored [K, M] (the form that takes either)
-  int a[2], b[2];    // by segment; gated: b by CTA of the pair (gate, up)
-  int o;             // backward: dg, du, h at o, o + 1, o + 2
-  int mt, nt, tile0; // row and column tiles; its first tile's number
-  // groups of rows of tiles (of pairs of them with pairing 2): their number of rows
-  // (log2), the last one's, and the division by a group's tiles and by that last height
-  int group_log2, height, tail_rows;
-  Div by_group, by_tail;
-};
-
-constexpr int kMaxProblems = 4, kMaxMaps = 11;
+constexpr int kMaxMaps = 11;
 
 struct PairMaps {
   CUtensorMap m[kMaxMaps];
 };
 
-// How a launch's tiles are dealt to its units (CTA pairs). With pairing 2 the tiles
-// 2i and 2i + 1 are vertical neighbours, and a unit may take both as one item: they
-// share B's loads. The first long_tiles tiles (all of problem 0) go first: whole, in
-// items of long_step, or each cut into `ways` pieces: n_long items in turn. Of the
-// n_rest items after them (n_double double ones, then single tiles) the first `early`
-// go to the units from `late_units` on, which had one long item less, and the others
-// to all in turn.
-struct Sched {
-  int units, pairing, long_tiles, long_step, ways, n_long, n_rest, n_double, early, late_units;
-};
-
-struct PairArgs {
-  Problem p[kMaxProblems];
-  int nprob, nmaps;
+struct PairArgs : Deal {
+  int nmaps;
   int st, stage;  // ring stages and their bytes: A, B and, with pairing 2, the second tile's A
-  Sched sched;
   float* partials;    // workspace of the pieces of cut tiles
   int act;
   int want_h;       // backward: store h
@@ -373,97 +335,6 @@ __device__ __forceinline__ void store_quad(void* p, int64_t e, int n, const floa
       if (j < n) o[j] = f2h<kF16>(v[j]);
   }
 }
-
-// ------------------------------------------------------------- scheduling --
-
-// Tiles go in twos (one load of B for both: 96 instead of 128 KB of operands) where the
-// contraction is long enough to cover that both epilogues end together, and there are
-// rounds enough: in k-blocks and rounds of tiles. Measured against single tiles: 4096
-// tokens, d 4096, f 11008: gate and up 478 -> 467 us, backward 2000 -> 1945; but the
-// backward of 2048 tokens, d 2048, f 5504 (8 rounds) 285 -> 292, of 1024 tokens, d 4096
-// (16 k-blocks) 549 -> 559. The backward projection's epilogue is too long for it
-// (417 -> 472 thousand cycles).
-constexpr int kTwosKb = 64, kTwosRounds = 2, kTwosKbGrads = 32, kTwosRoundsGrads = 16;
-// When a pair launch cuts its last round: pieces of at least kMinPieceKb k-blocks, at
-// most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time (16 instead of
-// 24: 1021 tokens, d 2048, f 5504, the gated form 41.1 -> 42.4 us, backward 163 -> 169).
-constexpr int kMinPieceKb = 4, kMaxWays = 4, kMinSavedKb = 24;
-
-// One piece of work: k-blocks [k0, k1) of `count` tiles from row tile bm on, column
-// tile bn, of a problem; `piece` of a cut tile, else -1.
-struct Item {
-  int tile, count, prob, bm, bn, k0, k1, piece;
-};
-
-// Tile -> problem and place: groups of 16 row tiles, row tiles fastest inside a
-// group. False for the tile below an odd number of row tiles.
-__device__ __forceinline__ bool place_tile(const PairArgs& g, Item& it) {
-  it.prob = 0;
-  for (int i = 1; i < kMaxProblems; ++i)
-    if (i < g.nprob && it.tile >= g.p[i].tile0) it.prob = i;
-  const Problem& p = g.p[it.prob];
-  const bool twos = g.sched.pairing == 2;
-  const int t = it.tile - p.tile0;
-  const int cell = twos ? t >> 1 : t;
-  const int group = p.by_group(cell), first = group << p.group_log2;
-  const int in = cell - first * p.nt;
-  int row;
-  if (p.height - first >= 1 << p.group_log2) {
-    row = in & ((1 << p.group_log2) - 1);
-    it.bn = in >> p.group_log2;
-  } else {
-    it.bn = p.by_tail(in);
-    row = in - it.bn * p.tail_rows;
-  }
-  row += first;
-  it.bm = twos ? 2 * row + (t & 1) : row;
-  it.k0 = 0;
-  it.k1 = p.kb * p.nseg;
-  it.piece = -1;
-  if (it.bm + it.count > p.mt) it.count = p.mt - it.bm;
-  return it.count > 0;
-}
-
-struct Items {
-  int unit, next_long, next_early, next_rest;
-  __device__ __forceinline__ Items(const Sched& s, int u)
-      : unit(u), next_long(u), next_early(u >= s.late_units ? u - s.late_units : s.early), next_rest(s.early + u) {}
-  __device__ __forceinline__ bool next(const PairArgs& g, Item& it) {
-    const Sched& s = g.sched;
-    while (true) {
-      if (next_long < s.n_long) {
-        int piece = 0;
-        it.tile = next_long * s.long_step;
-        if (s.ways > 1) {
-          it.tile = next_long / s.ways;
-          piece = next_long - it.tile * s.ways;
-        }
-        it.count = s.long_step;
-        next_long += s.units;
-        if (!place_tile(g, it)) continue;
-        if (s.ways > 1) {
-          const int kb = it.k1;
-          it.piece = piece;
-          it.k0 = (int)((int64_t)kb * piece / s.ways);
-          it.k1 = (int)((int64_t)kb * (piece + 1) / s.ways);
-        }
-        return true;
-      }
-      int j;
-      if (next_early < s.early) {
-        j = next_early;
-        next_early += s.units - s.late_units;
-      } else {
-        j = next_rest;
-        if (j >= s.n_rest) return false;
-        next_rest += s.units;
-      }
-      it.count = j < s.n_double ? 2 : 1;
-      it.tile = s.long_tiles + j + (j < s.n_double ? j : s.n_double);
-      if (place_tile(g, it)) return true;
-    }
-  }
-};
 
 // Programmatic dependent launch: let the next kernel of the call set up, and wait
 // for everything the previous ones wrote.
@@ -954,7 +825,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   if (threadIdx.x == 0 && *abort_flag) atomicExch(&g_ffn_err, 1);
 }
 
-// Completes the cut tiles of a pair launch (all of its problem 0): adds each one's pieces in contraction
+// Completes the cut tiles of a pair launch: adds each one's pieces in contraction
 // order and runs the product's epilogue. A warp takes 16 rows x 16 columns (features), a
 // lane a row's 8: it reads 256 contiguous bytes of a piece at a time, all of a thread's
 // loads in flight at once, and writes whole sectors. A CTA's warps take different rows
@@ -963,8 +834,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // with one piece's loads in flight at a time; f 4736: 28.8 -> 27.
 struct JoinArgs {
   PairArgs g;
-  void* o[3];
-  int64_t ldo[3];
+  void* o[kMaxProblems];  // of each problem; of the backward form: dg, du, h
+  int64_t ldo[kMaxProblems];
 };
 
 // What an SM has left beside a pair kernel's CTA (registers, 1.5 KB of shared memory) takes
@@ -1002,7 +873,6 @@ template <int kEpi, bool kF16>
 __global__ void __launch_bounds__(join_threads(kEpi)) k_ffn_join(const __grid_constant__ JoinArgs j) {
   pdl_trigger();
   const PairArgs& g = j.g;
-  const Problem& p0 = g.p[0];
   constexpr int kGroups = (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;  // of a piece's warp
   constexpr int kParts = is_plain(kEpi) ? 1 : 2;                                 // value, or g and u
   const int item = (int)(blockIdx.x * (join_threads(kEpi) / 32) + (threadIdx.x >> 5));
@@ -1013,6 +883,8 @@ __global__ void __launch_bounds__(join_threads(kEpi)) k_ffn_join(const __grid_co
   it.tile = item / kGroups / (2 * kEpiWarps);
   it.count = 1;
   if (it.tile >= g.sched.long_tiles || !place_tile(g, it)) return;
+  const Problem& p0 = g.p[it.prob];
+  const int out = is_plain(kEpi) ? it.prob : 0;
   const int half = (w16 & (kEpiWarps - 1)) >> 2;
   const int64_t row = (int64_t)it.bm * 2 * BM + w16 / kEpiWarps * BM + (w16 & 3) * 32 + lane;
   const int col =
@@ -1051,9 +923,9 @@ __global__ void __launch_bounds__(join_threads(kEpi)) k_ffn_join(const __grid_co
   else if (g.sched.ways == 3) add(std::integral_constant<int, 3>{});
   else add(std::integral_constant<int, 4>{});
   if constexpr (kEpi == kPlain) {
-    store_cols<kF16>(j.o[0], row * j.ldo[0] + col, n, v[0]);
+    store_cols<kF16>(j.o[out], row * j.ldo[out] + col, n, v[0]);
   } else if constexpr (kEpi == kPlainF32) {
-    float* o = static_cast<float*>(j.o[0]) + row * j.ldo[0] + col;
+    float* o = static_cast<float*>(j.o[out]) + row * j.ldo[out] + col;
 #pragma unroll
     for (int c = 0; c < kJoinCols; c += 4) {
       if (c + 4 <= n) {
@@ -1467,9 +1339,6 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
   return cfg;
 }
 
-constexpr int kTileKb = 6;
-constexpr int kLongDouble = 4;  // long tiles go in twos while one is at most this part of a pair's share
-constexpr int kMaxPairs = 96;  // pairs a launch may have, for the size of its workspace
 // Tokens up to which the weight-streaming kernel runs: the gated forms (at d 4096, f
 // 11008 and 100 tokens 45.6 us against the pair kernel's 50.0; from 129 on two of its
 // CTAs share an SM instead of three, and it is behind: d 1200, f 8000, 130 tokens 17.6
@@ -1480,75 +1349,6 @@ constexpr size_t kJoinBytes = (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial *
 
 // The workspace's joining part; a forward call whose products are all skinny has none.
 size_t join_bytes(int64_t tokens) { return tokens <= kSkinnyTokens ? 0 : kJoinBytes; }
-
-// One problem of `tiles` tiles of kb k-blocks over at most `most` pairs: full rounds of
-// whole tiles (double ones with pairing 2), and the last round's tiles cut when that
-// saves enough.
-Sched deal_one(int tiles, int kb, int most, int pairing) {
-  Sched s{};
-  s.units = tiles < most ? tiles : most;
-  s.pairing = pairing;
-  s.long_step = s.ways = 1;
-  int rest = tiles % most;
-  int ways = rest ? most / rest : 1;
-  if (ways > kMaxWays) ways = kMaxWays;
-  if (ways > kb / kMinPieceKb) ways = kb / kMinPieceKb;
-  if (rest && pairing == 2 && (rest & 1)) ++rest;  // what follows starts on a pair
-  if (ways >= 2 && rest * ways <= most && kb - kb / ways >= kMinSavedKb) {
-    s.long_tiles = rest;
-    s.ways = ways;
-    s.n_long = rest * ways;
-    s.units = tiles > most ? most : s.n_long;
-  }
-  const int whole = tiles - s.long_tiles;
-  s.n_double = pairing == 2 ? whole / (2 * most) * most : 0;
-  s.n_rest = whole - s.n_double;
-  return s;
-}
-
-// `first` tiles of long_kb k-blocks and `rest` tiles of kb: the long ones first, cut
-// when one of them is more than a pair's share of the whole, the others so that the
-// pairs end together. A tile costs about kTileKb k-blocks' time beside its own
-// (filling the ring, storing).
-Sched deal_two(int first, int64_t long_kb, int rest, int kb, int most, int pairing) {
-  const int64_t cost = kb + kTileKb;
-  const int64_t share = (first * (long_kb + kTileKb) + rest * cost + most - 1) / most;
-  Sched s{};
-  s.pairing = pairing;
-  s.long_tiles = first;
-  s.ways = s.long_step = 1;
-  if (long_kb > share) {
-    int ways = (int)((long_kb + share - 1) / share);
-    if (ways > kMaxWays) ways = kMaxWays;
-    if (ways > most / first) ways = most / first;
-    if (ways > long_kb / kMinPieceKb) ways = (int)(long_kb / kMinPieceKb);
-    if (ways > 1) s.ways = ways;
-  } else if (pairing == 2 && kLongDouble * long_kb <= share) {
-    s.long_step = 2;
-  }
-  s.n_long = first / s.long_step * s.ways;
-  // double tiles but for about the last two rounds
-  if (pairing == 2 && rest > 4 * most) s.n_double = (rest - 2 * most) / 2;
-  s.n_rest = rest - s.n_double;
-  s.units = s.n_long + s.n_rest < most ? s.n_long + s.n_rest : most;
-  s.late_units = s.n_long % s.units;
-  if (s.late_units > 0) {
-    // items that make up for a long one
-    const int64_t one = s.n_double > 0 ? 2 * cost : cost;
-    const int64_t lead = (s.long_step * long_kb / s.ways + kTileKb + one / 2) / one;
-    const int64_t early = (lead > 0 ? lead : 1) * (s.units - s.late_units);
-    const int most_early = s.n_double > 0 ? s.n_double : rest;
-    s.early = (int)(early < most_early ? early : most_early);
-  }
-  return s;
-}
-
-Div make_div(int64_t d) {
-  int log = 0;
-  while (((int64_t)1 << log) < d) ++log;
-  const int shift = 31 + log;
-  return {(uint32_t)((((uint64_t)1 << shift) + (uint64_t)d - 1) / (uint64_t)d), shift};
-}
 
 // The launch's maps: one for every matrix and box.
 struct MapSet {
@@ -1578,8 +1378,8 @@ struct MapSet {
   }
 };
 
-// `n` products of one kind in one launch; more than one only in the kAnyA form, the
-// first of them the one with the longest contraction, the others' alike.
+// `n` products of one kind in one launch; more than one only in the kAnyA form, by
+// falling contraction.
 template <int kEpi, bool kAnyA, bool kBMn, bool kF16>
 int launch_pair(const Product* qs, int n, Ctx& ctx) {
   auto kernel = &k_ffn_pair<kEpi, kAnyA, kBMn, kF16>;
@@ -1631,30 +1431,15 @@ int launch_pair(const Product* qs, int n, Ctx& ctx) {
   if (!maps.ok) return MB_ERR_CUDA;
   const Product& q = qs[0];
   const int most = entry.pairs[dev];
-  const bool twos = !is_bwd(kEpi) && tiles >= (n > 1 ? kTwosRoundsGrads : kTwosRounds) * most &&
-                    qs[n - 1].kblocks() >= (n > 1 ? kTwosKbGrads : kTwosKb);
-  const int pairing = twos ? 2 : 1;
-  int total = 0, first = 0;
-  for (int i = 0; i < n; ++i) {
-    Problem& p = g.p[i];
-    p.tile0 = total;
-    p.group_log2 = pairing == 2 ? kGroupLog2 - 1 : kGroupLog2;
-    p.height = (p.mt + pairing - 1) / pairing;
-    p.tail_rows = p.height & ((1 << p.group_log2) - 1);
-    p.by_group = make_div(p.nt << p.group_log2);
-    p.by_tail = make_div(p.tail_rows > 0 ? p.tail_rows : 1);
-    total += (g.p[i].mt + pairing - 1) / pairing * pairing * g.p[i].nt;
-    if (i == 0) first = total;
-  }
+  g.nprob = n;
+  deal_tiles(g, !is_bwd(kEpi), most);
+  const int pairing = g.sched.pairing;
   g.stage = pairing * kTileA + kTileB;
   g.st = ring_bytes(kEpi) / g.stage;
-  g.nprob = n;
   g.nmaps = maps.n;
   g.act = q.act; g.want_h = q.o[2].p != nullptr;
   g.dh = q.dh.p; g.lddh = q.dh.ld;
   take_fault(kFaultFfn, &g.fault.unit, &g.fault.limit_ns);
-  g.sched = n == 1 ? deal_one(first, (int)q.kblocks(), most, pairing)
-                   : deal_two(first, q.kblocks(), total - first, (int)qs[1].kblocks(), most, pairing);
   g.partials = ctx.partials;
   cudaLaunchAttribute at[2];
   cudaLaunchConfig_t cfg = launch_config(at, 2 * g.sched.units, kPairThreads, smem, 2, &ctx);
@@ -1662,9 +1447,10 @@ int launch_pair(const Product* qs, int n, Ctx& ctx) {
   ctx.chained = true;
   if (g.sched.ways == 1) return MB_OK;
   JoinArgs j{g, {}, {}};
-  for (int i = 0; i < 3; ++i) {
-    j.o[i] = const_cast<void*>(q.o[i].p);
-    j.ldo[i] = q.o[i].ld;
+  for (int i = 0; i < (n > 1 ? n : 3); ++i) {
+    const Mat& o = n > 1 ? qs[i].o[0] : q.o[i];
+    j.o[i] = const_cast<void*>(o.p);
+    j.ldo[i] = o.ld;
   }
   const int warps = g.sched.long_tiles * 2 * kEpiWarps * (is_plain(kEpi) ? kWarpCols : kFeat / 2) / kJoinCols;
   constexpr int per = join_threads(kEpi) / 32;
@@ -2014,25 +1800,26 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     rc = product(a->dtype, q, ctx);
     if (rc != MB_OK) return rc;
   }
-  // dx and the weight gradients need each other's results for nothing: one launch (a
-  // few tokens' dx is a stream over the weights, for the skinny kernel)
+  // dx and the weight gradients need each other's results for nothing: one launch, by
+  // falling contraction (a few tokens' dx is a stream over the weights, for the skinny
+  // kernel)
   Product grads[kMaxProblems];
   int n = 0;
+  Product q;
   if (r->dx) {
-    Product q;
     q.nseg = 2;
     q.a[0] = dg; q.a[1] = du;
     q.b[0] = gate; q.b[1] = up;
     q.b_mn = true;
     q.o[0] = dx;
     q.M = T; q.N = d; q.K = f;
-    if (T > kSkinnyTokensPlain) {
-      grads[n++] = q;
-    } else {
+    if (T <= kSkinnyTokensPlain) {
       rc = product(a->dtype, q, ctx);
       if (rc != MB_OK) return rc;
     }
   }
+  const bool dx_here = r->dx && T > kSkinnyTokensPlain, dx_last = q.kblocks() < (T + BK - 1) / BK;
+  if (dx_here && !dx_last) grads[n++] = q;
   auto weight = [&](const Mat& left, const Mat& right, const Mat& out) {  // out = left^T right
     if (!out.p) return;
     Product& q = grads[n++];
@@ -2045,6 +1832,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
   weight(dg, x, dgate);
   weight(du, x, dup);
   weight(dy, h, ddown);
+  if (dx_here && dx_last) grads[n++] = q;
   rc = products(a->dtype, grads, n, ctx);
   return rc == MB_OK ? pad.after(st) : rc;
 }

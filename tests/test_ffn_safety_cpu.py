@@ -1,5 +1,10 @@
 """The feed-forward block and the activation checkpoints on a host without a GPU: what
 they refuse, what they ask for, and how their launches are dealt."""
+import math
+import os
+import random
+import subprocess
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -8,6 +13,7 @@ from morph_b200 import ffn
 from morph_b200.precision import pack_activation
 
 BF16 = torch.bfloat16
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.mark.parametrize("grad_mode", [True, False])
@@ -38,3 +44,61 @@ def test_forward_mode_tangents_are_refused(which, grad_mode):
     with forward_ad.dual_level():  # without a tangent: the usual checks
         with pytest.raises(ValueError):
             pack_activation(torch.zeros(3, 64, dtype=BF16))
+
+
+def _launch(tokens, d, f, dx=True, weights=3, pairs=74):
+    """The problems of a backward pass's last launch, as mb_feed_forward_backward orders
+    them: (mt, nt, kb, nseg) by falling contraction."""
+    t = lambda n, size: -(-n // size)  # noqa: E731
+    w = [(t(f, 256), t(d, 256), t(tokens, 64), 1)] * min(weights, 2)
+    w += [(t(d, 256), t(f, 256), t(tokens, 64), 1)] * (weights > 2)
+    x = [(t(tokens, 256), t(d, 256), t(f, 64), 2)] if dx else []
+    problems = w + x if x and 2 * t(f, 64) < t(tokens, 64) else x + w
+    return " ".join(str(n) for n in [1, pairs, len(problems), *(n for p in problems for n in p)])
+
+
+@pytest.fixture(scope="module")
+def replay(tmp_path_factory):
+    exe = str(tmp_path_factory.mktemp("deal") / "ffn_deal")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-x", "c++", "-I", os.path.join(REPO, "morph_b200", "csrc"),
+                    os.path.join(REPO, "tests", "c", "ffn_deal.cpp"), "-o", exe], check=True)
+
+    def run(lines):
+        out = subprocess.run([exe], input="\n".join(lines), capture_output=True, text=True, check=True).stdout
+        return [tuple(int(n) for n in line.split()) for line in out.splitlines()]
+    return run
+
+
+def test_every_tile_is_dealt_once(replay):
+    """Random launches of one to four problems, single and double tiles, few and many
+    pairs: each k-block of each tile once, pieces inside the workspace."""
+    rng = random.Random(5)
+    log = lambda lo, hi: int(math.exp(rng.uniform(math.log(lo), math.log(hi + 1))))  # noqa: E731
+    lines = []
+    for _ in range(1500):
+        lines.append(_launch(log(161, 60000), log(1, 9000), log(1, 12000), rng.random() < 0.7, rng.choice([1, 2, 3, 3, 3]),
+                             rng.choice([1, 2, 30, 66, 72, 73, 74, 74, 96])))
+        lines.append(f"{rng.randrange(2)} {rng.choice([7, 70, 74, 96])} 1 {log(1, 200)} {log(1, 100)} {log(1, 600)} "
+                     f"{rng.choice([1, 2])}")
+    got = replay(lines)
+    assert len(got) == len(lines)
+    bad = [line for line, (ok, *_) in zip(lines, got) if not ok]
+    assert not bad, bad[:3]
+
+
+@pytest.mark.parametrize("tokens,d,f,dx,most", [
+    (8192, 512, 1024, True, 1.5), (8192, 512, 1024, False, 1.5), (32768, 512, 2048, True, 1.1),
+    # 48 tiles of 512 k-blocks: two pieces of each would be 96, more than the 74 pairs, so
+    # one pair has 512 + 6 against a share of 48 (512 + 6) / 74 = 336: 1.54
+    (32768, 512, 2048, False, 1.55),
+    # 6 tiles of 256 k-blocks in at most 4 pieces, 256 / 4 + 6 = 70, and 64 tiles of 16:
+    # a share of (24 (64 + 6) + 64 (16 + 6)) / 74 = 41.7: 1.68
+    (16384, 256, 512, True, 1.68), (65536, 1024, 1024, True, 1.1),
+    (4096, 4096, 11008, True, 1.1), (2048, 2048, 5504, True, 1.2)])
+def test_narrow_blocks_with_many_tokens_are_dealt_evenly(replay, tokens, d, f, dx, most):
+    """Past 2 f tokens the weight gradients have the longer contraction: they go first,
+    all three are cut where a tile is more than a pair's share, and the busiest pair ends
+    within `most` of the even share (8192 tokens, d 512, f 1024, dealt with dx first: 2.2
+    times, without dx 3.0)."""
+    [(ok, busiest, share, _)] = replay([_launch(tokens, d, f, dx)])
+    assert ok and busiest <= most * share, (busiest, share)

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import _ffn_ref as ref
-from test_ffn_gpu import _inputs
+from test_ffn_gpu import _assert_same_sum, _check_grads, _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -163,3 +163,22 @@ def test_a_module_with_frozen_parts(cuda):
     x.requires_grad_(True)
     m(x).sum().backward()
     assert x.grad.dtype == torch.float32 and torch.isfinite(x.grad).all() and (x.grad != 0).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("tokens,d,f", [(8192, 512, 1024), (5000, 136, 200), (3000, 264, 88), (9000, 72, 1111), (16384, 256, 512)])
+def test_narrow_blocks_with_many_tokens(cuda, tokens, d, f, dtype):
+    """More tokens than 2 f: the weight gradients have the longest contraction, and the
+    pieces of all three are joined into their own outputs."""
+    from morph_b200 import ffn
+    v = _inputs(tokens, d, f, dtype, cuda)
+    args = [v[n] for n in NAMES]
+    got = ffn.feed_forward_backward(v["grad"], *args)
+    want, sigmas = ref.backward(v["grad"], *args, "silu")
+    _check_grads(got, want, sigmas, dtype, ("dx", "dgate", "dup", "ddown"))
+    for needs in ((False, True, True, True), (True, False, True, False), (False, False, True, True), (True, False, False, True)):
+        for need, a, b in zip(needs, got, ffn.feed_forward_backward(v["grad"], *args, needs=needs)):
+            assert (b is None) == (not need)
+            if need:
+                _assert_same_sum(b, a)
+    ffn.check()
