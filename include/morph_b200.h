@@ -431,8 +431,11 @@ MB_API int mb_act_unpack(const uint8_t* codes, const uint8_t* scales, int64_t ro
  * MB_F16), row-major with row pitches ld (elements). Products accumulate in FP32;
  * h and the gradients of x gate^T and x up^T are rounded to `dtype` once each, as
  * the next product's operand. Matrices whose rows do not start on 16 bytes (base,
- * or a pitch that is no multiple of 8) are copied through the workspace, which then
- * has to be mb_ffn_padding_bytes larger (else MB_ERR_ALIGN). */
+ * or, with more than one row, a pitch that is no multiple of 8) are copied through the
+ * workspace, which then has to be larger (else MB_ERR_ALIGN): by rows * 2 * (columns
+ * rounded up to 8) bytes, rounded up to 256, for each such matrix of the call, inputs
+ * and outputs; mb_ffn_padding_bytes is enough for any call. Outputs overlap neither
+ * inputs nor one another. */
 typedef struct mb_ffn_args {
   int32_t dtype;
   int32_t activation; /* MB_ACT_* */

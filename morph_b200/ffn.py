@@ -99,9 +99,15 @@ def _two_d(t):
     return t if t.dim() == 2 else t.detach().reshape(-1, t.shape[-1])
 
 
+def _padding(*mats):
+    """Workspace bytes for the padded copies that the library makes of the matrices
+    (address, pitch, rows, columns) whose rows TMA cannot take (Padding of mb_ffn.cu)."""
+    return sum((rows * (-(-cols // 8) * 8) * 2 + 255) // 256 * 256 for at, ld, rows, cols in mats
+               if at and rows and (at % 16 or rows > 1 and ld % 8))
+
+
 def _args(code, tokens, d, f, x, gate, up, down):
-    """The C arguments, the tensors they point into, and whether TMA cannot take some of
-    their rows (the library then copies them)."""
+    """The C arguments, the tensors they point into, and the workspace for copies of them."""
     dtype = DTYPES[gate.dtype]
     gate, at_gate, ld_gate = _rows(gate, f, d)
     up, at_up, ld_up = _rows(up, f, d)
@@ -110,7 +116,9 @@ def _args(code, tokens, d, f, x, gate, up, down):
         x, at_x, ldx = _rows(x, tokens, d)
     if down is not None:
         down, at_down, ld_down = _rows(down, d, f)
-    pad = (at_gate | at_up | at_x | at_down) % 16 or (ld_gate | ld_up | ldx | ld_down | d | f) % 8
+    pad = 0
+    if (at_gate | at_up | at_x | at_down) % 16 or (ld_gate | ld_up | ldx | ld_down) % 8:
+        pad = _padding((at_x, ldx, tokens, d), (at_gate, ld_gate, f, d), (at_up, ld_up, f, d), (at_down, ld_down, d, f))
     return (_lib.FfnArgs(dtype, code, tokens, d, f, at_x, ldx, at_gate, ld_gate, at_up, ld_up, at_down, ld_down),
             (x, gate, up, down), pad)
 
@@ -141,8 +149,9 @@ def _forward(x, gate, up, down, code):
         name, run, nbytes = "gated_linear", L.mb_gated_linear, L.mb_gated_linear_workspace_bytes(tokens)
     else:
         name, run, nbytes = "feed_forward", L.mb_feed_forward, L.mb_feed_forward_workspace_bytes(tokens, f)
-    if pad:
-        nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
+    if width % 8:
+        pad += _padding((out.data_ptr(), width, tokens, width))
+    nbytes += pad
     ws, address = _workspace(nbytes, x)
     rc = run(ctypes.byref(a), out.data_ptr(), width, address, nbytes, stream)
     if rc:
@@ -177,17 +186,19 @@ def _backward(grad, saved, gate, up, down, code, needs):
     if codes is not None:
         r.codes, r.scales = codes.data_ptr(), scales.data_ptr()
     g2, r.dy, r.lddy = _rows(g2, tokens, f if down is None else d)
-    pad = pad or (r.dy or 0) % 16 or r.lddy % 8
+    mats = [(r.dy or 0, r.lddy, *g2.shape)]  # beside those of _args
     grads = [None] * len(needs)
     for i, (need, rows, cols) in enumerate(zip(needs, (tokens, f, f, d), (d, d, d, f))):
         if need:
             grads[i] = buf = gate.new_empty((rows, cols))
             setattr(r, GRADS[i], buf.data_ptr())
             setattr(r, PITCHES[i], cols)
+            mats.append((buf.data_ptr(), cols, rows, cols))
     L = _lib.lib()
     nbytes = L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, codes is not None, down is not None)
-    if pad:
-        nbytes += L.mb_ffn_padding_bytes(tokens, d, f)
+    if (d | f | r.lddy) % 8 or (r.dy or 0) % 16:
+        pad += _padding(*mats)
+    nbytes += pad
     ws, address = _workspace(nbytes, gate)
     rc = L.mb_feed_forward_backward(ctypes.byref(a), ctypes.byref(r), address, nbytes, stream)
     if rc:

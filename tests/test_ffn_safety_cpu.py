@@ -102,3 +102,34 @@ def test_narrow_blocks_with_many_tokens_are_dealt_evenly(replay, tokens, d, f, d
     times, without dx 3.0)."""
     [(ok, busiest, share, _)] = replay([_launch(tokens, d, f, dx)])
     assert ok and busiest <= most * share, (busiest, share)
+
+
+def _aligned(rows, cols, pitch=None, offset=0):
+    """A 16-bit view whose storage starts on 16 bytes, `offset` elements in."""
+    pitch = pitch or cols
+    buf = torch.zeros(rows * pitch + offset + 16, dtype=BF16)
+    skip = (-buf.data_ptr() % 16) // 2
+    return buf[skip + offset:][:rows * pitch].view(rows, pitch)[:, :cols]
+
+
+def test_only_unaligned_matrices_ask_for_room():
+    """The workspace grows by the copies that the call makes, not by those of every
+    matrix that a call may have."""
+    tokens, d, f = 5, 64, 96
+    area = lambda rows, cols: -(-rows * (-(-cols // 8) * 8) * 2 // 256) * 256  # noqa: E731
+    good = [(tokens, d), (f, d), (f, d), (d, f)]
+
+    def room(mats):
+        return ffn._args(0, tokens, d, f, *mats)[2]
+    assert room([_aligned(*s) for s in good]) == 0
+    assert room([_aligned(*s, pitch=s[1] + 8) for s in good]) == 0
+    for i, s in enumerate(good):
+        for bad in (dict(offset=1), dict(pitch=s[1] + 3), dict(pitch=s[1] + 8, offset=4)):
+            mats = [_aligned(*t, **(bad if i == j else {})) for j, t in enumerate(good)]
+            assert room(mats) == area(*s)
+    assert room([_aligned(*s, offset=1) for s in good]) == sum(area(*s) for s in good)
+    # a single row has no pitch
+    assert ffn._padding((4096, 67, 1, 67)) == 0 and ffn._padding((4098, 67, 1, 67)) == area(1, 67)
+    assert ffn._padding((0, 67, 0, 67)) == 0
+    odd = _aligned(f, 65), _aligned(f, 65)
+    assert ffn._args(0, tokens, 65, f, _aligned(tokens, 65), *odd, _aligned(65, f))[2] == area(tokens, 65) + 2 * area(f, 65)

@@ -182,3 +182,27 @@ def test_narrow_blocks_with_many_tokens(cuda, tokens, d, f, dtype):
             if need:
                 _assert_same_sum(b, a)
     ffn.check()
+
+
+@pytest.mark.parametrize("tokens,d,f", [(3, 4096, 8192), (300, 1024, 2048)])
+def test_one_unaligned_view_costs_its_own_copy(cuda, tokens, d, f):
+    """An x one element off 16 bytes among large aligned weights: the call's peak memory
+    is its outputs, its workspace and a copy of x."""
+    from morph_b200 import _lib, ffn
+    v = _inputs(tokens, d, f, BF16, cuda)
+    args = [v[n] for n in NAMES]
+    buf = torch.empty(tokens * d + 1, dtype=BF16, device=cuda)
+    x = buf[1:].view(tokens, d)
+    x.copy_(v["x"])
+    L = _lib.lib()
+    for call, out, ws in (
+            (lambda x: (ffn.feed_forward(x, *args[1:]),), tokens * d, L.mb_feed_forward_workspace_bytes(tokens, f)),
+            (lambda x: ffn.feed_forward_backward(v["grad"], x, *args[1:]), tokens * d + 3 * d * f,
+             L.mb_feed_forward_backward_workspace_bytes(tokens, d, f, 0, 1))):
+        want = call(v["x"])
+        base = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        got = call(x)
+        peak = torch.cuda.max_memory_allocated() - base
+        assert peak <= 2 * out + ws + 2 * tokens * d + (2 << 20) * 6, (peak, out, ws)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
