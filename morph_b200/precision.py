@@ -176,8 +176,9 @@ def pack_activation(x: torch.Tensor):
     ``(codes, scales)``, both uint8: E4M3FN codes of x's shape, and the biased
     exponent (s + 127) of one power-of-two scale per 128 features of a row,
     [..., ceil(d / 128)]. Nonfinite elements become NaN; their neighbours keep
-    their values. The relative error of a value within 2^-14 of its block's
-    largest is at most 2^-4; smaller ones round at a fixed step of their block."""
+    their values. The relative error of a value within 2^-13 of its block's
+    largest is at most 2^-4 (a block whose largest is below 2^-119 excepted: no scale
+    is smaller than 2^-127); smaller ones round at a fixed step of their block."""
     refuse_tangents(x)
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("pack_activation expects a CUDA tensor")
