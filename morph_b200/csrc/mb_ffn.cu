@@ -35,8 +35,11 @@
 //     stores through swizzled shared tiles and TMA, which clips ragged edges.
 // Tiles run in groups of 16 row tiles, row tiles fastest, so that what the ~74 pairs
 // read at one time (about 16 x 5 tiles' operands) stays in L2. Large products run at the
-// 1000 W limit, so traffic costs clock: with groups of 8 the sustained forward pass of
-// 8192 tokens (d 4096, f 11008) takes 1682 us against 1613-1650, with 4 1704.
+// 1000 W limit, so traffic costs clock. Back to back, groups of 16 against 8, in us at the
+// median SM clock: forward of 8192 tokens, d 4096, f 11008: 1621 at 1362 MHz / 1644 at
+// 1360; of 4096 tokens 835 at 1357 / 848 at 1392 (4 % fewer clocks); of 8192 tokens,
+// d 2048, f 5504: 441 at 1392 / 445 at 1383; backward of 4096 tokens 2327 at 1322 / 2323
+// at 1325.
 //
 // Its grid is persistent: whole tiles in turn, and where the last round would leave
 // most pairs idle, that round's tiles are cut along the contraction into equal
@@ -1339,11 +1342,18 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
   return cfg;
 }
 
-// Tokens up to which the weight-streaming kernel runs: the gated forms (at d 4096, f
-// 11008 and 100 tokens 45.6 us against the pair kernel's 50.0; from 129 on two of its
-// CTAs share an SM instead of three, and it is behind: d 1200, f 8000, 130 tokens 17.6
-// against 15.8), and the plain ones (160 tokens: 25.5 against 30.0, 11.1 against 11.4 at
-// d 1024, f 2816; 192 tokens at d 2048, f 5504: 27.7 against 15.6).
+// Tokens up to which the weight-streaming kernel runs. Past it the pair kernel's one row
+// tile holds all tokens and moves each weight as often, with more tokens to a load. The
+// gated forms, against the pair kernel, in us (up to 64 tokens three of its CTAs share an
+// SM, from 65 on two):
+//   tokens              65            100            128            144
+//   d 4096, f 11008     38.6 / 43.5   42.7 / 45.2    44.3 / 46.7    45.6 / 46.9
+//   d 2048, f 5504      14.5 / 16.1   16.5 / 16.3    17.2 / 16.4    17.7 / 16.4
+//   d 1024, f 2816       9.4 / 11.1   11.0 / 11.3    12.2 / 11.3    12.8 / 11.3
+//   d 1200, f 8000      12.2 / 12.6   14.1 / 12.7    15.3 / 12.9    16.2 / 12.9
+// so 128 is between the wide blocks' limit and the narrow ones', which is about 100. The
+// plain forms: 160 tokens, d 4096, f 11008: 25.5 / 30.0, d 1024, f 2816: 11.1 / 11.4; 192
+// tokens, d 2048, f 5504: 27.7 / 15.6.
 constexpr int64_t kSkinnyTokens = 128, kSkinnyTokensPlain = 160;
 constexpr size_t kJoinBytes = (size_t)kMaxPairs * 2 * kEpiWarps * kWarpPartial * 4;  // one piece a pair
 

@@ -73,15 +73,27 @@ struct Deal {
 
 // Tiles go in twos (one load of B for both: 96 instead of 128 KB of operands) where the
 // contraction is long enough to cover that both epilogues end together, and there are
-// rounds enough: in k-blocks and rounds of tiles. Measured against single tiles: 4096
-// tokens, d 4096, f 11008: gate and up 478 -> 467 us, backward 2000 -> 1945; but the
-// backward of 2048 tokens, d 2048, f 5504 (8 rounds) 285 -> 292, of 1024 tokens, d 4096
-// (16 k-blocks) 549 -> 559. The backward projection's epilogue is too long for it
-// (417 -> 472 thousand cycles).
+// rounds enough: in k-blocks and rounds of tiles. Measured against single tiles, one call
+// among idle ones: 4096 tokens, d 4096, f 11008: gate and up 478 -> 467 us, backward 2000
+// -> 1945; but the backward of 2048 tokens, d 2048, f 5504 (8 rounds) 285 -> 292, of 1024
+// tokens, d 4096 (16 k-blocks) 549 -> 559. Back to back, at the power limit, the gradients'
+// two limits matter less: 4 rounds instead of 16 gives 305 -> 310 and, for 8192 tokens,
+// d 1024, f 4096, 509 -> 492; 8 k-blocks instead of 32, of 1024 tokens, 621 -> 639; 2048
+// tokens, d 4096, f 11008 take 1180 whichever way. The backward projection's epilogue is
+// too long for it (417 -> 472 thousand cycles).
 constexpr int kTwosKb = 64, kTwosRounds = 2, kTwosKbGrads = 32, kTwosRoundsGrads = 16;
 // When a pair launch cuts its last round: pieces of at least kMinPieceKb k-blocks, at
-// most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time (16 instead of
-// 24: 1021 tokens, d 2048, f 5504, the gated form 41.1 -> 42.4 us, backward 163 -> 169).
+// most kMaxWays of them, for a gain of at least kMinSavedKb k-blocks' time, which covers
+// the partials and the join. In us, for a gain of 24, 16 and 8, and without cuts:
+//   gated, 1021 tokens, d 2048, f 5504     37.0   39.5   39.5   36.9
+//   backward of the same                  181    190    191    182
+//   forward, 256, 4096, 11008              78.7   78.2   78.9  109
+//   backward of the same                  244    244    245    240
+//   forward, 600, 4096, 11008             191    193    191    186
+//   forward, 777, 1024, 2816               31.0   31.0   34.8   34.5
+//   backward of the same                   64.5   64.5   70.9   64.7
+//   backward, 300, 1024, 4096              52.5   52.5   55.1   52.5
+//   backward, 1500, 1536, 4096            150    155    155    149
 constexpr int kMinPieceKb = 4, kMaxWays = 4, kMinSavedKb = 24;
 
 // One piece of work: k-blocks [k0, k1) of `count` tiles from row tile bm on, column
