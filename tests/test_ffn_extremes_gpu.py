@@ -125,3 +125,37 @@ def test_every_pass_past_32_bit_offsets(cuda, f):
         steps = turns * period / 16 * 2.0 ** -23
         ref.assert_close(a, turns * w, turns * (s + steps / 8 * (w.abs() + 8 * w.std())), name)
     ffn.check()
+
+
+@pytest.mark.parametrize("tokens", [4, 200])
+def test_weights_past_32_bit_offsets(cuda, tokens):
+    """2.16e9 elements in each weight and each weight gradient: y and dx over the whole
+    contraction, the weight gradients at the first, the last and the middle features."""
+    from morph_b200 import ffn
+    d, f, parts = 2056, 1_050_000, 50
+    assert d * f > 2 ** 31
+    g = torch.Generator(device=cuda).manual_seed(tokens)
+    r = lambda std, *s: torch.empty(*s, dtype=BF16, device=cuda).normal_(0, std, generator=g)  # noqa: E731
+    x, dy = r(1.0, tokens, d), r(0.5, tokens, d)
+    gate, up, down = r(d ** -0.5, f, d), r(d ** -0.5, f, d), r(f ** -0.5, d, f)
+    y = ffn.feed_forward(x, gate, up, down)
+    dx, dgate, dup, ddown = ffn.feed_forward_backward(dy, x, gate, up, down)
+    unit = 2.0 ** -9
+    want_y = sq_y = want_dx = sq_dx = 0
+    step = f // parts
+    for lo in range(0, f, step):
+        w = gate[lo:lo + step], up[lo:lo + step], down[:, lo:lo + step]
+        want_y = want_y + ref.forward(x, *w, "silu")
+        sq_y = sq_y + ref.forward_sigma(x, *w, "silu", unit) ** 2
+        want, sigmas = ref.backward(dy, x, *w, "silu")
+        s = sigmas(unit)
+        want_dx, sq_dx = want_dx + want[0], sq_dx + s[0] ** 2
+        if lo // step in (0, parts // 2, parts - 1):
+            ref.assert_close(dgate[lo:lo + step], want[1], s[1], "dgate")
+            ref.assert_close(dup[lo:lo + step], want[2], s[2], "dup")
+            ref.assert_close(ddown[:, lo:lo + step], want[3], s[3], "ddown")
+    # a part's sigma counts an FP32 sum of its own length: the whole one's is at most
+    # sqrt(parts) times the parts' together
+    ref.assert_close(y, want_y, (parts * sq_y).sqrt(), "y")
+    ref.assert_close(dx, want_dx, (parts * sq_dx).sqrt(), "dx")
+    ffn.check()
