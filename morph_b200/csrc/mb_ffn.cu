@@ -1349,10 +1349,10 @@ cudaLaunchConfig_t launch_config(cudaLaunchAttribute (&at)[2], int grid, int thr
 // gated forms, against the pair kernel, in us (up to 64 tokens three of its CTAs share an
 // SM, from 65 on two):
 //   tokens              65            100            128            144
-//   d 4096, f 11008     38.6 / 43.5   42.7 / 45.2    44.3 / 46.7    45.6 / 46.9
-//   d 2048, f 5504      14.5 / 16.1   16.5 / 16.3    17.2 / 16.4    17.7 / 16.4
-//   d 1024, f 2816       9.4 / 11.1   11.0 / 11.3    12.2 / 11.3    12.8 / 11.3
-//   d 1200, f 8000      12.2 / 12.6   14.1 / 12.7    15.3 / 12.9    16.2 / 12.9
+//   d 4096, f 11008     38.6 / 45.1   42.0 / 49.0    45.2 / 49.3    46.3 / 49.2
+//   d 2048, f 5504      14.7 / 16.7   16.1 / 16.2    16.8 / 16.3    17.4 / 16.2
+//   d 1024, f 2816       9.1 / 11.0   10.6 / 11.3    11.8 / 11.3    12.4 / 11.3
+//   d 1200, f 8000      11.8 / 12.4   13.7 / 12.5    14.9 / 12.7    15.8 / 12.6
 // so 128 is between the wide blocks' limit and the narrow ones', which is about 100. The
 // plain forms: 160 tokens, d 4096, f 11008: 25.5 / 30.0, d 1024, f 2816: 11.1 / 11.4; 192
 // tokens, d 2048, f 5504: 27.7 / 15.6.
