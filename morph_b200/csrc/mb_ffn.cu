@@ -1651,6 +1651,10 @@ int check_args(const mb_ffn_args* a, bool need_x, bool need_down) {
   return rc;
 }
 
+// A call's contractions, in k-blocks, are checked before its first launch: one that is
+// refused has written nothing.
+bool too_long(int64_t k, int nseg = 1) { return (k + BK - 1) / BK * nseg > kMaxKb; }
+
 Product gated_product(const mb_ffn_args* a, const Mat& x, const Mat& gate, const Mat& up) {
   Product q;
   q.epi = kGated;
@@ -1696,6 +1700,7 @@ static int forward(const mb_ffn_args* a, bool with_down, void* y, int64_t ldy, v
   if (rc != MB_OK) return rc;
   const int64_t T = a->tokens, d = a->d, f = a->f, width = with_down ? d : f;
   if (T == 0) return MB_OK;
+  if (too_long(d) || (with_down && too_long(f))) return MB_ERR_TOO_LARGE;
   rc = check_mat(y, width, ldy);
   if (rc != MB_OK) return rc;
   const size_t need = with_down ? mb_feed_forward_workspace_bytes(T, f) : mb_gated_linear_workspace_bytes(T);
@@ -1760,6 +1765,7 @@ MB_API int mb_feed_forward_backward(const mb_ffn_args* a, const mb_ffn_grads* r,
     return rc;
   }
   if (!r->dx && !r->dgate && !r->dup && !r->ddown) return MB_OK;
+  if (too_long(d) || (r->dx && too_long(f, 2)) || ((r->dgate || r->dup || r->ddown) && too_long(T))) return MB_ERR_TOO_LARGE;
   rc = check_mat(r->dy, with_down ? d : f, r->lddy);
   if (rc != MB_OK) return rc;
   if (from_codes && !r->scales) return MB_ERR_ARG;

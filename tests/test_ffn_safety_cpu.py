@@ -1,5 +1,6 @@
 """The feed-forward block and the activation checkpoints on a host without a GPU: what
 they refuse, what they ask for, and how their launches are dealt."""
+import ctypes
 import math
 import os
 import random
@@ -9,7 +10,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from morph_b200 import ffn
+from morph_b200 import _lib, ffn
 from morph_b200.precision import pack_activation
 
 BF16 = torch.bfloat16
@@ -133,3 +134,31 @@ def test_only_unaligned_matrices_ask_for_room():
     assert ffn._padding((0, 67, 0, 67)) == 0
     odd = _aligned(f, 65), _aligned(f, 65)
     assert ffn._args(0, tokens, 65, f, _aligned(tokens, 65), *odd, _aligned(65, f))[2] == area(tokens, 65) + 2 * area(f, 65)
+
+
+def test_too_long_contractions_are_refused_before_the_first_launch():
+    """Past 2^21 blocks of 64: in the backward pass only the last launch contracts over
+    tokens or over 2 f, and was refused after the others had run (without a device, a
+    launch fails with another status)."""
+    L = _lib.lib()
+    long = (1 << 27) + 1
+
+    def args(tokens, d, f):
+        return _lib.FfnArgs(_lib.MB_BF16, 0, tokens, d, f, 4096, d, 4096, d, 4096, d, 4096, f)
+
+    def forward(tokens, d, f):
+        a = args(tokens, d, f)
+        return (L.mb_feed_forward(ctypes.byref(a), 4096, d, 4096, 1 << 60, None),
+                L.mb_gated_linear(ctypes.byref(a), 4096, f, 4096, 1 << 60, None))
+
+    def backward(tokens, d, f, *wanted):
+        at = {n: 4096 for n in wanted}
+        r = _lib.FfnGrads(dy=4096, lddy=d, lddx=d, ld_dgate=d, ld_dup=d, ld_ddown=f, **at)
+        return L.mb_feed_forward_backward(ctypes.byref(args(tokens, d, f)), ctypes.byref(r), 4096, 1 << 60, None)
+    assert forward(300, long, 8) == (_lib.MB_ERR_TOO_LARGE,) * 2
+    assert forward(300, 8, long)[0] == _lib.MB_ERR_TOO_LARGE
+    assert backward(300, long, 8, "dx") == _lib.MB_ERR_TOO_LARGE
+    assert backward(300, 8, (long + 1) // 2, "dx") == _lib.MB_ERR_TOO_LARGE
+    for name in ("dgate", "dup", "ddown"):
+        assert backward(long, 8, 8, name) == _lib.MB_ERR_TOO_LARGE
+    assert backward(long, 8, 8) == _lib.MB_OK  # nothing asked
